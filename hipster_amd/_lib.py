@@ -50,6 +50,27 @@ class MoeTile(ctypes.Structure):
     _fields_ = [("expert", ctypes.c_int32), ("k0", ctypes.c_int32), ("ncols", ctypes.c_int32)]
 
 
+class XMX(ctypes.Structure):
+    """qmm_xmx: rows of MXFP4."""
+    _fields_ = [("q", c_vp), ("e", c_vp)]
+
+
+class RouteRule(ctypes.Structure):
+    """qmm_route_rule: how moe_route_groups chooses experts."""
+    _fields_ = [("bias", c_vp), ("scale", ctypes.c_float), ("score", ctypes.c_int32), ("groups", ctypes.c_int32), ("keep", ctypes.c_int32),
+                ("best", ctypes.c_int32), ("renorm", ctypes.c_int32), ("shared", ctypes.c_int32)]
+
+
+class Gate(ctypes.Structure):
+    """qmm_gate: the gate of a block's output."""
+    _fields_ = [("g", c_vp), ("ld", ctypes.c_size_t), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("per_value", ctypes.c_int32)]
+
+
+# element types (include/hipster_qmm.h)
+QMM_F32, QMM_BF16 = 0, 1
+
+_POSTNORM = [c_vp, c_vp, c_int, ctypes.c_size_t, c_vp, ctypes.POINTER(Gate), ctypes.c_float, c_vp, c_vp]
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "qmm_version": (ctypes.c_char_p, []),
@@ -116,6 +137,19 @@ SIGNATURES = {
     "qmm_add_rmsnorm_bf16": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, ctypes.c_float, c_vp]),
     "qmm_silu_mul_quant": (c_int, [c_vp, c_vp, XQ8, c_int, c_vp]),
     "qmm_silu_mul_bf16": (c_int, [c_vp, c_vp, c_vp, ctypes.c_size_t, c_vp]),
+    "qmm_quantize_mxfp4": (c_int, [c_vp, c_int, ctypes.c_size_t, XMX, c_int, c_int, c_vp]),
+    "qmm_dequant_mxfp4": (c_int, [XMX, c_vp, c_int, c_int, c_int, c_vp]),
+    "qmm_mxfp4_weight_bytes": (ctypes.c_size_t, [c_int, c_int]),
+    "qmm_pack_mxfp4": (c_int, [XMX, c_vp, c_int, c_int, c_vp]),
+    "qmm_repack_row_mxfp4": (c_int, [c_vp, c_vp, c_vp, c_int]),
+    "qmm_gemv_mxfp4": (c_int, [c_vp, XMX, c_vp, c_int, c_int, c_int, c_int, c_vp]),
+    "qmm_gemv_moe_mxfp4": (c_int, [c_vp, c_vp, ctypes.c_size_t, c_vp, XMX, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "qmm_gemm_mxfp4": (c_int, [c_vp, XMX, c_vp, c_int, c_int, c_int, c_int, c_vp]),
+    "qmm_moe_gemm_mxfp4": (c_int, [c_vp, c_vp, ctypes.c_size_t, c_vp, c_vp, c_int, c_vp, XMX, c_vp, c_int, c_int, c_int, c_vp]),
+    "qmm_moe_route_groups": (c_int, [c_vp, c_int, ctypes.POINTER(RouteRule), c_vp, c_vp, c_int, c_int, c_int, c_vp]),
+    "qmm_postnorm_add_rmsnorm_bf16": (c_int, _POSTNORM + [c_vp, c_int, c_int, ctypes.c_float, c_vp]),
+    "qmm_postnorm_add_rmsnorm_quant": (c_int, _POSTNORM + [c_vp, XQ8, c_int, c_int, ctypes.c_float, c_vp]),
+    "qmm_postnorm_add_rmsnorm_mxfp4": (c_int, _POSTNORM + [XMX, c_int, c_int, ctypes.c_float, c_vp]),
     "qmm_gemm_wq": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16_ld": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp]),

@@ -140,6 +140,24 @@ int qmm_repack_row_q5_0(const uint8_t* src, uint8_t* dst, int K) {
     return QMM_OK;
 }
 
+int qmm_repack_row_mxfp4(const uint8_t* src, uint8_t* q, uint8_t* e, int K) {
+    if (!src || !q || !e) return QMM_ERR_NULL;
+    if (K <= 0 || K % 32 != 0) return QMM_ERR_SHAPE;
+    const size_t steps = ((size_t)K + 127) / 128, nb = (size_t)K / 32;
+    memset(q + nb * 16, 0, steps * 64 - nb * 16);
+    memset(e + nb, 0, steps * 4 - nb);
+    for (size_t b = 0; b < nb; ++b) {
+        const uint8_t* blk = src + b * 17;
+        e[b] = blk[0];
+        for (int i = 0; i < 8; ++i) {      // weights 2i, 2i + 1 are the low halves, 16 + 2i, 17 + 2i the high ones
+            const uint8_t u = blk[1 + 2 * i], v = blk[2 + 2 * i];
+            q[b * 16 + i] = (uint8_t)((u & 15) | (v << 4));
+            q[b * 16 + 8 + i] = (uint8_t)((u >> 4) | (v & 0xf0));
+        }
+    }
+    return QMM_OK;
+}
+
 }  // extern "C"
 
 namespace {

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import GemvSeg, MoeSegs, MoeTile, QmmError, XQ8, XQ8K, check  # noqa: F401
+from ._lib import Gate, GemvSeg, MoeSegs, MoeTile, QmmError, RouteRule, XMX, XQ8, XQ8K, check  # noqa: F401
 
 WFmt = type("WFmt", (), {"Q4_K": _lib.QMM_Q4_K, "Q5_K": _lib.QMM_Q5_K, "IQ4_XS": _lib.QMM_IQ4_XS,
                          "Q6_K_SOA": _lib.QMM_Q6_K_SOA, "Q8_0_SOA": _lib.QMM_Q8_0_SOA,
@@ -380,3 +380,223 @@ def moe_gemm(fmt, shared_fmt, W, Wsh, ebytes, tiles, ntiles, stiles, nstiles, ct
     tiles[:ntiles] and shared tiles stiles[:nstiles] with host counts; y[k][N] f32, the q8 arithmetic."""
     check(_lib.lib().qmm_moe_gemm_q8(fmt, shared_fmt, _p(W), _p(Wsh), ebytes, _p(tiles), ntiles, _p(stiles), nstiles, ct,
                                      _p(rowtab), x.c(), _p(y), N, K, _stream(stream)), "moe_gemm")
+
+
+# ---- MXFP4 decoder blocks ----
+_DTYPE = {torch.float32: _lib.QMM_F32, torch.bfloat16: _lib.QMM_BF16}
+
+
+def _dtype(t, name):
+    if t.dtype not in _DTYPE:
+        raise QmmError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    return _DTYPE[t.dtype]
+
+
+def _here(t, name):
+    """t lies on the current device: the library launches there, on its current stream."""
+    if t.device.index != torch.cuda.current_device():
+        raise QmmError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _room(t, n, name):
+    """t is a contiguous tensor of at least n elements on the current device."""
+    _dev(t, None, name)
+    _here(t, name)
+    if t.numel() < n:
+        raise QmmError(f"{name} holds {t.numel()} elements, {n} are needed")
+    return t
+
+
+def _rows_of(t, n, name):
+    """Row stride of t, a device tensor [rows][n] (or one row [n]) whose rows are contiguous."""
+    if t is None or not t.is_cuda:
+        raise QmmError(f"{name} must be a CUDA tensor")
+    _here(t, name)
+    if t.dim() not in (1, 2) or t.shape[-1] != n or (n > 1 and t.stride(-1) != 1):
+        raise QmmError(f"{name} must be rows of {n} contiguous values, got shape {tuple(t.shape)}, strides {tuple(t.stride())}")
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < n:
+        raise QmmError(f"{name}: rows overlap (stride {t.stride(0)}, {n} values)")
+    return t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else n
+
+
+def _rows_match(t, rows, name):
+    have = t.shape[0] if t.dim() == 2 else 1
+    if have < rows:
+        raise QmmError(f"{name} has {have} rows, {rows} are needed")
+
+
+def mxfp4_steps(K):
+    """Steps of 128 values that a row of K takes."""
+    return -(-K // 128)
+
+
+class XMXBuf:
+    """Device buffers of rows of MXFP4: q [rows][64 per step of 128] uint8, e [rows][4 per step] uint8."""
+
+    def __init__(self, rows, K, device="cuda"):
+        self.rows, self.K = rows, K
+        self.q = torch.zeros((rows, 64 * mxfp4_steps(K)), dtype=torch.uint8, device=device)
+        self.e = torch.zeros((rows, 4 * mxfp4_steps(K)), dtype=torch.uint8, device=device)
+
+    def c(self):
+        return XMX(self.q.data_ptr(), self.e.data_ptr())
+
+
+def _xmx(x, rows, K, name):
+    if x.rows < rows or mxfp4_steps(x.K) != mxfp4_steps(K):
+        raise QmmError(f"{name} holds {x.rows} rows of {x.K} values, {rows} of {K} are needed")
+    return x.c()
+
+
+def quantize_mxfp4(x, out, rows, K, stream=None):
+    """x f32 or bf16 [rows][K] (rows may be strided) -> out (XMXBuf): blocks of 32, scale 2^(floor(log2 amax) - 2),
+    codes rounded to nearest even."""
+    ld = _rows_of(x, K, "x")
+    _rows_match(x, rows, "x")
+    check(_lib.lib().qmm_quantize_mxfp4(_p(x), _dtype(x, "x"), ld, _xmx(out, rows, K, "out"), rows, K, _stream(stream)), "quantize_mxfp4")
+
+
+def dequant_mxfp4(x, out, rows, K, stream=None):
+    """The values of x (XMXBuf) into out [rows][K], f32 or bf16 (exact in both)."""
+    _room(out, rows * K, "out")
+    check(_lib.lib().qmm_dequant_mxfp4(_xmx(x, rows, K, "x"), _p(out), _dtype(out, "out"), rows, K, _stream(stream)), "dequant_mxfp4")
+
+
+def mxfp4_weight_bytes(N, K):
+    """Bytes of a packed MXFP4 weight of N rows of K values."""
+    return _lib.lib().qmm_mxfp4_weight_bytes(N, K)
+
+
+def pack_mxfp4(q, e, W, N, K, stream=None):
+    """MXFP4 rows q [N][64 per step], e [N][4 per step] (an XMXBuf's tensors) -> W, the layout the products read."""
+    for t, per, name in ((q, 64, "q"), (e, 4, "e")):
+        _dev(t, torch.uint8, name)
+        if t.numel() != N * per * mxfp4_steps(K):
+            raise QmmError(f"{name} must hold {N} rows of {per * mxfp4_steps(K)} bytes")
+    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W")
+    check(_lib.lib().qmm_pack_mxfp4(XMX(q.data_ptr(), e.data_ptr()), _p(W), N, K, _stream(stream)), "pack_mxfp4")
+
+
+def repack_row_mxfp4(src, K):
+    """Host: one GGUF row of MXFP4 blocks (bytes) -> (q, e) bytes of one MXFP4 row."""
+    import numpy as np
+    src = np.ascontiguousarray(src, dtype=np.uint8)
+    if K > 0 and src.size != K // 32 * 17:
+        raise QmmError(f"a GGUF MXFP4 row of {K} weights has {K // 32 * 17} bytes, got {src.size}")
+    q, e = np.empty(64 * mxfp4_steps(K), np.uint8), np.empty(4 * mxfp4_steps(K), np.uint8)
+    check(_lib.lib().qmm_repack_row_mxfp4(src.ctypes.data, q.ctypes.data, e.ctypes.data, K), "repack_row_mxfp4")
+    return q, e
+
+
+def gemv_mxfp4(W, x, y, ncol, N, K, stream=None):
+    """y[m][n] = W[n] . x[m] for m < ncol <= 64 (x an XMXBuf, y f32 or bf16 [ncol][N])."""
+    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W"); _room(y, ncol * N, "y")
+    check(_lib.lib().qmm_gemv_mxfp4(_p(W), _xmx(x, ncol, K, "x"), _p(y), _dtype(y, "y"), ncol, N, K, _stream(stream)), "gemv_mxfp4")
+
+
+def gemm_mxfp4(W, x, D, M, N, K, stream=None):
+    """D[m][n] = W[n] . x[m] for any M (x an XMXBuf, D f32 or bf16 [M][N])."""
+    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W"); _room(D, M * N, "D")
+    check(_lib.lib().qmm_gemm_mxfp4(_p(W), _xmx(x, M, K, "x"), _p(D), _dtype(D, "D"), M, N, K, _stream(stream)), "gemm_mxfp4")
+
+
+def _experts(W, Wsh, ebytes, nexperts, N, K):
+    one = mxfp4_weight_bytes(N, K)
+    _dev(W, torch.uint8, "W"); _room(W, (nexperts - 1) * ebytes + one, "W")
+    if Wsh is not None:
+        _dev(Wsh, torch.uint8, "Wsh"); _room(Wsh, one, "Wsh")
+
+
+def gemv_moe_mxfp4(W, Wsh, ebytes, ids, x, y, T, nslot, nexperts, N, K, xrow_te=False, stream=None):
+    """y[te][n] = W_{ids[te]}[n] . x[te if xrow_te else t] for T <= 16 tokens (ids int32 [T][nslot], below 0: Wsh)."""
+    _experts(W, Wsh, ebytes, nexperts, N, K)
+    _dev(ids, torch.int32, "ids"); _room(ids, T * nslot, "ids"); _room(y, T * nslot * N, "y")
+    check(_lib.lib().qmm_gemv_moe_mxfp4(_p(W), _p(Wsh), ebytes, _p(ids), _xmx(x, T * nslot if xrow_te else T, K, "x"), _p(y), _dtype(y, "y"), T, nslot,
+                                        nexperts, N, K, int(xrow_te), _stream(stream)), "gemv_moe_mxfp4")
+
+
+def moe_gemm_mxfp4(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, N, K, stream=None):
+    """D[k] = W_e . x[rowtab[k]] over rows sorted by expert (moe_sort's tiles, counts, rowtok; rowtab None: x[k])."""
+    _dev(W, torch.uint8, "W"); _dev(tiles, torch.int32, "tiles"); _room(tiles, 3 * max_tiles, "tiles")
+    _dev(counts, torch.int32, "counts"); _room(counts, 2, "counts"); _dev(D, None, "D")
+    if rowtab is not None:
+        _dev(rowtab, torch.int32, "rowtab")
+    check(_lib.lib().qmm_moe_gemm_mxfp4(_p(W), _p(Wsh), ebytes, _p(tiles), _p(counts), max_tiles, _p(rowtab), _xmx(x, 0, K, "x"), _p(D), _dtype(D, "D"),
+                                        N, K, _stream(stream)), "moe_gemm_mxfp4")
+
+
+_SCORE = {"softmax": 0, "sigmoid": 1}
+_SHARED = {None: 0, "gate": 1, "one": 2}
+
+
+def moe_route_groups(logits, ids, w, T, nexp, topk, score="softmax", bias=None, groups=1, keep=1, best=1, renorm=True, scale=1.0, shared=None,
+                     stream=None):
+    """Experts of each token: scores (softmax or sigmoid of logits [T][>= nexp]), plus bias for the choice, the `keep`
+    best of `groups` groups (by their `best` = 1 or 2 largest), the topk experts of those (ties to the lower id);
+    weights: the scores, renormalised if renorm, times scale.  shared: None, "gate" (logit nexp's sigmoid) or "one",
+    a last slot of id -1.  ids int32, w f32 [T][topk (+ 1)]."""
+    _dev(logits, torch.float32, "logits"); _dev(ids, torch.int32, "ids"); _dev(w, torch.float32, "w")
+    if score not in _SCORE or shared not in _SHARED:
+        raise QmmError(f"score {score!r}, shared {shared!r}: softmax or sigmoid; None, 'gate' or 'one'")
+    slots = topk + (shared is not None)
+    _room(logits, T * logits.shape[-1], "logits"); _room(ids, T * slots, "ids"); _room(w, T * slots, "w")
+    if bias is not None:
+        _dev(bias, torch.float32, "bias"); _room(bias, nexp, "bias")
+    rule = RouteRule(None if bias is None else bias.data_ptr(), scale, _SCORE[score], groups, keep, best, int(renorm), _SHARED[shared])
+    check(_lib.lib().qmm_moe_route_groups(_p(logits), logits.shape[-1], ctypes.byref(rule), _p(ids), _p(w), T, nexp, topk, _stream(stream)),
+          "moe_route_groups")
+
+
+_ACT = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
+def _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n):
+    """The leading arguments of the postnorm_add_rmsnorm calls."""
+    _dev(x, torch.float32, "x"); _room(x, T * n, "x"); _dev(w, torch.float32, "w"); _room(w, n, "w")
+    ldy = _rows_of(y, n, "y")
+    _rows_match(y, T, "y")
+    if wy is not None:
+        _dev(wy, torch.float32, "wy"); _room(wy, n, "wy")
+    xo = x if xo is None else xo
+    _dev(xo, torch.float32, "xo"); _room(xo, T * n, "xo")
+    g = Gate(None, 0, 0, 0, 0)
+    if act not in _ACT:
+        raise QmmError(f"act {act!r}: none, sigmoid or silu")
+    if gate is not None:
+        if gate.dim() == 2 and gate.shape[1] == 1 and n > 1:                 # one value per token
+            _rows_match(gate, T, "gate")
+            if not gate.is_cuda:
+                raise QmmError("gate must be a CUDA tensor")
+            _here(gate, "gate")
+            ld, per = gate.stride(0), 0
+        else:
+            ld, per = _rows_of(gate, n, "gate"), 1
+            if gate.dim() == 1:                                              # one row for every token
+                ld = 0
+            else:
+                _rows_match(gate, T, "gate")
+        g = Gate(gate.data_ptr(), ld, _dtype(gate, "gate"), _ACT[act], per)
+    return [_p(x), _p(y), _dtype(y, "y"), ldy, _p(wy), ctypes.byref(g), alpha, _p(xo), _p(w)]
+
+
+def postnorm_add_rmsnorm_bf16(x, y, wy, w, xb, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
+    """Between two blocks, per row: p = rmsnorm(y) * wy (wy None: y), p *= act(gate), xo = x + alpha * p (xo None: in
+    place), xb = bf16(rmsnorm(xo) * w).  y f32 or bf16 rows; gate f32 or bf16 [T][1], [n] or [T][n]."""
+    a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
+    _dev(xb, torch.bfloat16, "xb"); _room(xb, T * n, "xb")
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_bf16(*a, _p(xb), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_bf16")
+
+
+def postnorm_add_rmsnorm_quant(x, y, wy, w, xn, xq, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
+    """The same with xn = rmsnorm(xo) * w in f32 and its q8 in xq (XQ8Buf of T x n); n % 32 == 0."""
+    a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
+    _dev(xn, torch.float32, "xn"); _room(xn, T * n, "xn")
+    if xq.ncol < T or xq.K != n:
+        raise QmmError(f"xq holds {xq.ncol} rows of {xq.K} values, {T} of {n} are needed")
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_quant(*a, _p(xn), xq.c(), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_quant")
+
+
+def postnorm_add_rmsnorm_mxfp4(x, y, wy, w, xq, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
+    """The same with rmsnorm(xo) * w as MXFP4 rows (XMXBuf of T x n)."""
+    a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_mxfp4(*a, _xmx(xq, T, n, "xq"), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_mxfp4")

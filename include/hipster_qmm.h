@@ -78,6 +78,27 @@ typedef struct { int32_t expert, k0, ncols; } qmm_moe_tile;
  * of each 32 (reference: XQ8K, gemv.h:33) */
 typedef struct { int8_t* q; float* d; int16_t* bs; } qmm_xq8k;
 
+/* element types of activations and outputs, where an entry point takes more than one */
+enum { QMM_F32 = 0, QMM_BF16 = 1 };
+/* rows of MXFP4 (OCP microscaling: blocks of 32 e2m1 codes and one E8M0 scale byte, 2^(byte - 127), 255 = NaN),
+ * K padded to K128 = ceil(K / 128) steps of 128 values with code 0, scale byte 0: q [rows][K128][64] (value 2i of a
+ * step in the low half of its byte i, value 2i + 1 in the high half), e [rows][K128][4] */
+typedef struct { uint8_t* q; uint8_t* e; } qmm_xmx;
+/* how qmm_moe_route_groups chooses experts */
+typedef struct {
+    const float* bias; /* [nexp] added to the scores for the choice only; NULL: none */
+    float scale;       /* factor of the weights */
+    int32_t score;     /* 0 softmax over the experts, 1 sigmoid of each logit */
+    int32_t groups;    /* equal groups of successive experts (1: none) ... */
+    int32_t keep;      /* ... of which this many stay ... */
+    int32_t best;      /* ... by the sum of their 1 or 2 largest choice values */
+    int32_t renorm;    /* 1: weights are divided by their sum */
+    int32_t shared;    /* slot topk: 0 none; 1 the shared expert, weight sigmoid(logit[nexp]); 2 with weight 1 */
+} qmm_route_rule;
+/* a block's gate: values act(g), act 0 none, 1 sigmoid, 2 silu; per_value 0: one value per token at g[t * ld];
+ * 1: n values per token at g + t * ld (ld 0: the same n for every token) */
+typedef struct { const void* g; size_t ld; int32_t dtype, act, per_value; } qmm_gate;
+
 /* ---- GGUF (the on-disk format of the weights; reference: engine/src/gguf.h, gguf.cpp) ---- */
 /* ggml tensor types (the reference's GType numbering, gguf.h:12-17) */
 enum {
@@ -387,6 +408,58 @@ int qmm_add_rmsnorm_bf16(float* x, const float* y, const float* w, uint16_t* xb,
 int qmm_silu_mul_quant(const float* gate, const float* up, qmm_xq8 xq, int n, void* stream);
 /* out = bf16(silu(gate) * up), n elements (reference: silu_mul_bf16, ops.h:20, ops.hip:131,765) */
 int qmm_silu_mul_bf16(const float* gate, const float* up, uint16_t* out, size_t n, void* stream);
+
+/* ---- MXFP4 decoder blocks (no reference counterpart) ---- */
+/* rows of x (dtype QMM_F32 or QMM_BF16, row stride ldx >= K values) -> MXFP4.  A block's scale is 2^E,
+ * E = max(floor(log2 amax) - 2, -127); a code is x * 2^-E rounded to nearest, ties to even, saturating at 6.  A block
+ * with a NaN or an infinity gets scale byte 255 (NaN).  Any K >= 1 up to 2^24 (values past K count as 0); x needs
+ * its type's alignment only (16-byte rows are read 16 bytes at a time), out.q 16 bytes, out.e 4. */
+int qmm_quantize_mxfp4(const void* x, int dtype, size_t ldx, qmm_xmx out, int rows, int K, void* stream);
+/* the values that rows of MXFP4 hold, [rows][K] f32 or bf16 (both exact) */
+int qmm_dequant_mxfp4(qmm_xmx x, void* out, int dtype, int rows, int K, void* stream);
+/* bytes of a packed weight of N rows of K values: whole strips of 16 rows (0: N or K out of range).  A strip holds
+ * 16 rows whole, so weights of N % 16 == 0 rows joined end to end are the packed joined weight. */
+size_t qmm_mxfp4_weight_bytes(int N, int K);
+/* N MXFP4 rows -> the packed layout of the products below (on the device, once per weight; W 16-byte aligned) */
+int qmm_pack_mxfp4(qmm_xmx rows, void* W, int N, int K, void* stream);
+/* one GGUF row of MXFP4 blocks (17 bytes per 32 weights: the scale byte, then 16 bytes with weight i in the low
+ * and weight i + 16 in the high half) -> q and e of one qmm_xmx row, padding included; host only, K % 32 == 0 */
+int qmm_repack_row_mxfp4(const uint8_t* src, uint8_t* q, uint8_t* e, int K);
+/* y[m][n] = W[n] . x[m] for m < ncol <= 64, y [ncol][N] f32 or bf16 (dtype), W packed: decode and draft
+ * verification.  Products and block scales are exact, sums f32 in an order set by K alone: a row's bits do not
+ * depend on ncol or N.  Any N, K. */
+int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K, void* stream);
+/* the same for the experts of T <= 16 tokens: slot te = t * nslot + s uses expert ids[te] (W + id * ebytes, a packed
+ * weight of N rows; below 0: Wsh, or expert 0 where Wsh is NULL; beyond the last: the last), x row te if xrow_te,
+ * else t; y [T * nslot][N].  An expert is read once for all its slots.  nslot <= 16; ebytes % 16 == 0.  A slot's
+ * row has the bits of qmm_gemv_mxfp4. */
+int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int* ids, qmm_xmx x, void* y, int dtype, int T, int nslot, int nexperts,
+                       int N, int K, int xrow_te, void* stream);
+/* D[m][n] = W[n] . x[m] for any number of rows, D [M][N] f32 or bf16: prompts.  An output is one chain of matrix
+ * instructions over K: its bits do not depend on M or N (they differ from qmm_gemv_mxfp4's, which cuts K). */
+int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K, void* stream);
+/* the same for rows sorted by expert (qmm_moe_sort): for tile i < counts[0] + counts[1] (read on the device) and
+ * r < ncols: D[k0 + r] = W_e . x[rowtab ? rowtab[k0 + r] : k0 + r], W_e at W + expert * ebytes, or Wsh (W where it
+ * is NULL) for expert -1.  max_tiles bounds the grid.  A row has the bits of qmm_gemm_mxfp4. */
+int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
+                       qmm_xmx x, void* D, int dtype, int N, int K, void* stream);
+/* Experts of each token from logits [T][stride] by rule (above): ids / w [T][topk + (shared != 0)] in falling order of
+ * the choice value, ties to the lower id.  Scores and comparisons are in 64 bits, a weight is rounded once.  An
+ * expert whose logit is -inf or NaN is never chosen; a slot without an expert gets id -1, weight 0.
+ * nexp <= 1024, topk <= 16, groups <= 64 dividing nexp, topk <= keep * (nexp / groups), stride >= nexp (+ 1 for
+ * shared 1). */
+int qmm_moe_route_groups(const float* logits, int stride, const qmm_route_rule* rule, int* ids, float* w, int T, int nexp, int topk, void* stream);
+/* Between two blocks, per row t < T (n <= 16384):  p = y / rms(y) * wy (wy NULL: p = y);  p *= act(gate) (gate or
+ * gate->g NULL: 1);  xo = x + alpha * p;  xn = xo / rms(xo) * w, rms(v) = sqrt(mean(v^2) + eps).  x, xo, w, wy f32;
+ * xo may be x; y f32 or bf16 with row stride ldy >= n.  xn goes out as bf16 (any n), ... */
+int qmm_postnorm_add_rmsnorm_bf16(const float* x, const void* y, int y_dtype, size_t ldy, const float* wy, const qmm_gate* gate, float alpha,
+                                  float* xo, const float* w, uint16_t* xb, int T, int n, float eps, void* stream);
+/* ... as f32 and q8 per 32 of it (n % 32 == 0; xq.ds filled when given), ... */
+int qmm_postnorm_add_rmsnorm_quant(const float* x, const void* y, int y_dtype, size_t ldy, const float* wy, const qmm_gate* gate, float alpha,
+                                   float* xo, const float* w, float* xn, qmm_xq8 xq, int T, int n, float eps, void* stream);
+/* ... or as MXFP4 rows, the codes that qmm_quantize_mxfp4 gives for the f32 xn (any n) */
+int qmm_postnorm_add_rmsnorm_mxfp4(const float* x, const void* y, int y_dtype, size_t ldy, const float* wy, const qmm_gate* gate, float alpha,
+                                   float* xo, const float* w, qmm_xmx xq, int T, int n, float eps, void* stream);
 
 #ifdef __cplusplus
 }
