@@ -52,6 +52,16 @@ __device__ __forceinline__ mx_v4f mx_mfma(const uint4& w, const uint4& a, mx_v4f
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vw, va, acc, kMxFp4, kMxFp4, BW, (int)sw, 0, (int)sa);
 }
 
+// the same on 32 x 32 x 64: lane l supplies row l % 32, block l / 32 of a half step; byte BW of sw, byte BA of sa;
+// acc[e] of lane l: weight row 8 (e / 4) + 4 (l / 32) + e % 4, activation row l % 32
+typedef float mx_v16f __attribute__((ext_vector_type(16)));
+template <int BW, int BA>
+__device__ __forceinline__ mx_v16f mx_mfma32(const uint4& w, const uint4& a, mx_v16f acc, uint32_t sw, uint32_t sa) {
+    const mx_v8i vw = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
+    const mx_v8i va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vw, va, acc, kMxFp4, kMxFp4, BW, (int)sw, BA, (int)sa);
+}
+
 // two values rounded to bf16 (to nearest even; NaN stays NaN), the first in the low half
 __device__ __forceinline__ uint32_t mx_bf16x2(float lo, float hi) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -5,12 +5,12 @@
 //   qmm_gemm_mxfp4       any number of rows: prompts
 //   qmm_moe_gemm_mxfp4   rows sorted by expert (qmm_moe_sort)
 //
-// One v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 weight rows by 16 activation rows over 128 values with
-// their block scales and adds to f32.  The weight is its first operand, so a lane ends with four successive
-// outputs of one activation row.
+// A scaled matrix instruction multiplies weight rows by activation rows with their block scales and adds to
+// f32: 16 x 16 over 128 values in the GEMV (few rows), 32 x 32 over 64 in the GEMM (6.4 PFLOP/s measured from
+// registers against 5.4 for the former: it reads half the operand bytes per product).  The weight is the first
+// operand, so a lane ends with four successive outputs of one activation row.
 //
-// Order of sums.  GEMM: an output is one chain of these instructions over K, whatever the tile, M or N.
-// GEMV: K's groups of four steps are cut into S contiguous runs, S chosen by K alone; each run is one chain
+// Order of sums.  GEMM: an output is one chain of instructions over K, whatever the tile, M or N.  GEMV: K's groups of four steps are cut into S contiguous runs, S chosen by K alone; each run is one chain
 // and the S sums are added in order.  So an output's bits depend on its own rows and K, not on the call.
 #include "mx.hpp"
 
@@ -183,170 +183,293 @@ __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uin
 }
 
 // ------------------------------------------------------------------------------------------
-// GEMM tile.  Four waves, WM of them along the rows: a wave owns 16 MF activation rows and NF strips.  A's
-// rows are staged two steps (128 bytes a row) at a time through registers into LDS, double buffered, in
-// 16-byte chunks at chunk ^ swz(row): both the row-wise writes and the operand reads (16 rows, one chunk) then
-// spread over the banks.  Weights go straight from memory to the operand registers, one step ahead: a strip
-// is read by one wave (WM = 1), so LDS would only add traffic.
+// GEMM tile, on v_mfma_scale_f32_32x32x64_f8f6f4.  WM x WN waves; a wave owns 32 MF activation rows and 32 NF
+// weight rows.  Both operands come by DMA (global_load_lds):
+//   - activations two steps (a pair, 128 bytes of a row: whole cache lines) at a time into NA buffers, 16-byte
+//     chunk c of a row at chunk c ^ swz(row).  Half lines, one step at a time, cost the vector cache a stall for
+//     every second half (the line is still on its way): half of all cycles, 155 instead of XX us below;
+//   - weights step by step into a ring of NS, a strip's kilobyte as it is in memory;
+//   - block scales by groups of four steps, 16 bytes a row, into two buffers.
+// The operand reads (16 lanes: 16 rows, one chunk) are free of bank conflicts.  A step k is: wait until the own
+// DMAs that it reads have landed, barrier, start those NS - 1 steps (pairs: NA - 1 pairs) ahead, whose buffers were
+// read before that barrier, multiply.
 __device__ __forceinline__ int a_swz(int row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
 
-template <int MF, int NF, int WM>
+template <int MF, int NF, int WM, int WN, int NS, int NA>
 struct MxTile {
-    static constexpr int kRows = 16 * MF * WM, kWN = 4 / WM, kCols = 16 * NF * kWN;
-    static constexpr int kChunks = (kRows * 8 + 255) / 256;       // 16-byte pieces of a stage per thread
-    static constexpr int kCodes = kRows * 128, kStage = kCodes + kRows * 8;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kWaves = WM * WN, kRows = 32 * MF * WM, kCols = 32 * NF * WN;
+    static constexpr int per(int pieces) { return (pieces + kWaves - 1) / kWaves; }
+    // DMAs (1 KB each): of a pair's activations, of a step's weights, of a group's scales; and per wave
+    static constexpr int kAPieces = kRows / 8, kWPieces = kCols / 16, kRowSc = (kRows + 63) / 64, kScPieces = kRowSc + (kCols + 63) / 64;
+    static constexpr int PA = per(kAPieces), PW = per(kWPieces), PS = per(kScPieces);
+    static constexpr int kABytes = kAPieces * 1024, kWBytes = kWPieces * 1024, kScBytes = kScPieces * 1024;
+    static constexpr int kWAt = NA * kABytes, kScAt = kWAt + NS * kWBytes, kLoopLds = kScAt + 2 * kScBytes;
+    static constexpr int kStoreLds = kWaves * 32 * (128 * NF + 16), kLds = kLoopLds > kStoreLds ? kLoopLds : kStoreLds;
+    // what a wave issues in step j (mod 4): scales of the next group, a pair, a step of weights, in this order
+    static constexpr int issued(int j) { return PW + ((j & 1) == 0 ? PA : 0) + ((j & 3) == 0 ? PS : 0); }
+    static constexpr int issued(int from, int to) { return from > to ? 0 : issued(from) + issued(from + 1, to); }
+    // DMAs younger than those that step k (mod 4, plus a multiple of 4) reads
+    static constexpr int younger(int k) {
+        const int w = issued(k - NS + 2, k - 1), a = PW + issued(k - 2 * (NA - 1) + 1, k - 1);
+        return (k & 1) == 0 && a < w ? a : w;
+    }
+    static_assert(NS >= 3 && NS <= 4 && NA >= 2 && NA <= 3, "the waits below hold for these");
 };
 
-// rows(r): the activation row of tile row r.  acc[f][j]: strip f, activation rows 16 j.. of this wave
-template <int MF, int NF, int WM, class Rows>
-__device__ __forceinline__ void mx_tile(uint8_t* smem, const uint8_t* W, qmm_xmx x, int strip0, int nstrips, int K128, Rows rows, mx_v4f (&acc)[NF][MF]) {
-    using T = MxTile<MF, NF, WM>;
+// s_waitcnt vmcnt(n)
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+    static_assert(N >= 0 && N < 64, "vmcnt has six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <int I, int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
+
+// rows(r): the activation row of tile row r.  acc[f][j]: weight rows 32 f.., activation rows 32 j.. of this wave
+template <int MF, int NF, int WM, int WN, int NS, int NA, class Rows>
+__device__ __forceinline__ void mx_tile(uint8_t* smem, const uint8_t* W, qmm_xmx x, int strip0, int nstrips, int K128, Rows rows, mx_v16f (&acc)[NF][MF]) {
+    using T = MxTile<MF, NF, WM, WN, NS, NA>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wn = wave % T::kWN, wm = wave / T::kWN;
-    const int G = mx_groups(K128);
-    const uint8_t* strip[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) strip[f] = W + (size_t)min(strip0 + wn * NF + f, nstrips - 1) * mx_strip_bytes(K128);
-    const uint32_t sc0 = (uint32_t)K128 * 1024u;
+    const int wn = wave % WN, wm = wave / WN, half = lane >> 5;
+    const uint32_t lds = lds_addr(smem);
 
-    // staging: piece i of this thread is chunk (tid + 256 i) % 8 of row (tid + 256 i) / 8
-    const uint8_t* qp[T::kChunks];
-    const int cj = tid & 7;
+    // this wave's pieces (where the waves do not divide them, the last one is fetched more than once): eight
+    // activation rows, a strip, 64 rows' scales (16 bytes; the last group of a row starts at step K128 - 4, so that
+    // it ends with the row) or four strips' scales (256 bytes)
+    const uint8_t* ap[T::PA];
+    uint32_t adst[T::PA];
+    bool late[T::PA];                                    // the lane's chunk is of the pair's second step
 #pragma unroll
-    for (int i = 0; i < T::kChunks; ++i) qp[i] = x.q + (size_t)rows(min((tid + 256 * i) >> 3, T::kRows - 1)) * K128 * 64 + (cj & 3) * 16;
-    const uint8_t* ep = x.e + (size_t)rows(min(tid, T::kRows - 1)) * K128 * 4;
-    uint4 pa[T::kChunks];
-    uint32_t pe[2];
-    auto fetch = [&](int st) {
-        const uint32_t kt = (uint32_t)min(2 * st + (cj >> 2), K128 - 1);
+    for (int i = 0; i < T::PA; ++i) {
+        const int p = min(wave + i * T::kWaves, T::kAPieces - 1), r = 8 * p + (lane >> 3), c = (lane & 7) ^ a_swz(r);
+        adst[i] = lds + (uint32_t)p * 1024u;
+        ap[i] = x.q + (size_t)rows(r) * K128 * 64 + c * 16;
+        late[i] = c >= 4;
+    }
+    const uint8_t* wp[T::PW];
+    uint32_t wdst[T::PW];
 #pragma unroll
-        for (int i = 0; i < T::kChunks; ++i) pa[i] = ld16(qp[i] + kt * 64u);
-        if (tid < T::kRows) {
-            pe[0] = *(const uint32_t*)(ep + (uint32_t)min(2 * st, K128 - 1) * 4u);
-            pe[1] = *(const uint32_t*)(ep + (uint32_t)min(2 * st + 1, K128 - 1) * 4u);
-        }
+    for (int i = 0; i < T::PW; ++i) {
+        const int p = min(wave + i * T::kWaves, T::kWPieces - 1);
+        wdst[i] = lds + T::kWAt + (uint32_t)p * 1024u;
+        wp[i] = W + (size_t)min(strip0 + p, nstrips - 1) * mx_strip_bytes(K128) + lane * 16;
+    }
+    const uint8_t* sp[T::PS];
+    uint32_t sdst[T::PS];
+    bool srow[T::PS];
+#pragma unroll
+    for (int i = 0; i < T::PS; ++i) {
+        const int p = min(wave + i * T::kWaves, T::kScPieces - 1);
+        sdst[i] = lds + T::kScAt + (uint32_t)p * 1024u;
+        srow[i] = p < T::kRowSc;
+        if (srow[i]) sp[i] = x.e + (size_t)rows(min(64 * p + lane, T::kRows - 1)) * K128 * 4;
+        else sp[i] = W + (size_t)min(strip0 + min(4 * (p - T::kRowSc) + (lane >> 4), T::kCols / 16 - 1), nstrips - 1) * mx_strip_bytes(K128) +
+                     (uint32_t)K128 * 1024u + (lane & 15) * 16;
+    }
+    auto issue_a = [&](int i, int pair, int buf) {       // piece i of a pair
+        const bool odd = 2 * pair + 1 >= K128;           // the pair's second step does not exist: the first again
+        dma16(ap[i] - (odd && late[i] ? 64 : 0), adst[i] + buf * T::kABytes);
+        ap[i] += 128;
     };
-    auto put = [&](int buf) {
-        uint8_t* d = smem + buf * T::kStage;
-#pragma unroll
-        for (int i = 0; i < T::kChunks; ++i) {
-            const int row = (tid + 256 * i) >> 3;
-            if (T::kRows * 8 % 256 == 0 || row < T::kRows) *(uint4*)(d + row * 128 + ((cj ^ a_swz(row)) << 4)) = pa[i];
-        }
-        if (tid < T::kRows) *(uint2*)(d + T::kCodes + tid * 8) = make_uint2(pe[0], pe[1]);
+    auto issue_w = [&](int i, int buf) {
+        dma16(wp[i], wdst[i] + buf * T::kWBytes);
+        wp[i] += 1024;
     };
-
-    uint4 w[2][NF];
-    uint32_t ws[NF], wsn[NF];
-    auto loadw = [&](uint4 (&d)[NF], int kt) {
-        const uint32_t off = (uint32_t)min(kt, K128 - 1) * 1024u + lane * 16;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) d[f] = ld16(strip[f] + off);
-    };
-    auto loadws = [&](uint32_t (&d)[NF], int g) {
-        const uint32_t off = sc0 + (uint32_t)min(g, G - 1) * 256u + lane * 4;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) d[f] = *(const uint32_t*)(strip[f] + off);
+    auto issue_s = [&](int i, int g) {
+        const uint32_t off = srow[i] ? (uint32_t)max(min(4 * g, K128 - 4), 0) * 4u : (uint32_t)g * 256u;
+        if (!srow[i] || K128 >= 4) dma16(sp[i] + off, sdst[i] + (g & 1) * T::kScBytes);
     };
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int j = 0; j < MF; ++j) acc[f][j] = mx_v4f{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < MF; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[f][j][e] = 0.f;
 
-    const int r0 = wm * 16 * MF + (lane & 15), blk = lane >> 4;
-    auto step = [&](auto sc) {                           // step S of the current group
+    if (K128 < 4) {                                      // rows shorter than a 16-byte piece of scales
+        for (int i = tid; i < T::kRows * K128; i += 64 * T::kWaves) {
+            const int r = i / K128, s = i - r * K128;
+            *(uint32_t*)(smem + T::kScAt + r * 16 + s * 4) = *(const uint32_t*)(x.e + ((size_t)rows(r) * K128 + s) * 4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < T::PS; ++i) issue_s(i, 0);
+#pragma unroll
+    for (int p = 0; p < NA - 1; ++p)
+        if (2 * p < K128)
+#pragma unroll
+            for (int i = 0; i < T::PA; ++i) issue_a(i, p, p);
+#pragma unroll
+    for (int k = 0; k < NS - 1; ++k)
+        if (k < K128)
+#pragma unroll
+            for (int i = 0; i < T::PW; ++i) issue_w(i, k);
+
+    const int r0 = wm * 32 * MF + (lane & 31), sw = a_swz(r0);                      // rows 32 apart: the same rotation
+    const uint32_t a_at = (uint32_t)r0 * 128u;
+    const uint32_t w_at = (uint32_t)(2 * wn * NF + ((lane >> 4) & 1)) * 1024u + (uint32_t)(half * 16 + (lane & 15)) * 16u;
+    const uint32_t ws_at = (uint32_t)T::kScAt + T::kRowSc * 1024u + (uint32_t)(2 * wn * NF + ((lane >> 4) & 1)) * 256u +
+                           (uint32_t)(half * 16 + (lane & 15)) * 4u;
+    uint32_t ws[NF][2];
+    int wbuf = 0, abuf = 0;
+    // Step k.  S = k % 4 in the steady groups, straight code in which every DMA exists and every wait is a constant;
+    // S = -1 for the first group and the last steps.
+    auto step = [&](auto sc, int k) {
         constexpr int S = decltype(sc)::value;
-        const uint8_t* d = smem + (S >> 1) * T::kStage;
-#pragma unroll
-        for (int j = 0; j < MF; ++j) {
-            const int row = r0 + 16 * j;
-            const uint4 a = *(const uint4*)(d + row * 128 + (((4 * (S & 1) + blk) ^ a_swz(row)) << 4));
-            const uint32_t sa = d[T::kCodes + row * 8 + 4 * (S & 1) + blk];
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma<S>(w[S & 1][f], a, acc[f][j], ws[f], sa);
-        }
-    };
-
-    fetch(0);
-    loadws(ws, 0);
-    loadw(w[0], 0);
-    put(0);
-    lds_barrier();
-    for (int g = 0; g < G; ++g) {
-        const int kt = 4 * g;
-        loadws(wsn, g + 1);
-        fetch(2 * g + 1);
-        loadw(w[1], kt + 1);
-        step(std::integral_constant<int, 0>{});
-        if (kt + 1 < K128) {
-            loadw(w[0], kt + 2);
-            step(std::integral_constant<int, 1>{});
-        }
-        put(1);
+        constexpr bool kSteady = S >= 0;
+        const int g = k >> 2;
+        // At the start the pairs came before the weights and near the end nothing new was issued: there only the
+        // weights of the steps after this one may still be out (they are younger than everything that it reads).
+        if constexpr (kSteady) vm_wait<T::younger(S + 8)>();
+        else if (K128 >= 4 && k + NS - 2 < K128) vm_wait<(NS - 2) * T::PW>();
+        else if (K128 >= 4 && NS == 4 && k + 1 < K128) vm_wait<T::PW>();
+        else vm_wait<0>();
         lds_barrier();
-        if (kt + 2 < K128) {
-            fetch(2 * g + 2);
-            loadw(w[1], kt + 3);
-            step(std::integral_constant<int, 2>{});
-            if (kt + 3 < K128) {
-                loadw(w[0], kt + 4);
-                step(std::integral_constant<int, 3>{});
-            }
-            put(0);
-            lds_barrier();
-        }
+        // this step's DMAs, spread over its 2 MF batches of products: issued together they hold up both waves of a
+        // SIMD while the address unit takes them, and nothing multiplies
+        const int an = abuf == 0 ? NA - 1 : abuf - 1, wn_ = wbuf == 0 ? NS - 1 : wbuf - 1;
+        auto issue = [&](auto bc) {
+            constexpr int B = decltype(bc)::value, nS = S <= 0 ? T::PS : 0, nA = !kSteady || (S & 1) == 0 ? T::PA : 0, n = nS + nA + T::PW;
+            constexpr int lo = B * n / (2 * MF), hi = (B + 1) * n / (2 * MF);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) ws[f] = wsn[f];
+            for (int i = lo; i < hi; ++i) {
+                if (i < nS) { if (kSteady || ((k & 3) == 0 && k + 4 < K128)) issue_s(i, g + 1); }
+                else if (i < nS + nA) { if (kSteady || ((k & 1) == 0 && k + 2 * (NA - 1) < K128)) issue_a(i - nS, (k >> 1) + NA - 1, an); }
+                else { if (kSteady || k + NS - 1 < K128) issue_w(i - nS - nA, wn_); }
+            }
+        };
+        const uint8_t* sa_ = smem + abuf * T::kABytes + a_at;
+        const uint8_t* sw_ = smem + T::kWAt + wbuf * T::kWBytes + w_at;
+        const uint32_t so = (uint32_t)(g & 1) * T::kScBytes;
+        if constexpr (S <= 0) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    ws[f][h] = *(const uint32_t*)(smem + ws_at + so + f * 512 + h * 128);
+                    if constexpr (!kSteady) ws[f][h] >>= 8 * (k & 3);
+                }
+        }
+        const int c0 = 4 * (k & 1) + half;               // the lane's first block
+        const uint8_t* sa_row = smem + T::kScAt + so + r0 * 16 + 4 * (k - max(min(4 * g, K128 - 4), 0));
+        uint4 w[NF][2];
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[f][h] = *(const uint4*)(sw_ + f * 2048 + h * 512);
+        static_for<0, MF>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const uint4 a0 = *(const uint4*)(sa_ + j * 4096 + ((c0 ^ sw) << 4));
+            const uint4 a1 = *(const uint4*)(sa_ + j * 4096 + (((c0 + 2) ^ sw) << 4));
+            // the step's four scale bytes, this lane's two in bytes 0 and 2
+            const uint32_t sa = *(const uint32_t*)(sa_row + j * 512) >> (8 * half);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 0>(w[f][0], a0, acc[f][j], ws[f][0], sa);
+            issue(std::integral_constant<int, 2 * j>{});
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 2>(w[f][1], a1, acc[f][j], ws[f][1], sa);
+            issue(std::integral_constant<int, 2 * j + 1>{});
+        });
+        wbuf = wbuf == NS - 1 ? 0 : wbuf + 1;
+        if (k & 1) abuf = abuf == NA - 1 ? 0 : abuf + 1;
+    };
+    int k = 0;
+    for (; k < min(4, K128); ++k) step(std::integral_constant<int, -1>{}, k);
+    for (; k + 8 <= K128; k += 4) {                      // every DMA of these steps exists: the last reaches step k + 7
+        step(std::integral_constant<int, 0>{}, k);
+        step(std::integral_constant<int, 1>{}, k + 1);
+        step(std::integral_constant<int, 2>{}, k + 2);
+        step(std::integral_constant<int, 3>{}, k + 3);
+    }
+    for (; k < K128; ++k) step(std::integral_constant<int, -1>{}, k);
+    // The matrix unit writes its result after the instruction, and a read of it before then is not held up: the
+    // compiler counts the wait states, but was seen to count too few where branches around the DMAs come between
+    // (element 15 of an accumulator read stale).  Nothing reads an accumulator before this.
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[f][j]));
+}
+
+// The wave's outputs through its part of LDS, 32 activation rows at a time, so that they leave as 16-byte pieces of
+// whole row segments (64 bytes to 384; stored straight from the accumulators, 8 bytes of each of 32 rows at a time, they
+// took as long as the loop: 34 us of 132).  row(r): the output row of the wave's activation row r, below 0: none.
+template <int MF, int NF, bool BF, class Row>
+__device__ __forceinline__ void mx_store(uint8_t* smem, const mx_v16f (&acc)[NF][MF], void* D, int n0, int N, int vec, Row row) {
+    constexpr int kSize = BF ? 2 : 4, kPer = 16 / kSize, kRow = 32 * NF * kSize, kStride = kRow + 16, kPieces = kRow / 16;
+    const int lane = threadIdx.x & 63;
+    uint8_t* buf = smem + (threadIdx.x >> 6) * 32 * kStride;
+    __syncthreads();                                     // every wave is done with the operands
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint8_t* d = buf + (lane & 31) * kStride + (32 * f + 8 * e + 4 * (lane >> 5)) * kSize;
+                const mx_v16f& v = acc[f][j];
+                if constexpr (BF) *(uint2*)d = make_uint2(mx_bf16x2(v[4 * e], v[4 * e + 1]), mx_bf16x2(v[4 * e + 2], v[4 * e + 3]));
+                else *(mx_v4f*)d = mx_v4f{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own writes, read by its other lanes
+#pragma unroll
+        for (int i = 0; i < 32 * kPieces / 64; ++i) {
+            const int p = lane + 64 * i, r = p / kPieces, c = p - r * kPieces, n = n0 + c * kPer;
+            const uint4 v = *(const uint4*)(buf + r * kStride + c * 16);
+            const int64_t m = row(32 * j + r);
+            if (m < 0 || n >= N) continue;
+            uint8_t* d = (uint8_t*)D + ((size_t)m * N + n) * kSize;
+            if (vec) {
+                *(uint4*)d = v;
+            } else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int q = 0; q < kPer; ++q)
+                    if (n + q < N) {
+                        if constexpr (BF) ((uint16_t*)d)[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+                        else ((uint32_t*)d)[q] = w[q];
+                    }
+            }
+        }
+        asm volatile("" ::: "memory");                   // reads before the next rows' writes (LDS is in order)
     }
 }
 
-template <int MF, int NF, int WM, bool BF>
-__global__ void __launch_bounds__(256, 2) k_gemm_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ D, int M, int N, int K128,
-                                                       int mtiles, int vec) {
-    using T = MxTile<MF, NF, WM>;
-    __shared__ __align__(16) uint8_t smem[T::kLds];
+template <int MF, int NF, int WM, int WN, int NS, int NA, bool BF>
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_gemm_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ D, int M, int N, int K128,
+                                                                int mtiles, int vec) {
+    using T = MxTile<MF, NF, WM, WN, NS, NA>;
+    extern __shared__ __align__(16) uint8_t smem[];
     // workgroup i runs on XCD i % 8: each XCD takes a contiguous range of tiles, rows fastest, so that the
     // tiles it runs together share weight strips in its L2
     const uint32_t total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, rem = total & 7;
     const uint32_t t = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
     const int m0 = (int)(t % (uint32_t)mtiles) * T::kRows, n0 = (int)(t / (uint32_t)mtiles) * T::kCols;
-    mx_v4f acc[NF][MF];
-    mx_tile<MF, NF, WM>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % T::kWN, wm = wave / T::kWN;
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        const int n = n0 + 16 * (wn * NF + f) + 4 * (lane >> 4);
-#pragma unroll
-        for (int j = 0; j < MF; ++j) {
-            const int m = m0 + 16 * (wm * MF + j) + (lane & 15);
-            if (m < M && n < N) mx_store4<BF>(D, (size_t)m * N + n, acc[f][j], N - n, vec);
-        }
-    }
+    mx_v16f acc[NF][MF];
+    mx_tile<MF, NF, WM, WN, NS, NA>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
+    const int wave = threadIdx.x >> 6, mw = m0 + 32 * MF * (wave / WN);
+    mx_store<MF, NF, BF>(smem, acc, D, n0 + 32 * NF * (wave % WN), N, vec, [&](int r) { return mw + r < M ? (int64_t)(mw + r) : -1; });
 }
 
 // Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 64 at a time, with as
-// many 16-row fragments as they need.
-constexpr int kMoeNF = 2, kMoeCols = 16 * kMoeNF * 4, kMoeRows = 64;
+// many 32-row fragments as they need.
+constexpr int kMoeNS = 4, kMoeNA = 3, kMoeCols = 128, kMoeRows = 64;
 
 template <int MF, bool BF>
 __device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_xmx x, const int* rowtab, int k0, int n, int n0, void* D, int N, int K128,
                                          int vec) {
-    mx_v4f acc[kMoeNF][MF];
-    mx_tile<MF, kMoeNF, 1>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
+    mx_v16f acc[1][MF];
+    mx_tile<MF, 1, 1, 4, kMoeNS, kMoeNA>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
         const int k = k0 + min(r, n - 1);
         return rowtab ? rowtab[k] : k;
     }, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int f = 0; f < kMoeNF; ++f) {
-        const int nn = n0 + 16 * (wave * kMoeNF + f) + 4 * (lane >> 4);
-#pragma unroll
-        for (int j = 0; j < MF; ++j) {
-            const int m = 16 * j + (lane & 15);
-            if (m < n && nn < N) mx_store4<BF>(D, (size_t)(k0 + m) * N + nn, acc[f][j], N - nn, vec);
-        }
-    }
+    mx_store<MF, 1, BF>(smem, acc, D, n0 + 32 * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return r < n ? (int64_t)(k0 + r) : -1; });
 }
 
 template <bool BF>
@@ -354,7 +477,7 @@ __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __rest
                                                            const qmm_moe_tile* __restrict__ tiles, const int* __restrict__ counts,
                                                            const int* __restrict__ rowtab, qmm_xmx x, void* __restrict__ D, int N, int K128,
                                                            uint32_t nblocks, int vec) {
-    __shared__ __align__(16) uint8_t smem[MxTile<4, kMoeNF, 1>::kLds];
+    extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t ti = blockIdx.x / nblocks;
     if (ti >= (uint32_t)(counts[0] + counts[1])) return;
     const qmm_moe_tile t = tiles[ti];
@@ -362,10 +485,9 @@ __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __rest
     const uint8_t* We = t.expert < 0 ? (Wsh ? Wsh : W) : W + (size_t)t.expert * ebytes;
     for (int r = 0; r < t.ncols; r += kMoeRows) {
         const int n = min(t.ncols - r, kMoeRows);
-        if (n <= 16) moe_rows<1, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else if (n <= 32) moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else moe_rows<4, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        lds_barrier();
+        if (n <= 32) moe_rows<1, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+        else moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+        __syncthreads();                                 // the ring is filled again
     }
 }
 
@@ -379,19 +501,23 @@ int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int N, in
     if (misaligned(W, 16) || misaligned(x.q, 16) || misaligned(x.e, 4) || misaligned(y, dtype == QMM_BF16 ? 2 : 4)) return QMM_ERR_ARG;
     return QMM_OK;
 }
-// whether four outputs of a row are one aligned store
+// whether four outputs of a row are one aligned store, and whether 16 bytes of them are
 int vec_out(const void* y, int dtype, int N) { return N % 4 == 0 && !misaligned(y, dtype == QMM_BF16 ? 8 : 16); }
+int vec16_out(const void* y, int dtype, int N) { return N % (dtype == QMM_BF16 ? 8 : 4) == 0 && !misaligned(y, 16); }
 
-template <int MF, int NF, int WM>
+template <int MF, int NF, int WM, int WN, int NS, int NA>
 int launch_gemm(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K128, hipStream_t s) {
-    using T = MxTile<MF, NF, WM>;
+    using T = MxTile<MF, NF, WM, WN, NS, NA>;
+    static_assert(T::kLds <= 160 * 1024, "LDS of a CU");
     const int64_t mt = ((int64_t)M + T::kRows - 1) / T::kRows, nt = ((int64_t)N + T::kCols - 1) / T::kCols;
     if (mt * nt > 0x7fffffff) return QMM_ERR_SHAPE;
-    const dim3 grid((unsigned)(mt * nt));
+    const dim3 grid((unsigned)(mt * nt)), block(64 * T::kWaves);
     if (dtype == QMM_BF16)
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, true>), grid, dim3(256), 0, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, vec_out(D, dtype, N));
+        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, true>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt,
+                           vec16_out(D, dtype, N));
     else
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, false>), grid, dim3(256), 0, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, vec_out(D, dtype, N));
+        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, false>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt,
+                           vec16_out(D, dtype, N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
 }
@@ -458,9 +584,9 @@ int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, i
     const int K128 = mx_steps(K);
     hipStream_t s = (hipStream_t)stream;
     const auto tiles = [&](int bm, int bn) { return (((int64_t)M + bm - 1) / bm) * (((int64_t)N + bn - 1) / bn); };
-    if (tiles(128, 256) >= 512) return launch_gemm<8, 4, 1>(W, x, D, dtype, M, N, K128, s);
-    if (tiles(128, 128) >= 256) return launch_gemm<8, 2, 1>(W, x, D, dtype, M, N, K128, s);
-    return launch_gemm<4, 1, 1>(W, x, D, dtype, M, N, K128, s);
+    if (tiles(256, 192) >= 256) return launch_gemm<2, 3, 2, 2, 3, 2>(W, x, D, dtype, M, N, K128, s);
+    if (tiles(128, 128) >= 256) return launch_gemm<2, 2, 2, 2, 3, 2>(W, x, D, dtype, M, N, K128, s);
+    return launch_gemm<2, 1, 1, 4, 4, 2>(W, x, D, dtype, M, N, K128, s);
 }
 
 int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
@@ -475,13 +601,14 @@ int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_
     if ((uint64_t)nblocks * max_tiles > 0x7fffffffu) return QMM_ERR_SHAPE;
     const int K128 = mx_steps(K);
     const dim3 grid(nblocks * (uint32_t)max_tiles);
+    constexpr size_t lds = MxTile<2, 1, 1, 4, kMoeNS, kMoeNA>::kLds;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == QMM_BF16)
-        hipLaunchKernelGGL(k_moe_gemm_mxfp4<true>, grid, dim3(256), 0, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
-                           K128, nblocks, vec_out(D, dtype, N));
+        hipLaunchKernelGGL(k_moe_gemm_mxfp4<true>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
+                           K128, nblocks, vec16_out(D, dtype, N));
     else
-        hipLaunchKernelGGL(k_moe_gemm_mxfp4<false>, grid, dim3(256), 0, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
-                           K128, nblocks, vec_out(D, dtype, N));
+        hipLaunchKernelGGL(k_moe_gemm_mxfp4<false>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
+                           K128, nblocks, vec16_out(D, dtype, N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
 }

@@ -383,46 +383,58 @@ def moe_gemm(fmt, shared_fmt, W, Wsh, ebytes, tiles, ntiles, stiles, nstiles, ct
 
 
 # ---- MXFP4 decoder blocks ----
+# These calls answer in a few microseconds on the device, so their checks are kept to one pass over each
+# tensor and the arguments go to the library as plain integers.
 _DTYPE = {torch.float32: _lib.QMM_F32, torch.bfloat16: _lib.QMM_BF16}
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _handle(stream):
+    """The stream to launch on: the current one of the current device, or one of that device."""
+    if stream is None:
+        return _raw_stream(_device())
+    if stream.device_index != _device():
+        raise QmmError(f"the stream is of cuda:{stream.device_index}, the current device is cuda:{_device()}")
+    return stream.cuda_stream
+
+
+def _in(t, n, name, dtype=None):
+    """The address of t: a contiguous tensor of at least n elements on the current device (the library launches there)."""
+    if t is None or not t.is_cuda or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
+        _dev(t, dtype, name)
+    if t.get_device() != _device():
+        raise QmmError(f"{name} is on {t.device}, the current device is cuda:{_device()}")
+    if t.numel() < n:
+        raise QmmError(f"{name} holds {t.numel()} elements, {n} are needed")
+    return t.data_ptr()
 
 
 def _dtype(t, name):
-    if t.dtype not in _DTYPE:
+    d = _DTYPE.get(t.dtype)
+    if d is None:
         raise QmmError(f"{name} must be float32 or bfloat16, got {t.dtype}")
-    return _DTYPE[t.dtype]
+    return d
 
 
-def _here(t, name):
-    """t lies on the current device: the library launches there, on its current stream."""
-    if t.device.index != torch.cuda.current_device():
-        raise QmmError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _room(t, n, name):
-    """t is a contiguous tensor of at least n elements on the current device."""
-    _dev(t, None, name)
-    _here(t, name)
-    if t.numel() < n:
-        raise QmmError(f"{name} holds {t.numel()} elements, {n} are needed")
-    return t
-
-
-def _rows_of(t, n, name):
-    """Row stride of t, a device tensor [rows][n] (or one row [n]) whose rows are contiguous."""
+def _rows(t, rows, n, name):
+    """The row stride of t, `rows` rows of n contiguous values (or one row [n]) on the current device."""
     if t is None or not t.is_cuda:
         raise QmmError(f"{name} must be a CUDA tensor")
-    _here(t, name)
-    if t.dim() not in (1, 2) or t.shape[-1] != n or (n > 1 and t.stride(-1) != 1):
-        raise QmmError(f"{name} must be rows of {n} contiguous values, got shape {tuple(t.shape)}, strides {tuple(t.stride())}")
-    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < n:
-        raise QmmError(f"{name}: rows overlap (stride {t.stride(0)}, {n} values)")
-    return t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else n
-
-
-def _rows_match(t, rows, name):
-    have = t.shape[0] if t.dim() == 2 else 1
+    if t.get_device() != _device():
+        raise QmmError(f"{name} is on {t.device}, the current device is cuda:{_device()}")
+    shape = t.shape
+    if len(shape) not in (1, 2) or shape[-1] != n or (n > 1 and t.stride(-1) != 1):
+        raise QmmError(f"{name} must be rows of {n} contiguous values, got shape {tuple(shape)}, strides {tuple(t.stride())}")
+    have = shape[0] if len(shape) == 2 else 1
     if have < rows:
         raise QmmError(f"{name} has {have} rows, {rows} are needed")
+    if have == 1:
+        return n
+    ld = t.stride(0)
+    if ld < n:
+        raise QmmError(f"{name}: rows overlap (stride {ld}, {n} values)")
+    return ld
 
 
 def mxfp4_steps(K):
@@ -443,23 +455,22 @@ class XMXBuf:
 
 
 def _xmx(x, rows, K, name):
-    if x.rows < rows or mxfp4_steps(x.K) != mxfp4_steps(K):
-        raise QmmError(f"{name} holds {x.rows} rows of {x.K} values, {rows} of {K} are needed")
-    return x.c()
+    steps = (K + 127) // 128
+    if (x.K + 127) // 128 != steps:
+        raise QmmError(f"{name} holds rows of {x.K} values, rows of {K} are needed")
+    return XMX(_in(x.q, rows * steps * 64, name, torch.uint8), _in(x.e, rows * steps * 4, name, torch.uint8))
 
 
 def quantize_mxfp4(x, out, rows, K, stream=None):
     """x f32 or bf16 [rows][K] (rows may be strided) -> out (XMXBuf): blocks of 32, scale 2^(floor(log2 amax) - 2),
     codes rounded to nearest even."""
-    ld = _rows_of(x, K, "x")
-    _rows_match(x, rows, "x")
-    check(_lib.lib().qmm_quantize_mxfp4(_p(x), _dtype(x, "x"), ld, _xmx(out, rows, K, "out"), rows, K, _stream(stream)), "quantize_mxfp4")
+    ld = _rows(x, rows, K, "x")
+    check(_lib.lib().qmm_quantize_mxfp4(x.data_ptr(), _dtype(x, "x"), ld, _xmx(out, rows, K, "out"), rows, K, _handle(stream)), "quantize_mxfp4")
 
 
 def dequant_mxfp4(x, out, rows, K, stream=None):
     """The values of x (XMXBuf) into out [rows][K], f32 or bf16 (exact in both)."""
-    _room(out, rows * K, "out")
-    check(_lib.lib().qmm_dequant_mxfp4(_xmx(x, rows, K, "x"), _p(out), _dtype(out, "out"), rows, K, _stream(stream)), "dequant_mxfp4")
+    check(_lib.lib().qmm_dequant_mxfp4(_xmx(x, rows, K, "x"), _in(out, rows * K, "out"), _dtype(out, "out"), rows, K, _handle(stream)), "dequant_mxfp4")
 
 
 def mxfp4_weight_bytes(N, K):
@@ -467,14 +478,19 @@ def mxfp4_weight_bytes(N, K):
     return _lib.lib().qmm_mxfp4_weight_bytes(N, K)
 
 
+def _weight(W, N, K, name="W", extra=0):
+    """The address of a packed weight of N rows of K values, `extra` bytes into its buffer."""
+    steps = (K + 127) // 128
+    return _in(W, extra + (N + 15) // 16 * (steps * 1024 + (steps + 3) // 4 * 256), name, torch.uint8)
+
+
 def pack_mxfp4(q, e, W, N, K, stream=None):
     """MXFP4 rows q [N][64 per step], e [N][4 per step] (an XMXBuf's tensors) -> W, the layout the products read."""
     for t, per, name in ((q, 64, "q"), (e, 4, "e")):
-        _dev(t, torch.uint8, name)
+        _in(t, 0, name, torch.uint8)
         if t.numel() != N * per * mxfp4_steps(K):
             raise QmmError(f"{name} must hold {N} rows of {per * mxfp4_steps(K)} bytes")
-    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W")
-    check(_lib.lib().qmm_pack_mxfp4(XMX(q.data_ptr(), e.data_ptr()), _p(W), N, K, _stream(stream)), "pack_mxfp4")
+    check(_lib.lib().qmm_pack_mxfp4(XMX(q.data_ptr(), e.data_ptr()), _weight(W, N, K), N, K, _handle(stream)), "pack_mxfp4")
 
 
 def repack_row_mxfp4(src, K):
@@ -490,39 +506,29 @@ def repack_row_mxfp4(src, K):
 
 def gemv_mxfp4(W, x, y, ncol, N, K, stream=None):
     """y[m][n] = W[n] . x[m] for m < ncol <= 64 (x an XMXBuf, y f32 or bf16 [ncol][N])."""
-    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W"); _room(y, ncol * N, "y")
-    check(_lib.lib().qmm_gemv_mxfp4(_p(W), _xmx(x, ncol, K, "x"), _p(y), _dtype(y, "y"), ncol, N, K, _stream(stream)), "gemv_mxfp4")
+    check(_lib.lib().qmm_gemv_mxfp4(_weight(W, N, K), _xmx(x, ncol, K, "x"), _in(y, ncol * N, "y"), _dtype(y, "y"), ncol, N, K, _handle(stream)),
+          "gemv_mxfp4")
 
 
 def gemm_mxfp4(W, x, D, M, N, K, stream=None):
     """D[m][n] = W[n] . x[m] for any M (x an XMXBuf, D f32 or bf16 [M][N])."""
-    _dev(W, torch.uint8, "W"); _room(W, mxfp4_weight_bytes(N, K), "W"); _room(D, M * N, "D")
-    check(_lib.lib().qmm_gemm_mxfp4(_p(W), _xmx(x, M, K, "x"), _p(D), _dtype(D, "D"), M, N, K, _stream(stream)), "gemm_mxfp4")
-
-
-def _experts(W, Wsh, ebytes, nexperts, N, K):
-    one = mxfp4_weight_bytes(N, K)
-    _dev(W, torch.uint8, "W"); _room(W, (nexperts - 1) * ebytes + one, "W")
-    if Wsh is not None:
-        _dev(Wsh, torch.uint8, "Wsh"); _room(Wsh, one, "Wsh")
+    check(_lib.lib().qmm_gemm_mxfp4(_weight(W, N, K), _xmx(x, M, K, "x"), _in(D, M * N, "D"), _dtype(D, "D"), M, N, K, _handle(stream)), "gemm_mxfp4")
 
 
 def gemv_moe_mxfp4(W, Wsh, ebytes, ids, x, y, T, nslot, nexperts, N, K, xrow_te=False, stream=None):
     """y[te][n] = W_{ids[te]}[n] . x[te if xrow_te else t] for T <= 16 tokens (ids int32 [T][nslot], below 0: Wsh)."""
-    _experts(W, Wsh, ebytes, nexperts, N, K)
-    _dev(ids, torch.int32, "ids"); _room(ids, T * nslot, "ids"); _room(y, T * nslot * N, "y")
-    check(_lib.lib().qmm_gemv_moe_mxfp4(_p(W), _p(Wsh), ebytes, _p(ids), _xmx(x, T * nslot if xrow_te else T, K, "x"), _p(y), _dtype(y, "y"), T, nslot,
-                                        nexperts, N, K, int(xrow_te), _stream(stream)), "gemv_moe_mxfp4")
+    slots = T * nslot
+    check(_lib.lib().qmm_gemv_moe_mxfp4(_weight(W, N, K, "W", (nexperts - 1) * ebytes), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
+                                        _in(ids, slots, "ids", torch.int32), _xmx(x, slots if xrow_te else T, K, "x"), _in(y, slots * N, "y"),
+                                        _dtype(y, "y"), T, nslot, nexperts, N, K, int(xrow_te), _handle(stream)), "gemv_moe_mxfp4")
 
 
 def moe_gemm_mxfp4(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, N, K, stream=None):
     """D[k] = W_e . x[rowtab[k]] over rows sorted by expert (moe_sort's tiles, counts, rowtok; rowtab None: x[k])."""
-    _dev(W, torch.uint8, "W"); _dev(tiles, torch.int32, "tiles"); _room(tiles, 3 * max_tiles, "tiles")
-    _dev(counts, torch.int32, "counts"); _room(counts, 2, "counts"); _dev(D, None, "D")
-    if rowtab is not None:
-        _dev(rowtab, torch.int32, "rowtab")
-    check(_lib.lib().qmm_moe_gemm_mxfp4(_p(W), _p(Wsh), ebytes, _p(tiles), _p(counts), max_tiles, _p(rowtab), _xmx(x, 0, K, "x"), _p(D), _dtype(D, "D"),
-                                        N, K, _stream(stream)), "moe_gemm_mxfp4")
+    check(_lib.lib().qmm_moe_gemm_mxfp4(_weight(W, N, K), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
+                                        _in(tiles, 3 * max_tiles, "tiles", torch.int32), _in(counts, 2, "counts", torch.int32), max_tiles,
+                                        None if rowtab is None else _in(rowtab, 0, "rowtab", torch.int32), _xmx(x, 0, K, "x"), _in(D, 0, "D"),
+                                        _dtype(D, "D"), N, K, _handle(stream)), "moe_gemm_mxfp4")
 
 
 _SCORE = {"softmax": 0, "sigmoid": 1}
@@ -535,16 +541,13 @@ def moe_route_groups(logits, ids, w, T, nexp, topk, score="softmax", bias=None, 
     best of `groups` groups (by their `best` = 1 or 2 largest), the topk experts of those (ties to the lower id);
     weights: the scores, renormalised if renorm, times scale.  shared: None, "gate" (logit nexp's sigmoid) or "one",
     a last slot of id -1.  ids int32, w f32 [T][topk (+ 1)]."""
-    _dev(logits, torch.float32, "logits"); _dev(ids, torch.int32, "ids"); _dev(w, torch.float32, "w")
     if score not in _SCORE or shared not in _SHARED:
         raise QmmError(f"score {score!r}, shared {shared!r}: softmax or sigmoid; None, 'gate' or 'one'")
-    slots = topk + (shared is not None)
-    _room(logits, T * logits.shape[-1], "logits"); _room(ids, T * slots, "ids"); _room(w, T * slots, "w")
-    if bias is not None:
-        _dev(bias, torch.float32, "bias"); _room(bias, nexp, "bias")
-    rule = RouteRule(None if bias is None else bias.data_ptr(), scale, _SCORE[score], groups, keep, best, int(renorm), _SHARED[shared])
-    check(_lib.lib().qmm_moe_route_groups(_p(logits), logits.shape[-1], ctypes.byref(rule), _p(ids), _p(w), T, nexp, topk, _stream(stream)),
-          "moe_route_groups")
+    stride, slots = logits.shape[-1], T * (topk + (shared is not None))
+    rule = RouteRule(None if bias is None else _in(bias, nexp, "bias", torch.float32), scale, _SCORE[score], groups, keep, best, int(renorm),
+                     _SHARED[shared])
+    check(_lib.lib().qmm_moe_route_groups(_in(logits, T * stride, "logits", torch.float32), stride, rule, _in(ids, slots, "ids", torch.int32),
+                                          _in(w, slots, "w", torch.float32), T, nexp, topk, _handle(stream)), "moe_route_groups")
 
 
 _ACT = {"none": 0, "sigmoid": 1, "silu": 2}
@@ -552,51 +555,42 @@ _ACT = {"none": 0, "sigmoid": 1, "silu": 2}
 
 def _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n):
     """The leading arguments of the postnorm_add_rmsnorm calls."""
-    _dev(x, torch.float32, "x"); _room(x, T * n, "x"); _dev(w, torch.float32, "w"); _room(w, n, "w")
-    ldy = _rows_of(y, n, "y")
-    _rows_match(y, T, "y")
-    if wy is not None:
-        _dev(wy, torch.float32, "wy"); _room(wy, n, "wy")
-    xo = x if xo is None else xo
-    _dev(xo, torch.float32, "xo"); _room(xo, T * n, "xo")
-    g = Gate(None, 0, 0, 0, 0)
+    px = _in(x, T * n, "x", torch.float32)
+    ldy = _rows(y, T, n, "y")
     if act not in _ACT:
         raise QmmError(f"act {act!r}: none, sigmoid or silu")
+    g = None
     if gate is not None:
-        if gate.dim() == 2 and gate.shape[1] == 1 and n > 1:                 # one value per token
-            _rows_match(gate, T, "gate")
-            if not gate.is_cuda:
-                raise QmmError("gate must be a CUDA tensor")
-            _here(gate, "gate")
+        if gate.dim() == 2 and gate.shape[1] == 1 and n > 1:             # one value per token
+            _rows(gate, T, 1, "gate")
             ld, per = gate.stride(0), 0
+        elif gate.dim() == 1:                                            # one row for every token
+            _rows(gate, 1, n, "gate")
+            ld, per = 0, 1
         else:
-            ld, per = _rows_of(gate, n, "gate"), 1
-            if gate.dim() == 1:                                              # one row for every token
-                ld = 0
-            else:
-                _rows_match(gate, T, "gate")
+            ld, per = _rows(gate, T, n, "gate"), 1
         g = Gate(gate.data_ptr(), ld, _dtype(gate, "gate"), _ACT[act], per)
-    return [_p(x), _p(y), _dtype(y, "y"), ldy, _p(wy), ctypes.byref(g), alpha, _p(xo), _p(w)]
+    return (px, y.data_ptr(), _dtype(y, "y"), ldy, None if wy is None else _in(wy, n, "wy", torch.float32), g, alpha,
+            px if xo is None else _in(xo, T * n, "xo", torch.float32), _in(w, n, "w", torch.float32))
 
 
 def postnorm_add_rmsnorm_bf16(x, y, wy, w, xb, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
     """Between two blocks, per row: p = rmsnorm(y) * wy (wy None: y), p *= act(gate), xo = x + alpha * p (xo None: in
     place), xb = bf16(rmsnorm(xo) * w).  y f32 or bf16 rows; gate f32 or bf16 [T][1], [n] or [T][n]."""
     a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
-    _dev(xb, torch.bfloat16, "xb"); _room(xb, T * n, "xb")
-    check(_lib.lib().qmm_postnorm_add_rmsnorm_bf16(*a, _p(xb), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_bf16")
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_bf16(*a, _in(xb, T * n, "xb", torch.bfloat16), T, n, eps, _handle(stream)), "postnorm_add_rmsnorm_bf16")
 
 
 def postnorm_add_rmsnorm_quant(x, y, wy, w, xn, xq, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
     """The same with xn = rmsnorm(xo) * w in f32 and its q8 in xq (XQ8Buf of T x n); n % 32 == 0."""
     a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
-    _dev(xn, torch.float32, "xn"); _room(xn, T * n, "xn")
     if xq.ncol < T or xq.K != n:
         raise QmmError(f"xq holds {xq.ncol} rows of {xq.K} values, {T} of {n} are needed")
-    check(_lib.lib().qmm_postnorm_add_rmsnorm_quant(*a, _p(xn), xq.c(), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_quant")
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_quant(*a, _in(xn, T * n, "xn", torch.float32), xq.c(), T, n, eps, _handle(stream)),
+          "postnorm_add_rmsnorm_quant")
 
 
 def postnorm_add_rmsnorm_mxfp4(x, y, wy, w, xq, T, n, eps, gate=None, act="none", alpha=1.0, xo=None, stream=None):
     """The same with rmsnorm(xo) * w as MXFP4 rows (XMXBuf of T x n)."""
     a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
-    check(_lib.lib().qmm_postnorm_add_rmsnorm_mxfp4(*a, _xmx(xq, T, n, "xq"), T, n, eps, _stream(stream)), "postnorm_add_rmsnorm_mxfp4")
+    check(_lib.lib().qmm_postnorm_add_rmsnorm_mxfp4(*a, _xmx(xq, T, n, "xq"), T, n, eps, _handle(stream)), "postnorm_add_rmsnorm_mxfp4")
