@@ -14,6 +14,7 @@
 // and the S sums are added in order.  So an output's bits depend on its own rows and K, not on the call.
 #include "mx.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace qmm {
@@ -193,6 +194,9 @@ __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uin
 // The operand reads (16 lanes: 16 rows, one chunk) are free of bank conflicts.  A step k is: wait until the own
 // DMAs that it reads have landed, barrier, start those NS - 1 steps (pairs: NA - 1 pairs) ahead, whose buffers were
 // read before that barrier, multiply.
+//
+// Eight waves run as two halves (the rows' halves, one wave of each on a SIMD), half a step apart: while one half reads
+// its operands from LDS and issues its DMAs, the other multiplies, and a barrier ends each phase.
 __device__ __forceinline__ int a_swz(int row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
 
 template <int MF, int NF, int WM, int WN, int NS, int NA>
@@ -205,6 +209,9 @@ struct MxTile {
     static constexpr int kABytes = kAPieces * 1024, kWBytes = kWPieces * 1024, kScBytes = kScPieces * 1024;
     static constexpr int kWAt = NA * kABytes, kScAt = kWAt + NS * kWBytes, kLoopLds = kScAt + 2 * kScBytes;
     static constexpr int kStoreLds = kWaves * 32 * (128 * NF + 16), kLds = kLoopLds > kStoreLds ? kLoopLds : kStoreLds;
+    // eight waves, two on each SIMD: they work half a step apart
+    static constexpr bool kTwo = kWaves == 8;
+    static_assert(!kTwo || WM == 2, "the two halves are the waves 0 .. 3 and 4 .. 7");
     // what a wave issues in step j (mod 4): scales of the next group, a pair, a step of weights, in this order
     static constexpr int issued(int j) { return PW + ((j & 1) == 0 ? PA : 0) + ((j & 3) == 0 ? PS : 0); }
     static constexpr int issued(int from, int to) { return from > to ? 0 : issued(from) + issued(from + 1, to); }
@@ -223,6 +230,12 @@ __device__ __forceinline__ void vm_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+// the value exists here, in registers (no instruction)
+__device__ __forceinline__ void pin(uint32_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void pin(mx_v16f& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void pin(uint4& a, uint4& b) {
+    asm volatile("" : "+v"(a.x), "+v"(a.y), "+v"(a.z), "+v"(a.w), "+v"(b.x), "+v"(b.y), "+v"(b.z), "+v"(b.w));
+}
 template <int I, int N, class F>
 __device__ __forceinline__ void static_for(F f) {
     if constexpr (I < N) {
@@ -318,25 +331,32 @@ __device__ __forceinline__ void mx_tile(uint8_t* smem, const uint8_t* W, qmm_xmx
                            (uint32_t)(half * 16 + (lane & 15)) * 4u;
     uint32_t ws[NF][2];
     int wbuf = 0, abuf = 0;
-    // Step k.  S = k % 4 in the steady groups, straight code in which every DMA exists and every wait is a constant;
-    // S = -1 for the first group and the last steps.
-    auto step = [&](auto sc, int k) {
+    // Everything that step k reads has landed in this wave's part.  S = k % 4 in the steady groups, where every DMA
+    // exists and the wait is a constant; S = -1 for the first group and the last steps: at the start the pairs came
+    // before the weights and near the end nothing new was issued, so only the weights of the steps after this one
+    // may still be out (they are younger than everything that it reads).
+    auto landed = [&](auto sc, int k) {
         constexpr int S = decltype(sc)::value;
-        constexpr bool kSteady = S >= 0;
-        const int g = k >> 2;
-        // At the start the pairs came before the weights and near the end nothing new was issued: there only the
-        // weights of the steps after this one may still be out (they are younger than everything that it reads).
-        if constexpr (kSteady) vm_wait<T::younger(S + 8)>();
+        if constexpr (S >= 0) vm_wait<T::younger(S + 8)>();
         else if (K128 >= 4 && k + NS - 2 < K128) vm_wait<(NS - 2) * T::PW>();
         else if (K128 >= 4 && NS == 4 && k + 1 < K128) vm_wait<T::PW>();
         else vm_wait<0>();
-        lds_barrier();
-        // this step's DMAs, spread over its 2 MF batches of products: issued together they hold up both waves of a
-        // SIMD while the address unit takes them, and nothing multiplies
+    };
+    using Next = std::integral_constant<int, -1>;
+    auto step = [&](auto sc, auto nc, int k) {           // nc: S of the step after this one
+        constexpr int S = decltype(sc)::value;
+        constexpr bool kSteady = S >= 0;
+        const int g = k >> 2;
+        if constexpr (!T::kTwo) {
+            landed(sc, k);
+            lds_barrier();
+        }
         const int an = abuf == 0 ? NA - 1 : abuf - 1, wn_ = wbuf == 0 ? NS - 1 : wbuf - 1;
-        auto issue = [&](auto bc) {
-            constexpr int B = decltype(bc)::value, nS = S <= 0 ? T::PS : 0, nA = !kSteady || (S & 1) == 0 ? T::PA : 0, n = nS + nA + T::PW;
-            constexpr int lo = B * n / (2 * MF), hi = (B + 1) * n / (2 * MF);
+        // the step's DMAs: part B of P
+        auto issue = [&](auto bc, auto pc) {
+            constexpr int B = decltype(bc)::value, P = decltype(pc)::value;
+            constexpr int nS = S <= 0 ? T::PS : 0, nA = !kSteady || (S & 1) == 0 ? T::PA : 0, n = nS + nA + T::PW;
+            constexpr int lo = B * n / P, hi = (B + 1) * n / P;
 #pragma unroll
             for (int i = lo; i < hi; ++i) {
                 if (i < nS) { if (kSteady || ((k & 3) == 0 && k + 4 < K128)) issue_s(i, g + 1); }
@@ -358,36 +378,70 @@ __device__ __forceinline__ void mx_tile(uint8_t* smem, const uint8_t* W, qmm_xmx
         }
         const int c0 = 4 * (k & 1) + half;               // the lane's first block
         const uint8_t* sa_row = smem + T::kScAt + so + r0 * 16 + 4 * (k - max(min(4 * g, K128 - 4), 0));
-        uint4 w[NF][2];
+        uint4 w[NF][2], a[MF][2];
+        uint32_t sa[MF];
+        auto read_a = [&](int j) {
+            a[j][0] = *(const uint4*)(sa_ + j * 4096 + ((c0 ^ sw) << 4));
+            a[j][1] = *(const uint4*)(sa_ + j * 4096 + (((c0 + 2) ^ sw) << 4));
+            // the step's four scale bytes, this lane's two in bytes 0 and 2
+            sa[j] = *(const uint32_t*)(sa_row + j * 512) >> (8 * half);
+        };
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
             for (int h = 0; h < 2; ++h) w[f][h] = *(const uint4*)(sw_ + f * 2048 + h * 512);
+        if constexpr (T::kTwo) {
+#pragma unroll
+            for (int j = 0; j < MF; ++j) read_a(j);
+            issue(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{});
+            // the compiler would move the reads and the products to where they suit it: they stay in their phases
+#pragma unroll
+            for (int f = 0; f < NF; ++f) pin(w[f][0], w[f][1]);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) { pin(a[j][0], a[j][1]); pin(sa[j]); }
+            if (wm != 0) landed(nc, k + 1);
+            lds_barrier();
+            __builtin_amdgcn_s_setprio(1);
+        }
         static_for<0, MF>([&](auto jc) {
             constexpr int j = decltype(jc)::value;
-            const uint4 a0 = *(const uint4*)(sa_ + j * 4096 + ((c0 ^ sw) << 4));
-            const uint4 a1 = *(const uint4*)(sa_ + j * 4096 + (((c0 + 2) ^ sw) << 4));
-            // the step's four scale bytes, this lane's two in bytes 0 and 2
-            const uint32_t sa = *(const uint32_t*)(sa_row + j * 512) >> (8 * half);
+            if constexpr (!T::kTwo) read_a(j);
 #pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 0>(w[f][0], a0, acc[f][j], ws[f][0], sa);
-            issue(std::integral_constant<int, 2 * j>{});
+            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 0>(w[f][0], a[j][0], acc[f][j], ws[f][0], sa[j]);
+            if constexpr (!T::kTwo) issue(std::integral_constant<int, 2 * j>{}, std::integral_constant<int, 2 * MF>{});
 #pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 2>(w[f][1], a1, acc[f][j], ws[f][1], sa);
-            issue(std::integral_constant<int, 2 * j + 1>{});
+            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 2>(w[f][1], a[j][1], acc[f][j], ws[f][1], sa[j]);
+            if constexpr (!T::kTwo) issue(std::integral_constant<int, 2 * j + 1>{}, std::integral_constant<int, 2 * MF>{});
         });
+        if constexpr (T::kTwo) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int j = 0; j < MF; ++j) pin(acc[f][j]);
+            __builtin_amdgcn_s_setprio(0);
+            if (wm == 0) landed(nc, k + 1);
+            lds_barrier();
+        }
         wbuf = wbuf == NS - 1 ? 0 : wbuf + 1;
         if (k & 1) abuf = abuf == NA - 1 ? 0 : abuf + 1;
     };
-    int k = 0;
-    for (; k < min(4, K128); ++k) step(std::integral_constant<int, -1>{}, k);
-    for (; k + 8 <= K128; k += 4) {                      // every DMA of these steps exists: the last reaches step k + 7
-        step(std::integral_constant<int, 0>{}, k);
-        step(std::integral_constant<int, 1>{}, k + 1);
-        step(std::integral_constant<int, 2>{}, k + 2);
-        step(std::integral_constant<int, 3>{}, k + 3);
+    if constexpr (T::kTwo) {
+        landed(Next{}, 0);
+        lds_barrier();
+        if (wm != 0) lds_barrier();                      // half a step behind
     }
-    for (; k < K128; ++k) step(std::integral_constant<int, -1>{}, k);
+    int k = 0;
+    const int first = min(4, K128);
+    for (; k < first; ++k) step(Next{}, Next{}, k);
+    for (; k + 8 <= K128; k += 4) {                      // every DMA of these steps exists: the last reaches step k + 7
+        step(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, k);
+        step(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, k + 1);
+        step(std::integral_constant<int, 2>{}, std::integral_constant<int, 3>{}, k + 2);
+        step(std::integral_constant<int, 3>{}, std::integral_constant<int, 0>{}, k + 3);
+    }
+    for (; k < K128; ++k) step(Next{}, Next{}, k);
+    if constexpr (T::kTwo)
+        if (wm == 0) lds_barrier();
     // The matrix unit writes its result after the instruction, and a read of it before then is not held up: the
     // compiler counts the wait states, but was seen to count too few where branches around the DMAs come between
     // (element 15 of an accumulator read stale).  Nothing reads an accumulator before this.
@@ -443,14 +497,16 @@ __device__ __forceinline__ void mx_store(uint8_t* smem, const mx_v16f (&acc)[NF]
 
 template <int MF, int NF, int WM, int WN, int NS, int NA, bool BF>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_gemm_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ D, int M, int N, int K128,
-                                                                int mtiles, int vec) {
+                                                                int mtiles, int panel, int vec) {
     using T = MxTile<MF, NF, WM, WN, NS, NA>;
     extern __shared__ __align__(16) uint8_t smem[];
     // workgroup i runs on XCD i % 8: each XCD takes a contiguous range of tiles, rows fastest, so that the
     // tiles it runs together share weight strips in its L2
     const uint32_t total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, rem = total & 7;
     const uint32_t t = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
-    const int m0 = (int)(t % (uint32_t)mtiles) * T::kRows, n0 = (int)(t / (uint32_t)mtiles) * T::kCols;
+    const uint32_t ntiles = total / (uint32_t)mtiles, pan = t / (panel * ntiles), left = t - pan * panel * ntiles;
+    const uint32_t pm = min((uint32_t)panel, (uint32_t)mtiles - pan * panel);
+    const int m0 = (int)(pan * panel + left % pm) * T::kRows, n0 = (int)(left / pm) * T::kCols;
     mx_v16f acc[NF][MF];
     mx_tile<MF, NF, WM, WN, NS, NA>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
     const int wave = threadIdx.x >> 6, mw = m0 + 32 * MF * (wave / WN);
@@ -505,6 +561,8 @@ int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int N, in
 int vec_out(const void* y, int dtype, int N) { return N % 4 == 0 && !misaligned(y, dtype == QMM_BF16 ? 8 : 16); }
 int vec16_out(const void* y, int dtype, int N) { return N % (dtype == QMM_BF16 ? 8 : 4) == 0 && !misaligned(y, 16); }
 
+constexpr int64_t kPanelBytes = 5 << 19;
+
 template <int MF, int NF, int WM, int WN, int NS, int NA>
 int launch_gemm(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K128, hipStream_t s) {
     using T = MxTile<MF, NF, WM, WN, NS, NA>;
@@ -512,11 +570,13 @@ int launch_gemm(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int 
     const int64_t mt = ((int64_t)M + T::kRows - 1) / T::kRows, nt = ((int64_t)N + T::kCols - 1) / T::kCols;
     if (mt * nt > 0x7fffffff) return QMM_ERR_SHAPE;
     const dim3 grid((unsigned)(mt * nt)), block(64 * T::kWaves);
+    const int64_t fit = std::max<int64_t>(1, kPanelBytes / ((int64_t)T::kRows * K128 * 64)), np = (mt + fit - 1) / fit;
+    const int panel = (int)((mt + np - 1) / np);
     if (dtype == QMM_BF16)
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, true>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt,
+        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, true>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, panel,
                            vec16_out(D, dtype, N));
     else
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, false>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt,
+        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, false>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, panel,
                            vec16_out(D, dtype, N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
@@ -584,7 +644,7 @@ int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, i
     const int K128 = mx_steps(K);
     hipStream_t s = (hipStream_t)stream;
     const auto tiles = [&](int bm, int bn) { return (((int64_t)M + bm - 1) / bm) * (((int64_t)N + bn - 1) / bn); };
-    if (tiles(256, 192) >= 256) return launch_gemm<2, 3, 2, 2, 3, 2>(W, x, D, dtype, M, N, K128, s);
+    if (tiles(192, 384) >= 200) return launch_gemm<3, 3, 2, 4, 3, 2>(W, x, D, dtype, M, N, K128, s);
     if (tiles(128, 128) >= 256) return launch_gemm<2, 2, 2, 2, 3, 2>(W, x, D, dtype, M, N, K128, s);
     return launch_gemm<2, 1, 1, 4, 4, 2>(W, x, D, dtype, M, N, K128, s);
 }
