@@ -12,10 +12,9 @@
 //
 // Order of sums.  GEMM: an output is one chain of instructions over K, whatever the tile, M or N.  GEMV: K's groups of four steps are cut into S contiguous runs, S chosen by K alone; each run is one chain
 // and the S sums are added in order.  So an output's bits depend on its own rows and K, not on the call.
-#include "mx.hpp"
+#include "mx_tile.hpp"
 
-#include <algorithm>
-#include <type_traits>
+#include <cmath>
 
 namespace qmm {
 namespace {
@@ -184,348 +183,51 @@ __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uin
 }
 
 // ------------------------------------------------------------------------------------------
-// GEMM tile, on v_mfma_scale_f32_32x32x64_f8f6f4.  WM x WN waves; a wave owns 32 MF activation rows and 32 NF
-// weight rows.  Both operands come by DMA (global_load_lds):
-//   - activations two steps (a pair, 128 bytes of a row: whole cache lines) at a time into NA buffers, 16-byte
-//     chunk c of a row at chunk c ^ swz(row).  Half lines, one step at a time, cost the vector cache a stall for
-//     every second half (the line is still on its way): half of all cycles, 155 instead of XX us below;
-//   - weights step by step into a ring of NS, a strip's kilobyte as it is in memory;
-//   - block scales by groups of four steps, 16 bytes a row, into two buffers.
-// The operand reads (16 lanes: 16 rows, one chunk) are free of bank conflicts.  A step k is: wait until the own
-// DMAs that it reads have landed, barrier, start those NS - 1 steps (pairs: NA - 1 pairs) ahead, whose buffers were
-// read before that barrier, multiply.
-//
-// Eight waves run as two halves (the rows' halves, one wave of each on a SIMD), half a step apart: while one half reads
-// its operands from LDS and issues its DMAs, the other multiplies, and a barrier ends each phase.
-__device__ __forceinline__ int a_swz(int row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
-
-template <int MF, int NF, int WM, int WN, int NS, int NA>
-struct MxTile {
-    static constexpr int kWaves = WM * WN, kRows = 32 * MF * WM, kCols = 32 * NF * WN;
-    static constexpr int per(int pieces) { return (pieces + kWaves - 1) / kWaves; }
-    // DMAs (1 KB each): of a pair's activations, of a step's weights, of a group's scales; and per wave
-    static constexpr int kAPieces = kRows / 8, kWPieces = kCols / 16, kRowSc = (kRows + 63) / 64, kScPieces = kRowSc + (kCols + 63) / 64;
-    static constexpr int PA = per(kAPieces), PW = per(kWPieces), PS = per(kScPieces);
-    static constexpr int kABytes = kAPieces * 1024, kWBytes = kWPieces * 1024, kScBytes = kScPieces * 1024;
-    static constexpr int kWAt = NA * kABytes, kScAt = kWAt + NS * kWBytes, kLoopLds = kScAt + 2 * kScBytes;
-    static constexpr int kStoreLds = kWaves * 32 * (128 * NF + 16), kLds = kLoopLds > kStoreLds ? kLoopLds : kStoreLds;
-    // eight waves, two on each SIMD: they work half a step apart
-    static constexpr bool kTwo = kWaves == 8;
-    static_assert(!kTwo || WM == 2, "the two halves are the waves 0 .. 3 and 4 .. 7");
-    // what a wave issues in step j (mod 4): scales of the next group, a pair, a step of weights, in this order
-    static constexpr int issued(int j) { return PW + ((j & 1) == 0 ? PA : 0) + ((j & 3) == 0 ? PS : 0); }
-    static constexpr int issued(int from, int to) { return from > to ? 0 : issued(from) + issued(from + 1, to); }
-    // DMAs younger than those that step k (mod 4, plus a multiple of 4) reads
-    static constexpr int younger(int k) {
-        const int w = issued(k - NS + 2, k - 1), a = PW + issued(k - 2 * (NA - 1) + 1, k - 1);
-        return (k & 1) == 0 && a < w ? a : w;
-    }
-    static_assert(NS >= 3 && NS <= 4 && NA >= 2 && NA <= 3, "the waits below hold for these");
-};
-
-// s_waitcnt vmcnt(n)
-template <int N>
-__device__ __forceinline__ void vm_wait() {
-    static_assert(N >= 0 && N < 64, "vmcnt has six bits");
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-
-// the value exists here, in registers (no instruction)
-__device__ __forceinline__ void pin(uint32_t& v) { asm volatile("" : "+v"(v)); }
-__device__ __forceinline__ void pin(mx_v16f& v) { asm volatile("" : "+v"(v)); }
-__device__ __forceinline__ void pin(uint4& a, uint4& b) {
-    asm volatile("" : "+v"(a.x), "+v"(a.y), "+v"(a.z), "+v"(a.w), "+v"(b.x), "+v"(b.y), "+v"(b.z), "+v"(b.w));
-}
-template <int I, int N, class F>
-__device__ __forceinline__ void static_for(F f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<I + 1, N>(f);
-    }
-}
-
-// rows(r): the activation row of tile row r.  acc[f][j]: weight rows 32 f.., activation rows 32 j.. of this wave
-template <int MF, int NF, int WM, int WN, int NS, int NA, class Rows>
-__device__ __forceinline__ void mx_tile(uint8_t* smem, const uint8_t* W, qmm_xmx x, int strip0, int nstrips, int K128, Rows rows, mx_v16f (&acc)[NF][MF]) {
-    using T = MxTile<MF, NF, WM, WN, NS, NA>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wn = wave % WN, wm = wave / WN, half = lane >> 5;
-    const uint32_t lds = lds_addr(smem);
-
-    // this wave's pieces (where the waves do not divide them, the last one is fetched more than once): eight
-    // activation rows, a strip, 64 rows' scales (16 bytes; the last group of a row starts at step K128 - 4, so that
-    // it ends with the row) or four strips' scales (256 bytes)
-    const uint8_t* ap[T::PA];
-    uint32_t adst[T::PA];
-    bool late[T::PA];                                    // the lane's chunk is of the pair's second step
-#pragma unroll
-    for (int i = 0; i < T::PA; ++i) {
-        const int p = min(wave + i * T::kWaves, T::kAPieces - 1), r = 8 * p + (lane >> 3), c = (lane & 7) ^ a_swz(r);
-        adst[i] = lds + (uint32_t)p * 1024u;
-        ap[i] = x.q + (size_t)rows(r) * K128 * 64 + c * 16;
-        late[i] = c >= 4;
-    }
-    const uint8_t* wp[T::PW];
-    uint32_t wdst[T::PW];
-#pragma unroll
-    for (int i = 0; i < T::PW; ++i) {
-        const int p = min(wave + i * T::kWaves, T::kWPieces - 1);
-        wdst[i] = lds + T::kWAt + (uint32_t)p * 1024u;
-        wp[i] = W + (size_t)min(strip0 + p, nstrips - 1) * mx_strip_bytes(K128) + lane * 16;
-    }
-    const uint8_t* sp[T::PS];
-    uint32_t sdst[T::PS];
-    bool srow[T::PS];
-#pragma unroll
-    for (int i = 0; i < T::PS; ++i) {
-        const int p = min(wave + i * T::kWaves, T::kScPieces - 1);
-        sdst[i] = lds + T::kScAt + (uint32_t)p * 1024u;
-        srow[i] = p < T::kRowSc;
-        if (srow[i]) sp[i] = x.e + (size_t)rows(min(64 * p + lane, T::kRows - 1)) * K128 * 4;
-        else sp[i] = W + (size_t)min(strip0 + min(4 * (p - T::kRowSc) + (lane >> 4), T::kCols / 16 - 1), nstrips - 1) * mx_strip_bytes(K128) +
-                     (uint32_t)K128 * 1024u + (lane & 15) * 16;
-    }
-    auto issue_a = [&](int i, int pair, int buf) {       // piece i of a pair
-        const bool odd = 2 * pair + 1 >= K128;           // the pair's second step does not exist: the first again
-        dma16(ap[i] - (odd && late[i] ? 64 : 0), adst[i] + buf * T::kABytes);
-        ap[i] += 128;
-    };
-    auto issue_w = [&](int i, int buf) {
-        dma16(wp[i], wdst[i] + buf * T::kWBytes);
-        wp[i] += 1024;
-    };
-    auto issue_s = [&](int i, int g) {
-        const uint32_t off = srow[i] ? (uint32_t)max(min(4 * g, K128 - 4), 0) * 4u : (uint32_t)g * 256u;
-        if (!srow[i] || K128 >= 4) dma16(sp[i] + off, sdst[i] + (g & 1) * T::kScBytes);
-    };
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int j = 0; j < MF; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[f][j][e] = 0.f;
-
-    if (K128 < 4) {                                      // rows shorter than a 16-byte piece of scales
-        for (int i = tid; i < T::kRows * K128; i += 64 * T::kWaves) {
-            const int r = i / K128, s = i - r * K128;
-            *(uint32_t*)(smem + T::kScAt + r * 16 + s * 4) = *(const uint32_t*)(x.e + ((size_t)rows(r) * K128 + s) * 4);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < T::PS; ++i) issue_s(i, 0);
-#pragma unroll
-    for (int p = 0; p < NA - 1; ++p)
-        if (2 * p < K128)
-#pragma unroll
-            for (int i = 0; i < T::PA; ++i) issue_a(i, p, p);
-#pragma unroll
-    for (int k = 0; k < NS - 1; ++k)
-        if (k < K128)
-#pragma unroll
-            for (int i = 0; i < T::PW; ++i) issue_w(i, k);
-
-    const int r0 = wm * 32 * MF + (lane & 31), sw = a_swz(r0);                      // rows 32 apart: the same rotation
-    const uint32_t a_at = (uint32_t)r0 * 128u;
-    const uint32_t w_at = (uint32_t)(2 * wn * NF + ((lane >> 4) & 1)) * 1024u + (uint32_t)(half * 16 + (lane & 15)) * 16u;
-    const uint32_t ws_at = (uint32_t)T::kScAt + T::kRowSc * 1024u + (uint32_t)(2 * wn * NF + ((lane >> 4) & 1)) * 256u +
-                           (uint32_t)(half * 16 + (lane & 15)) * 4u;
-    uint32_t ws[NF][2];
-    int wbuf = 0, abuf = 0;
-    // Everything that step k reads has landed in this wave's part.  S = k % 4 in the steady groups, where every DMA
-    // exists and the wait is a constant; S = -1 for the first group and the last steps: at the start the pairs came
-    // before the weights and near the end nothing new was issued, so only the weights of the steps after this one
-    // may still be out (they are younger than everything that it reads).
-    auto landed = [&](auto sc, int k) {
-        constexpr int S = decltype(sc)::value;
-        if constexpr (S >= 0) vm_wait<T::younger(S + 8)>();
-        else if (K128 >= 4 && k + NS - 2 < K128) vm_wait<(NS - 2) * T::PW>();
-        else if (K128 >= 4 && NS == 4 && k + 1 < K128) vm_wait<T::PW>();
-        else vm_wait<0>();
-    };
-    using Next = std::integral_constant<int, -1>;
-    auto step = [&](auto sc, auto nc, int k) {           // nc: S of the step after this one
-        constexpr int S = decltype(sc)::value;
-        constexpr bool kSteady = S >= 0;
-        const int g = k >> 2;
-        if constexpr (!T::kTwo) {
-            landed(sc, k);
-            lds_barrier();
-        }
-        const int an = abuf == 0 ? NA - 1 : abuf - 1, wn_ = wbuf == 0 ? NS - 1 : wbuf - 1;
-        // the step's DMAs: part B of P
-        auto issue = [&](auto bc, auto pc) {
-            constexpr int B = decltype(bc)::value, P = decltype(pc)::value;
-            constexpr int nS = S <= 0 ? T::PS : 0, nA = !kSteady || (S & 1) == 0 ? T::PA : 0, n = nS + nA + T::PW;
-            constexpr int lo = B * n / P, hi = (B + 1) * n / P;
-#pragma unroll
-            for (int i = lo; i < hi; ++i) {
-                if (i < nS) { if (kSteady || ((k & 3) == 0 && k + 4 < K128)) issue_s(i, g + 1); }
-                else if (i < nS + nA) { if (kSteady || ((k & 1) == 0 && k + 2 * (NA - 1) < K128)) issue_a(i - nS, (k >> 1) + NA - 1, an); }
-                else { if (kSteady || k + NS - 1 < K128) issue_w(i - nS - nA, wn_); }
-            }
-        };
-        const uint8_t* sa_ = smem + abuf * T::kABytes + a_at;
-        const uint8_t* sw_ = smem + T::kWAt + wbuf * T::kWBytes + w_at;
-        const uint32_t so = (uint32_t)(g & 1) * T::kScBytes;
-        if constexpr (S <= 0) {
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    ws[f][h] = *(const uint32_t*)(smem + ws_at + so + f * 512 + h * 128);
-                    if constexpr (!kSteady) ws[f][h] >>= 8 * (k & 3);
-                }
-        }
-        const int c0 = 4 * (k & 1) + half;               // the lane's first block
-        const uint8_t* sa_row = smem + T::kScAt + so + r0 * 16 + 4 * (k - max(min(4 * g, K128 - 4), 0));
-        uint4 w[NF][2], a[MF][2];
-        uint32_t sa[MF];
-        auto read_a = [&](int j) {
-            a[j][0] = *(const uint4*)(sa_ + j * 4096 + ((c0 ^ sw) << 4));
-            a[j][1] = *(const uint4*)(sa_ + j * 4096 + (((c0 + 2) ^ sw) << 4));
-            // the step's four scale bytes, this lane's two in bytes 0 and 2
-            sa[j] = *(const uint32_t*)(sa_row + j * 512) >> (8 * half);
-        };
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[f][h] = *(const uint4*)(sw_ + f * 2048 + h * 512);
-        if constexpr (T::kTwo) {
-#pragma unroll
-            for (int j = 0; j < MF; ++j) read_a(j);
-            issue(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{});
-            // the compiler would move the reads and the products to where they suit it: they stay in their phases
-#pragma unroll
-            for (int f = 0; f < NF; ++f) pin(w[f][0], w[f][1]);
-#pragma unroll
-            for (int j = 0; j < MF; ++j) { pin(a[j][0], a[j][1]); pin(sa[j]); }
-            if (wm != 0) landed(nc, k + 1);
-            lds_barrier();
-            __builtin_amdgcn_s_setprio(1);
-        }
-        static_for<0, MF>([&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            if constexpr (!T::kTwo) read_a(j);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 0>(w[f][0], a[j][0], acc[f][j], ws[f][0], sa[j]);
-            if constexpr (!T::kTwo) issue(std::integral_constant<int, 2 * j>{}, std::integral_constant<int, 2 * MF>{});
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<kSteady ? S : 0, 2>(w[f][1], a[j][1], acc[f][j], ws[f][1], sa[j]);
-            if constexpr (!T::kTwo) issue(std::integral_constant<int, 2 * j + 1>{}, std::integral_constant<int, 2 * MF>{});
-        });
-        if constexpr (T::kTwo) {
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-                for (int j = 0; j < MF; ++j) pin(acc[f][j]);
-            __builtin_amdgcn_s_setprio(0);
-            if (wm == 0) landed(nc, k + 1);
-            lds_barrier();
-        }
-        wbuf = wbuf == NS - 1 ? 0 : wbuf + 1;
-        if (k & 1) abuf = abuf == NA - 1 ? 0 : abuf + 1;
-    };
-    if constexpr (T::kTwo) {
-        landed(Next{}, 0);
-        lds_barrier();
-        if (wm != 0) lds_barrier();                      // half a step behind
-    }
-    int k = 0;
-    const int first = min(4, K128);
-    for (; k < first; ++k) step(Next{}, Next{}, k);
-    for (; k + 8 <= K128; k += 4) {                      // every DMA of these steps exists: the last reaches step k + 7
-        step(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, k);
-        step(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, k + 1);
-        step(std::integral_constant<int, 2>{}, std::integral_constant<int, 3>{}, k + 2);
-        step(std::integral_constant<int, 3>{}, std::integral_constant<int, 0>{}, k + 3);
-    }
-    for (; k < K128; ++k) step(Next{}, Next{}, k);
-    if constexpr (T::kTwo)
-        if (wm == 0) lds_barrier();
-    // The matrix unit writes its result after the instruction, and a read of it before then is not held up: the
-    // compiler counts the wait states, but was seen to count too few where branches around the DMAs come between
-    // (element 15 of an accumulator read stale).  Nothing reads an accumulator before this.
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int j = 0; j < MF; ++j) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[f][j]));
-}
-
-// The wave's outputs through its part of LDS, 32 activation rows at a time, so that they leave as 16-byte pieces of
-// whole row segments (64 bytes to 384; stored straight from the accumulators, 8 bytes of each of 32 rows at a time, they
-// took as long as the loop: 34 us of 132).  row(r): the output row of the wave's activation row r, below 0: none.
-template <int MF, int NF, bool BF, class Row>
-__device__ __forceinline__ void mx_store(uint8_t* smem, const mx_v16f (&acc)[NF][MF], void* D, int n0, int N, int vec, Row row) {
-    constexpr int kSize = BF ? 2 : 4, kPer = 16 / kSize, kRow = 32 * NF * kSize, kStride = kRow + 16, kPieces = kRow / 16;
-    const int lane = threadIdx.x & 63;
-    uint8_t* buf = smem + (threadIdx.x >> 6) * 32 * kStride;
-    __syncthreads();                                     // every wave is done with the operands
-#pragma unroll
-    for (int j = 0; j < MF; ++j) {
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint8_t* d = buf + (lane & 31) * kStride + (32 * f + 8 * e + 4 * (lane >> 5)) * kSize;
-                const mx_v16f& v = acc[f][j];
-                if constexpr (BF) *(uint2*)d = make_uint2(mx_bf16x2(v[4 * e], v[4 * e + 1]), mx_bf16x2(v[4 * e + 2], v[4 * e + 3]));
-                else *(mx_v4f*)d = mx_v4f{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
-            }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own writes, read by its other lanes
-#pragma unroll
-        for (int i = 0; i < 32 * kPieces / 64; ++i) {
-            const int p = lane + 64 * i, r = p / kPieces, c = p - r * kPieces, n = n0 + c * kPer;
-            const uint4 v = *(const uint4*)(buf + r * kStride + c * 16);
-            const int64_t m = row(32 * j + r);
-            if (m < 0 || n >= N) continue;
-            uint8_t* d = (uint8_t*)D + ((size_t)m * N + n) * kSize;
-            if (vec) {
-                *(uint4*)d = v;
-            } else {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int q = 0; q < kPer; ++q)
-                    if (n + q < N) {
-                        if constexpr (BF) ((uint16_t*)d)[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
-                        else ((uint32_t*)d)[q] = w[q];
-                    }
-            }
-        }
-        asm volatile("" ::: "memory");                   // reads before the next rows' writes (LDS is in order)
-    }
-}
-
-template <int MF, int NF, int WM, int WN, int NS, int NA, bool BF>
-__global__ void __launch_bounds__(64 * WM * WN, 2) k_gemm_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ D, int M, int N, int K128,
-                                                                int mtiles, int panel, int vec) {
-    using T = MxTile<MF, NF, WM, WN, NS, NA>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    // workgroup i runs on XCD i % 8: each XCD takes a contiguous range of tiles, rows fastest, so that the
-    // tiles it runs together share weight strips in its L2
+// GEMM.  Workgroup i runs on XCD i % 8: each XCD takes a contiguous range of tiles, rows fastest, so that the tiles
+// it runs together share weight strips in its L2.
+__device__ __forceinline__ uint32_t xcd_tile() {
     const uint32_t total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, rem = total & 7;
-    const uint32_t t = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
-    const uint32_t ntiles = total / (uint32_t)mtiles, pan = t / (panel * ntiles), left = t - pan * panel * ntiles;
-    const uint32_t pm = min((uint32_t)panel, (uint32_t)mtiles - pan * panel);
-    const int m0 = (int)(pan * panel + left % pm) * T::kRows, n0 = (int)(left / pm) * T::kCols;
+    return xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
+}
+
+template <int MF, int NF, int D, int PER, bool BF>
+__global__ void __launch_bounds__(256, PER) k_gemm_mxfp4_reg(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ Dst, int M, int N, int K128,
+                                                             int mtiles, int vec) {
+    using T = MxReg<MF, NF>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t t = xcd_tile();
+    const int m0 = (int)(t % (uint32_t)mtiles) * T::kRows, n0 = (int)(t / (uint32_t)mtiles) * T::kCols;
     mx_v16f acc[NF][MF];
-    mx_tile<MF, NF, WM, WN, NS, NA>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
-    const int wave = threadIdx.x >> 6, mw = m0 + 32 * MF * (wave / WN);
-    mx_store<MF, NF, BF>(smem, acc, D, n0 + 32 * NF * (wave % WN), N, vec, [&](int r) { return mw + r < M ? (int64_t)(mw + r) : -1; });
+    mx_tile_reg<MF, NF, D, PER == 1>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
+    mx_store<MF, NF, BF>(smem, acc, Dst, n0 + 32 * NF * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return m0 + r < M ? (int64_t)(m0 + r) : -1; });
+}
+
+template <int MF, int NF, int NS, bool BF>
+__global__ void __launch_bounds__(512, 2) k_gemm_mxfp4_dma(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ Dst, int M, int N, int K128,
+                                                           int mtiles, int vec) {
+    using T = MxDma<MF, NF, NS>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t t = xcd_tile();
+    const int m0 = (int)(t % (uint32_t)mtiles) * T::kRows, n0 = (int)(t / (uint32_t)mtiles) * T::kCols;
+    mx_v16f acc[NF][MF];
+    mx_tile_dma<MF, NF, NS>(smem, W, x, n0 / 16, (N + 15) / 16, K128, [&](int r) { return min(m0 + r, M - 1); }, acc);
+    const int wave = threadIdx.x >> 6, mw = m0 + 32 * MF * (wave >> 2);
+    mx_store<MF, NF, BF>(smem, acc, Dst, n0 + 32 * NF * (wave & 3), N, vec, [&](int r) { return mw + r < M ? (int64_t)(mw + r) : -1; });
 }
 
 // Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 64 at a time, with as
 // many 32-row fragments as they need.
-constexpr int kMoeNS = 4, kMoeNA = 3, kMoeCols = 128, kMoeRows = 64;
+constexpr int kMoeNF = 1, kMoeD = 8, kMoeCols = 128 * kMoeNF, kMoeRows = 64;
 
 template <int MF, bool BF>
 __device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_xmx x, const int* rowtab, int k0, int n, int n0, void* D, int N, int K128,
                                          int vec) {
-    mx_v16f acc[1][MF];
-    mx_tile<MF, 1, 1, 4, kMoeNS, kMoeNA>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
+    mx_v16f acc[kMoeNF][MF];
+    mx_tile_reg<MF, kMoeNF, kMoeD, false>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
         const int k = k0 + min(r, n - 1);
         return rowtab ? rowtab[k] : k;
     }, acc);
-    mx_store<MF, 1, BF>(smem, acc, D, n0 + 32 * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return r < n ? (int64_t)(k0 + r) : -1; });
+    mx_store<MF, kMoeNF, BF>(smem, acc, D, n0 + 32 * kMoeNF * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return r < n ? (int64_t)(k0 + r) : -1; });
 }
 
 template <bool BF>
@@ -543,7 +245,7 @@ __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __rest
         const int n = min(t.ncols - r, kMoeRows);
         if (n <= 32) moe_rows<1, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
         else moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        __syncthreads();                                 // the ring is filled again
+        __syncthreads();                                 // LDS is filled again
     }
 }
 
@@ -561,25 +263,61 @@ int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int N, in
 int vec_out(const void* y, int dtype, int N) { return N % 4 == 0 && !misaligned(y, dtype == QMM_BF16 ? 8 : 16); }
 int vec16_out(const void* y, int dtype, int N) { return N % (dtype == QMM_BF16 ? 8 : 4) == 0 && !misaligned(y, 16); }
 
-constexpr int64_t kPanelBytes = 5 << 19;
+struct GemmCall { const uint8_t* W; qmm_xmx x; void* D; int dtype, M, N, K128; hipStream_t s; };
 
-template <int MF, int NF, int WM, int WN, int NS, int NA>
-int launch_gemm(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K128, hipStream_t s) {
-    using T = MxTile<MF, NF, WM, WN, NS, NA>;
-    static_assert(T::kLds <= 160 * 1024, "LDS of a CU");
-    const int64_t mt = ((int64_t)M + T::kRows - 1) / T::kRows, nt = ((int64_t)N + T::kCols - 1) / T::kCols;
+template <class T, class F>
+int launch_tiles(const GemmCall& c, F f) {
+    const int64_t mt = ((int64_t)c.M + T::kRows - 1) / T::kRows, nt = ((int64_t)c.N + T::kCols - 1) / T::kCols;
     if (mt * nt > 0x7fffffff) return QMM_ERR_SHAPE;
-    const dim3 grid((unsigned)(mt * nt)), block(64 * T::kWaves);
-    const int64_t fit = std::max<int64_t>(1, kPanelBytes / ((int64_t)T::kRows * K128 * 64)), np = (mt + fit - 1) / fit;
-    const int panel = (int)((mt + np - 1) / np);
-    if (dtype == QMM_BF16)
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, true>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, panel,
-                           vec16_out(D, dtype, N));
-    else
-        hipLaunchKernelGGL((k_gemm_mxfp4<MF, NF, WM, WN, NS, NA, false>), grid, block, T::kLds, s, (const uint8_t*)W, x, D, M, N, K128, (int)mt, panel,
-                           vec16_out(D, dtype, N));
+    f(dim3((unsigned)(mt * nt)), (int)mt, vec16_out(c.D, c.dtype, c.N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
+}
+template <int MF, int NF, int D, int PER>
+int launch_reg(const GemmCall& c) {
+    using T = MxReg<MF, NF>;
+    static_assert(T::kLds * PER <= 160 * 1024, "LDS of a CU");
+    return launch_tiles<T>(c, [&](dim3 grid, int mt, int vec) {
+        if (c.dtype == QMM_BF16)
+            hipLaunchKernelGGL((k_gemm_mxfp4_reg<MF, NF, D, PER, true>), grid, dim3(256), T::kLds, c.s, c.W, c.x, c.D, c.M, c.N, c.K128, mt, vec);
+        else
+            hipLaunchKernelGGL((k_gemm_mxfp4_reg<MF, NF, D, PER, false>), grid, dim3(256), T::kLds, c.s, c.W, c.x, c.D, c.M, c.N, c.K128, mt, vec);
+    });
+}
+template <int MF, int NF, int NS>
+int launch_dma(const GemmCall& c) {
+    using T = MxDma<MF, NF, NS>;
+    static_assert(T::kLds <= 160 * 1024, "LDS of a CU");
+    return launch_tiles<T>(c, [&](dim3 grid, int mt, int vec) {
+        if (c.dtype == QMM_BF16)
+            hipLaunchKernelGGL((k_gemm_mxfp4_dma<MF, NF, NS, true>), grid, dim3(512), T::kLds, c.s, c.W, c.x, c.D, c.M, c.N, c.K128, mt, vec);
+        else
+            hipLaunchKernelGGL((k_gemm_mxfp4_dma<MF, NF, NS, false>), grid, dim3(512), T::kLds, c.s, c.W, c.x, c.D, c.M, c.N, c.K128, mt, vec);
+    });
+}
+
+// The tiles, and what a GEMM takes on each, in microseconds: a + steps (b + c (rounds - 1) + d load), rounds =
+// ceil(tiles / 256 CUs), load = tiles / 256.  Fitted to 108 shapes (M 65 .. 4096, N 512 .. 17408, K 2048, 5120, 17408; mean
+// error 2 to 10 %); the tile that it names takes 0.4 % more than the best of the seven on (geometric) average, 10 % at
+// most.  Fewer tiles cost more: without the two DMA tiles 1.6 % (22 % at 4096 x 17408 x 2048), without 96 x 128 and 64 x 256 1 %
+// (23 % at 512 x 5120 x 5120).
+struct MxTileCost { int rows, cols; float a, b, c, d; int (*launch)(const GemmCall&); };
+const MxTileCost kMxTiles[] = {
+    {192, 384, 7.42f, 0.736f, 1.116f, 0.254f, launch_dma<3, 3, 3>}, {192, 256, 6.49f, 0.572f, 0.850f, 0.192f, launch_dma<3, 2, 4>},
+    {128, 256, 5.48f, 0.415f, 0.558f, 0.185f, launch_reg<4, 2, 4, 1>}, {96, 128, 4.11f, 0.225f, 0.245f, 0.065f, launch_reg<3, 1, 8, 2>},
+    {64, 256, 3.64f, 0.289f, 0.265f, 0.126f, launch_reg<2, 2, 4, 2>}, {64, 128, 4.00f, 0.180f, 0.208f, 0.051f, launch_reg<2, 1, 8, 2>},
+    {32, 128, 4.22f, 0.129f, 0.134f, 0.028f, launch_reg<1, 1, 8, 2>},
+};
+
+const MxTileCost& pick_tile(int M, int N, int K128) {
+    const MxTileCost* best = nullptr;
+    float least = 0.f;
+    for (const MxTileCost& t : kMxTiles) {
+        const float tiles = (float)(((int64_t)M + t.rows - 1) / t.rows) * (float)(((int64_t)N + t.cols - 1) / t.cols);
+        const float cost = t.a + (float)K128 * (t.b + t.c * (ceilf(tiles / 256.f) - 1.f) + t.d * tiles / 256.f);
+        if (!best || cost < least) { best = &t; least = cost; }
+    }
+    return *best;
 }
 
 template <int MF>
@@ -643,10 +381,12 @@ int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, i
     if (M == 0) return QMM_OK;
     const int K128 = mx_steps(K);
     hipStream_t s = (hipStream_t)stream;
-    const auto tiles = [&](int bm, int bn) { return (((int64_t)M + bm - 1) / bm) * (((int64_t)N + bn - 1) / bn); };
-    if (tiles(192, 384) >= 200) return launch_gemm<3, 3, 2, 4, 3, 2>(W, x, D, dtype, M, N, K128, s);
-    if (tiles(128, 128) >= 256) return launch_gemm<2, 2, 2, 2, 3, 2>(W, x, D, dtype, M, N, K128, s);
-    return launch_gemm<2, 1, 1, 4, 4, 2>(W, x, D, dtype, M, N, K128, s);
+    return pick_tile(M, N, K128).launch(GemmCall{(const uint8_t*)W, x, D, dtype, M, N, K128, s});
+}
+
+int qmm_gemm_mxfp4_tile(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
+    return (int)(&pick_tile(M, N, mx_steps(K)) - kMxTiles);
 }
 
 int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
@@ -661,7 +401,7 @@ int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_
     if ((uint64_t)nblocks * max_tiles > 0x7fffffffu) return QMM_ERR_SHAPE;
     const int K128 = mx_steps(K);
     const dim3 grid(nblocks * (uint32_t)max_tiles);
-    constexpr size_t lds = MxTile<2, 1, 1, 4, kMoeNS, kMoeNA>::kLds;
+    constexpr size_t lds = MxReg<kMoeRows / 32, kMoeNF>::kLds;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == QMM_BF16)
         hipLaunchKernelGGL(k_moe_gemm_mxfp4<true>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,

@@ -515,6 +515,11 @@ def gemm_mxfp4(W, x, D, M, N, K, stream=None):
     check(_lib.lib().qmm_gemm_mxfp4(_weight(W, N, K), _xmx(x, M, K, "x"), _in(D, M * N, "D"), _dtype(D, "D"), M, N, K, _handle(stream)), "gemm_mxfp4")
 
 
+def gemm_mxfp4_tile(M, N, K):
+    """Index of the tile that gemm_mxfp4 runs for this shape."""
+    return _lib.lib().qmm_gemm_mxfp4_tile(M, N, K)
+
+
 def gemv_moe_mxfp4(W, Wsh, ebytes, ids, x, y, T, nslot, nexperts, N, K, xrow_te=False, stream=None):
     """y[te][n] = W_{ids[te]}[n] . x[te if xrow_te else t] for T <= 16 tokens (ids int32 [T][nslot], below 0: Wsh)."""
     slots = T * nslot

@@ -438,6 +438,8 @@ int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int*
 /* D[m][n] = W[n] . x[m] for any number of rows, D [M][N] f32 or bf16: prompts.  An output is one chain of matrix
  * instructions over K: its bits do not depend on M or N (they differ from qmm_gemv_mxfp4's, which cuts K). */
 int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K, void* stream);
+/* the tile (0 ..) that qmm_gemm_mxfp4 runs for a shape, for tests and benchmarks (the choice changes no bit) */
+int qmm_gemm_mxfp4_tile(int M, int N, int K);
 /* the same for rows sorted by expert (qmm_moe_sort): for tile i < counts[0] + counts[1] (read on the device) and
  * r < ncols: D[k0 + r] = W_e . x[rowtab ? rowtab[k0 + r] : k0 + r], W_e at W + expert * ebytes, or Wsh (W where it
  * is NULL) for expert -1.  max_tiles bounds the grid.  A row has the bits of qmm_gemm_mxfp4. */

@@ -219,6 +219,36 @@ def test_bits_do_not_depend_on_the_call(gpu):
     assert np.array_equal(bits(run_dense(qmm.gemm_mxfp4, W2, x, 700, N + 48, K, "f32"))[:, :N], m[:700])
 
 
+# shapes whose choice is each tile, with steps of 128 that end everywhere in a group of four and a pair
+TILES = [(0, 6000, 20000, 130), (0, 4000, 12300, 260), (0, 2000, 16400, 400), (0, 2000, 8200, 513), (0, 577, 20000, 900), (0, 577, 20000, 1025),
+         (0, 577, 20000, 1160), (0, 577, 16400, 2050), (1, 3000, 20000, 400), (1, 3000, 20000, 640), (1, 500, 16400, 900), (1, 385, 20000, 1025),
+         (1, 385, 20000, 1160), (1, 769, 10000, 2050), (2, 6000, 12300, 400), (2, 6000, 12300, 513), (2, 6000, 6200, 900), (2, 577, 10000, 1160),
+         (2, 700, 8200, 2050), (3, 769, 10000, 260), (3, 769, 5000, 400), (3, 200, 16400, 640), (3, 200, 8200, 1025), (4, 200, 1000, 32),
+         (4, 200, 8200, 513), (4, 200, 12300, 1160), (5, 385, 4100, 300), (5, 200, 5000, 900), (5, 200, 5000, 2050), (6, 200, 1000, 513),
+         (6, 200, 1000, 1025), (6, 200, 1000, 2180)]
+
+
+@pytest.mark.parametrize("tile,M,N,K", TILES)
+def test_gemm_every_tile(gpu, tile, M, N, K):
+    """Each tile against float64 (on the GPU: the sizes that choose the large ones), odd ends of M, N and K; and its bits
+    against those of calls of few rows, which run small tiles."""
+    assert qmm.gemm_mxfp4_tile(M, N, K) == tile
+    rng = np.random.default_rng(tile + K)
+    (ac, ab), (wc, wb) = mx_ref.random_rows(rng, M, K), mx_ref.random_rows(rng, N, K)
+    W, x = packed(wc, wb, N, K), xmx(ac, ab)
+    y = run_dense(qmm.gemm_mxfp4, W, x, M, N, K, "f32")
+    a, w = dev(mx_ref.values(ac, ab)), dev(mx_ref.values(wc, wb))
+    err = (y.double() - a @ w.t()).abs_()
+    bound = (a.abs() @ w.abs().t()) * ((mx_ref.steps(K) + 8) * 2.0 ** -23)
+    assert bool((err <= bound).all()), float((err / bound).max())
+    del err, bound
+    for r in (0, M // 2, M - 40):
+        part = run_dense(qmm.gemm_mxfp4, W, xmx(ac[r:r + 40], ab[r:r + 40]), 40, N, K, "f32")
+        assert torch.equal(part, y[r:r + 40])
+    low = run_dense(qmm.gemm_mxfp4, W, x, M, N, K, "bf16")
+    assert torch.equal(low, y.bfloat16())
+
+
 def test_output_beyond_32_bits(gpu):
     """M x N beyond 2^32 elements: the last rows are right."""
     rng = np.random.default_rng(8)
