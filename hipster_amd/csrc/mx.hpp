@@ -11,10 +11,9 @@
 //     codes  [K128][64 lanes][16 bytes]         lane l: row l % 16, block l / 16 of the step
 //     scales [ceil(K128 / 4)][64 lanes][4 bytes] the four bytes: the lane's block of four successive steps
 //
-// The strip is the operand order of v_mfma_scale_f32_16x16x128_f8f6f4: lane l supplies the 32 codes of row
-// l % 16, block l / 16, and the block's scale in one byte of a register (which byte, the instruction
-// says).  So a wave reads a weight step as one contiguous kilobyte and four steps' scales as one dword per
-// lane, with no shuffle.  The instruction's sum of 128 products is exact to f32 rounding for fp4 operands
+// The strip is in the order of the scaled matrix instructions: a lane supplies 32 codes of one row, a block, and the
+// block's scale in one byte of a register (which byte, the instruction says).  So a wave reads half a step of two
+// strips as two runs of 512 bytes and four steps' scales as one dword per lane, with no shuffle.  The instruction's sum of 128 products is exact to f32 rounding for fp4 operands
 // (measured: within 1.3 * 2^-24 of the sum of magnitudes with block scales spread over 2^+-40); fp8 operands
 // are not (products 2^15 below a group's largest are dropped), which is why activations are fp4 too.
 #pragma once
@@ -24,6 +23,7 @@ namespace qmm {
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
 typedef float mx_v4f __attribute__((ext_vector_type(4)));
+typedef float mx_v16f __attribute__((ext_vector_type(16)));
 
 constexpr int kMxMaxK = 1 << 24;                 // a strip's byte offsets stay in 32 bits
 constexpr int kMxFp4 = 4;                        // the instruction's number for e2m1
@@ -43,18 +43,9 @@ __device__ __forceinline__ uint32_t mx_codes2(uint32_t old, float lo, float hi) 
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, lo, hi, 1.f, B);
 }
 
-// acc += W . A^T over one step of 128: w and a the two operands' 16 bytes, sw / sa their scales (byte BW of
-// sw, byte 0 of sa).  acc[i] of lane l: weight row 4 (l / 16) + i, activation row l % 16.
-template <int BW>
-__device__ __forceinline__ mx_v4f mx_mfma(const uint4& w, const uint4& a, mx_v4f acc, uint32_t sw, uint32_t sa) {
-    const mx_v8i vw = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
-    const mx_v8i va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vw, va, acc, kMxFp4, kMxFp4, BW, (int)sw, 0, (int)sa);
-}
-
-// the same on 32 x 32 x 64: lane l supplies row l % 32, block l / 32 of a half step; byte BW of sw, byte BA of sa;
-// acc[e] of lane l: weight row 8 (e / 4) + 4 (l / 32) + e % 4, activation row l % 32
-typedef float mx_v16f __attribute__((ext_vector_type(16)));
+// acc += W . A^T over half a step (64 values), 32 x 32: w and a the two operands' 16 bytes (lane l: row l % 32, block
+// l / 32 of the half), their scales in byte BW of sw and byte BA of sa.  acc[e] of lane l: weight row
+// 8 (e / 4) + 4 (l / 32) + e % 4, activation row l % 32.
 template <int BW, int BA>
 __device__ __forceinline__ mx_v16f mx_mfma32(const uint4& w, const uint4& a, mx_v16f acc, uint32_t sw, uint32_t sa) {
     const mx_v8i vw = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};

@@ -5,23 +5,27 @@
 //   qmm_gemm_mxfp4       any number of rows: prompts
 //   qmm_moe_gemm_mxfp4   rows sorted by expert (qmm_moe_sort)
 //
-// A scaled matrix instruction multiplies weight rows by activation rows with their block scales and adds to
-// f32: 16 x 16 over 128 values in the GEMV (few rows), 32 x 32 over 64 in the GEMM (6.4 PFLOP/s measured from
-// registers against 5.4 for the former: it reads half the operand bytes per product).  The weight is the first
-// operand, so a lane ends with four successive outputs of one activation row.
+// v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 32 weight rows by 32 activation rows over 64 values with their block
+// scales and adds to f32 (16 x 16 over 128 reads twice the operand bytes per product: 5.4 against 6.4 PFLOP/s from
+// registers).  The weight is the first operand, so a lane ends with runs of four successive outputs of one
+// activation row.
 //
 // Order of sums.  GEMM: an output is one chain of instructions over K, whatever the tile, M or N.  GEMV: K's groups of four steps are cut into S contiguous runs, S chosen by K alone; each run is one chain
 // and the S sums are added in order.  So an output's bits depend on its own rows and K, not on the call.
 #include "mx_tile.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace qmm {
 namespace {
 
 // ------------------------------------------------------------------------------------------
-// GEMV.  A workgroup is one strip (16 weight rows), its S waves the runs of K: a weight byte is read once, by
-// contiguous kilobytes, straight into the operand registers, two groups (8 KB a wave) ahead.
+// GEMV.  A workgroup is two strips (32 weight rows), its S waves the runs of K.  A wave reads its weights straight into
+// the operand registers, by kilobytes, two steps (a pair) at a time, the next pair in flight while one is multiplied.
+// The activation rows beside them come as whole 128-byte lines (a pair of a row, eight lanes) and turn into operands in
+// LDS that is the wave's own: loaded in operand order, 16 bytes of 32 rows at a time, four loads touch each line, and the
+// vector cache holds every load up whose line is still on its way (64 rows x 17408 x 5120: 66 us that way).
 constexpr int kGemvMaxWaves = 8, kGemvMaxRows = 64;
 
 // S for G groups: one wave a group up to 8, else the count of 4 .. 8 that leaves the least imbalance
@@ -33,115 +37,147 @@ int gemv_waves(int G) {
     return best;
 }
 
-template <int MF>
-struct GemvGroup {
-    uint4 w[4], a[MF][4];
-    uint32_t ws, as[MF][4];
-};
+// QN: eights of activation rows that are loaded (1, 2, 4 or 8), MF fragments of 32
+template <int QN> constexpr int gemv_mf() { return QN == 8 ? 2 : 1; }
+// LDS of one wave: a pair of 32 MF rows, and a group's scales of them (16 bytes a row)
+template <int QN> constexpr int gemv_wave_lds() { return 32 * gemv_mf<QN>() * (128 + 16); }
 
-template <int MF>
-__device__ __forceinline__ void gemv_load(GemvGroup<MF>& r, const uint8_t* strip, const uint8_t* const (&qr)[MF], const uint8_t* const (&er)[MF],
-                                          int g, int K128, int lane) {
-    const uint8_t* ws = strip + (uint32_t)K128 * 1024u;
+// this wave's run of K: weight rows of `strip` and the next strip (sb bytes on, or 0 where there is none); row(r):
+// the activation row of tile row r, of which n are real.  No branch lies around a load (the compiler would wait for
+// every load in flight where the paths meet): the last group is a body of its own.
+template <int QN, class Row>
+__device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uint32_t sb, qmm_xmx x, int n, Row row, int K128, int S, int wave,
+                                         mx_v16f (&acc)[1][gemv_mf<QN>()]) {
+    constexpr int MF = gemv_mf<QN>();
+    const int lane = threadIdx.x & 63, half = lane >> 5, G = mx_groups(K128), last = K128 - 1;
+    const int g0 = wave * G / S, g1 = (wave + 1) * G / S;
+    const uint8_t* wp = strip + ((lane & 16) ? sb : 0u);
+    const uint32_t slot = (uint32_t)(half * 16 + (lane & 15));
+    const uint8_t* qp[QN];                               // chunk lane % 8 of rows lane / 8 + 8 i
+    const int cj = lane & 7;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const uint32_t kt = (uint32_t)min(4 * g + s, K128 - 1);      // a short last group re-reads its last step, unused
-        r.w[s] = ld16(strip + kt * 1024u + lane * 16);
-    }
-    r.ws = *(const uint32_t*)(ws + (uint32_t)g * 256u + lane * 4);
+    for (int i = 0; i < QN; ++i) qp[i] = x.q + (size_t)row(min(8 * i + (lane >> 3), n - 1)) * K128 * 64 + (cj & 3) * 16;
+    const int er = MF == 2 ? lane : lane & 31;           // the row whose scales this lane brings
+    const uint8_t* ep = x.e + (size_t)row(min(er, n - 1)) * K128 * 4;
+    struct Pair { uint4 w[2][2], a[QN]; };
+    struct Scales { uint32_t w[2], a[4]; };
+    auto load = [&](Pair& r, int p) {                    // a step past the end re-reads the last one, unused
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) r.w[s][h] = ld16(wp + (uint32_t)min(2 * p + s, last) * 1024u + slot * 16u + h * 512u);
+        const uint32_t off = (uint32_t)min(2 * p + (cj >> 2), last) * 64u;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) r.a[i] = ld16(qp[i] + off);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load_s = [&](Scales& r, int g) {
+        const uint32_t sc = (uint32_t)K128 * 1024u + (uint32_t)g * 256u + slot * 4u;
+        r.w[0] = *(const uint32_t*)(wp + sc);
+        r.w[1] = *(const uint32_t*)(wp + sc + 128u);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) r.a[s] = *(const uint32_t*)(ep + 4u * (uint32_t)min(4 * g + s, last));
+    };
+    const int fr = lane & 31, sw = a_swz(fr);
+    uint8_t* es = lds + 32 * MF * 128;
+    // the products of pair P of a group, `steps` (1 or 2) of them
+    auto mul = [&](const Pair& r, const Scales& sc, auto pc, int steps) {
+        constexpr int P = decltype(pc)::value;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int q = 8 * i + (lane >> 3);
+            *(uint4*)(lds + q * 128 + ((cj ^ a_swz(q)) << 4)) = r.a[i];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (s == steps) break;
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                const uint8_t* d = lds + (fr + 32 * f) * 128;
+                const uint4 a0 = *(const uint4*)(d + (((4 * s + half) ^ sw) << 4)), a1 = *(const uint4*)(d + (((4 * s + 2 + half) ^ sw) << 4));
+                const uint32_t sa = *(const uint32_t*)(es + (fr + 32 * f) * 16 + 4 * (2 * P + s)) >> (8 * half);
+                if (s == 0) {
+                    acc[0][f] = mx_mfma32<2 * P, 0>(r.w[0][0], a0, acc[0][f], sc.w[0], sa);
+                    acc[0][f] = mx_mfma32<2 * P, 2>(r.w[0][1], a1, acc[0][f], sc.w[1], sa);
+                } else {
+                    acc[0][f] = mx_mfma32<2 * P + 1, 0>(r.w[1][0], a0, acc[0][f], sc.w[0], sa);
+                    acc[0][f] = mx_mfma32<2 * P + 1, 2>(r.w[1][1], a1, acc[0][f], sc.w[1], sa);
+                }
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < MF; ++f) pin<false>(acc[0][f]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
     for (int f = 0; f < MF; ++f)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint32_t kt = (uint32_t)min(4 * g + s, K128 - 1);
-            r.a[f][s] = ld16(qr[f] + kt * 64u);
-            r.as[f][s] = er[f][kt * 4u];
+        for (int e = 0; e < 16; ++e) acc[0][f][e] = 0.f;
+    if (g0 < g1) {
+        Pair r0, r1;
+        Scales sc;
+        load_s(sc, g0);
+        load(r0, 2 * g0);
+        load(r1, 2 * g0 + 1);
+        for (int g = g0; g < g1 - 1; ++g) {
+            *(uint4*)(es + er * 16) = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
+            const Scales now = sc;
+            load_s(sc, g + 1);
+            mul(r0, now, std::integral_constant<int, 0>{}, 2);
+            load(r0, 2 * g + 2);
+            mul(r1, now, std::integral_constant<int, 1>{}, 2);
+            load(r1, 2 * g + 3);
         }
+        const int left = K128 - 4 * (g1 - 1);            // steps of the last group (beyond 4: whole)
+        *(uint4*)(es + er * 16) = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
+        mul(r0, sc, std::integral_constant<int, 0>{}, min(left, 2));
+        if (left > 2) mul(r1, sc, std::integral_constant<int, 1>{}, min(left - 2, 2));
+    }
+    settle<false>(acc);
 }
 
+// The S runs' sums, added in order: item i = 4 (64 f + lane) + e of the tile, four outputs each (weight rows 8 e ..)
 template <int MF>
-__device__ __forceinline__ void gemv_mul(const GemvGroup<MF>& r, mx_v4f (&acc)[MF], int g, int K128) {
-    const int n = K128 - 4 * g;                          // steps left (uniform)
+__device__ __forceinline__ void gemv_reduce(mx_v4f* red, const mx_v16f (&acc)[1][MF], int wave) {
+    __syncthreads();                                     // the same LDS held the waves' operands
 #pragma unroll
-    for (int f = 0; f < MF; ++f) acc[f] = mx_mfma<0>(r.w[0], r.a[f][0], acc[f], r.ws, r.as[f][0]);
-    if (n > 1) {
+    for (int f = 0; f < MF; ++f)
 #pragma unroll
-        for (int f = 0; f < MF; ++f) acc[f] = mx_mfma<1>(r.w[1], r.a[f][1], acc[f], r.ws, r.as[f][1]);
-    }
-    if (n > 2) {
-#pragma unroll
-        for (int f = 0; f < MF; ++f) acc[f] = mx_mfma<2>(r.w[2], r.a[f][2], acc[f], r.ws, r.as[f][2]);
-    }
-    if (n > 3) {
-#pragma unroll
-        for (int f = 0; f < MF; ++f) acc[f] = mx_mfma<3>(r.w[3], r.a[f][3], acc[f], r.ws, r.as[f][3]);
-    }
-}
-
-// this wave's run of K for activation rows row[f] (per lane: row of lane % 16)
-template <int MF>
-__device__ __forceinline__ void gemv_run(const uint8_t* strip, qmm_xmx x, const int (&row)[MF], int K128, int S, int wave, mx_v4f (&acc)[MF]) {
-    const int lane = threadIdx.x & 63, blk = lane >> 4, G = mx_groups(K128);
-    const int g0 = wave * G / S, g1 = (wave + 1) * G / S;
-    const uint8_t* qr[MF];
-    const uint8_t* er[MF];
-#pragma unroll
-    for (int f = 0; f < MF; ++f) {
-        qr[f] = x.q + (size_t)row[f] * K128 * 64 + blk * 16;
-        er[f] = x.e + (size_t)row[f] * K128 * 4 + blk;
-        acc[f] = mx_v4f{0.f, 0.f, 0.f, 0.f};
-    }
-    GemvGroup<MF> r0, r1;
-    if (g0 < g1) gemv_load<MF>(r0, strip, qr, er, g0, K128, lane);
-    for (int g = g0; g < g1; g += 2) {
-        if (g + 1 < g1) gemv_load<MF>(r1, strip, qr, er, g + 1, K128, lane);
-        gemv_mul<MF>(r0, acc, g, K128);
-        if (g + 1 < g1) {
-            if (g + 2 < g1) gemv_load<MF>(r0, strip, qr, er, g + 2, K128, lane);
-            gemv_mul<MF>(r1, acc, g + 1, K128);
-        }
-    }
-}
-
-// the S runs' sums, added in order: thread i of the workgroup gets item i = 64 f + lane
-template <int MF>
-__device__ __forceinline__ void gemv_reduce(mx_v4f* red, const mx_v4f (&acc)[MF], int wave) {
-#pragma unroll
-    for (int f = 0; f < MF; ++f) red[(wave * MF + f) * 64 + (threadIdx.x & 63)] = acc[f];
+        for (int e = 0; e < 4; ++e)
+            red[((wave * MF + f) * 4 + e) * 64 + (threadIdx.x & 63)] = mx_v4f{acc[0][f][4 * e], acc[0][f][4 * e + 1], acc[0][f][4 * e + 2], acc[0][f][4 * e + 3]};
     __syncthreads();
 }
 template <int MF>
 __device__ __forceinline__ mx_v4f gemv_sum(const mx_v4f* red, int i, int S) {
     mx_v4f v = red[i];
-    for (int w = 1; w < S; ++w) v += red[w * MF * 64 + i];
+    for (int w = 1; w < S; ++w) v += red[w * MF * 256 + i];
     return v;
 }
 
-template <int MF, bool BF>
+template <int QN, bool BF>
 __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ y, int N, int K128,
                                                                    int ncol, int vec) {
+    constexpr int MF = gemv_mf<QN>();
     extern __shared__ __align__(16) uint8_t smem[];
     mx_v4f* red = (mx_v4f*)smem;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = blockDim.x >> 6;
-    const uint8_t* strip = W + (size_t)blockIdx.x * mx_strip_bytes(K128);
-    int row[MF];
-#pragma unroll
-    for (int f = 0; f < MF; ++f) row[f] = min(16 * f + (lane & 15), ncol - 1);
-    mx_v4f acc[MF];
-    gemv_run<MF>(strip, x, row, K128, S, wave, acc);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = blockDim.x >> 6;
+    const int n0 = (int)blockIdx.x * 32;
+    const uint32_t sb = mx_strip_bytes(K128);
+    mx_v16f acc[1][MF];
+    gemv_run<QN>(smem + wave * gemv_wave_lds<QN>(), W + (size_t)blockIdx.x * 2 * sb, n0 + 16 < N ? sb : 0u, x, ncol, [](int r) { return r; }, K128, S, wave,
+                 acc);
     gemv_reduce<MF>(red, acc, wave);
-    for (int i = threadIdx.x; i < 64 * MF; i += blockDim.x) {
-        const mx_v4f v = gemv_sum<MF>(red, i, S);
-        const int m = 16 * (i >> 6) + (i & 15), n = (int)blockIdx.x * 16 + 4 * ((i >> 4) & 3);
-        if (m < ncol && n < N) mx_store4<BF>(y, (size_t)m * N + n, v, N - n, vec);
+    for (int i = threadIdx.x; i < 256 * MF; i += blockDim.x) {
+        const int m = 32 * (i >> 8) + (i & 31), n = n0 + 8 * ((i >> 6) & 3) + 4 * ((i >> 5) & 1);
+        if (m < ncol && n < N) mx_store4<BF>(y, (size_t)m * N + n, gemv_sum<MF>(red, i, S), N - n, vec);
     }
 }
 
-// Experts by ids: workgroup (strip, slot).  The first slot of an expert computes all slots that hold it, 16 at
-// a time (a token lists an expert once, so 16 tokens make one pass), the others leave: an expert is read once.
+// Experts by ids: workgroup (two strips, slot).  The first slot of an expert computes all slots that hold it, 8 QN at
+// a time (a token lists an expert once, so T tokens make one pass), the others leave: an expert is read once.
 constexpr int kMoeGemvMaxT = 16, kMoeGemvMaxSlots = kMoeGemvMaxT * kMoeMaxSlots;
 
-template <bool BF>
+template <int QN, bool BF>
 __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uint8_t* __restrict__ W, const uint8_t* __restrict__ Wsh, size_t ebytes,
                                                                        const int* __restrict__ ids, qmm_xmx x, void* __restrict__ y, int nslots,
                                                                        int per_token, int xrow_te, int nexp, int N, int K128, int vec) {
@@ -166,17 +202,19 @@ __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uin
         n += __builtin_popcountll(hit);
     }
     __syncthreads();
-    const uint8_t* strip = (id < 0 ? Wsh : W + (size_t)id * ebytes) + (size_t)blockIdx.x * mx_strip_bytes(K128);
-    for (int c0 = 0; c0 < n; c0 += 16) {
-        const int slot = cols[min(c0 + (lane & 15), n - 1)];
-        const int row[1] = {xrow_te ? slot : slot / per_token};
-        mx_v4f acc[1];
-        gemv_run<1>(strip, x, row, K128, S, wave, acc);
+    const int n0 = (int)blockIdx.x * 32;
+    const uint32_t sb = mx_strip_bytes(K128);
+    const uint8_t* strip = (id < 0 ? Wsh : W + (size_t)id * ebytes) + (size_t)blockIdx.x * 2 * sb;
+    for (int c0 = 0; c0 < n; c0 += 8 * QN) {
+        mx_v16f acc[1][1];
+        gemv_run<QN>(smem + wave * gemv_wave_lds<QN>(), strip, n0 + 16 < N ? sb : 0u, x, min(n - c0, 8 * QN), [&](int r) {
+            const int slot = cols[c0 + r];
+            return xrow_te ? slot : slot / per_token;
+        }, K128, S, wave, acc);
         gemv_reduce<1>(red, acc, wave);
-        if (threadIdx.x < 64) {
-            const mx_v4f v = gemv_sum<1>(red, threadIdx.x, S);
-            const int m = c0 + (lane & 15), nn = (int)blockIdx.x * 16 + 4 * (lane >> 4);
-            if (m < n && nn < N) mx_store4<BF>(y, (size_t)slot * N + nn, v, N - nn, vec);
+        for (int i = threadIdx.x; i < 256; i += blockDim.x) {
+            const int c = c0 + (i & 31), nn = n0 + 8 * (i >> 6) + 4 * ((i >> 5) & 1);
+            if ((i & 31) < 8 * QN && c < n && nn < N) mx_store4<BF>(y, (size_t)cols[c] * N + nn, gemv_sum<1>(red, i, S), N - nn, vec);
         }
         __syncthreads();                                 // red is written again
     }
@@ -320,15 +358,31 @@ const MxTileCost& pick_tile(int M, int N, int K128) {
     return *best;
 }
 
-template <int MF>
+template <int QN>
 int launch_gemv(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K128, hipStream_t s) {
     const int S = gemv_waves(mx_groups(K128));
-    const dim3 grid((unsigned)((N + 15) / 16)), block(64 * S);
-    const size_t lds = (size_t)S * MF * 64 * sizeof(mx_v4f);
+    const dim3 grid((unsigned)((N + 31) / 32)), block(64 * S);
+    const size_t lds = (size_t)S * std::max<size_t>(gemv_mf<QN>() * 256 * sizeof(mx_v4f), gemv_wave_lds<QN>());
     if (dtype == QMM_BF16)
-        hipLaunchKernelGGL((k_gemv_mxfp4<MF, true>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
+        hipLaunchKernelGGL((k_gemv_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
     else
-        hipLaunchKernelGGL((k_gemv_mxfp4<MF, false>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
+        hipLaunchKernelGGL((k_gemv_mxfp4<QN, false>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
+    QMM_LAUNCH_CHECK();
+    return QMM_OK;
+}
+
+template <int QN>
+int launch_gemv_moe(const void* W, const void* Wsh, size_t ebytes, const int* ids, qmm_xmx x, void* y, int dtype, int T, int nslot, int nexperts, int N,
+                    int K128, int xrow_te, hipStream_t s) {
+    const int S = gemv_waves(mx_groups(K128));
+    const dim3 grid((unsigned)((N + 31) / 32), (unsigned)(T * nslot)), block(64 * S);
+    const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), gemv_wave_lds<QN>());
+    if (dtype == QMM_BF16)
+        hipLaunchKernelGGL((k_gemv_moe_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
+                           xrow_te, nexperts, N, K128, vec_out(y, dtype, N));
+    else
+        hipLaunchKernelGGL((k_gemv_moe_mxfp4<QN, false>), grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
+                           xrow_te, nexperts, N, K128, vec_out(y, dtype, N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
 }
@@ -347,9 +401,10 @@ int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N
     if (ncol == 0) return QMM_OK;
     const int K128 = mx_steps(K);
     hipStream_t s = (hipStream_t)stream;
-    if (ncol <= 16) return launch_gemv<1>(W, x, y, dtype, ncol, N, K128, s);
-    if (ncol <= 32) return launch_gemv<2>(W, x, y, dtype, ncol, N, K128, s);
-    return launch_gemv<4>(W, x, y, dtype, ncol, N, K128, s);
+    if (ncol <= 8) return launch_gemv<1>(W, x, y, dtype, ncol, N, K128, s);
+    if (ncol <= 16) return launch_gemv<2>(W, x, y, dtype, ncol, N, K128, s);
+    if (ncol <= 32) return launch_gemv<4>(W, x, y, dtype, ncol, N, K128, s);
+    return launch_gemv<8>(W, x, y, dtype, ncol, N, K128, s);
 }
 
 int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int* ids, qmm_xmx x, void* y, int dtype, int T, int nslot, int nexperts,
@@ -360,18 +415,8 @@ int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int*
     if (T < 0 || T > kMoeGemvMaxT || nslot < 1 || nslot > kMoeMaxSlots || nexperts < 1) return QMM_ERR_SHAPE;
     if (ebytes % 16 != 0 || (nexperts > 1 && ebytes < qmm_mxfp4_weight_bytes(N, K)) || misaligned(Wsh, 16) || misaligned(ids, 4)) return QMM_ERR_ARG;
     if (T == 0) return QMM_OK;
-    const int K128 = mx_steps(K), S = gemv_waves(mx_groups(K128));
-    const dim3 grid((unsigned)((N + 15) / 16), (unsigned)(T * nslot)), block(64 * S);
-    const size_t lds = (size_t)S * 64 * sizeof(mx_v4f);
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == QMM_BF16)
-        hipLaunchKernelGGL(k_gemv_moe_mxfp4<true>, grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
-                           xrow_te, nexperts, N, K128, vec_out(y, dtype, N));
-    else
-        hipLaunchKernelGGL(k_gemv_moe_mxfp4<false>, grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
-                           xrow_te, nexperts, N, K128, vec_out(y, dtype, N));
-    QMM_LAUNCH_CHECK();
-    return QMM_OK;
+    if (T <= 8) return launch_gemv_moe<1>(W, Wsh, ebytes, ids, x, y, dtype, T, nslot, nexperts, N, mx_steps(K), xrow_te, (hipStream_t)stream);
+    return launch_gemv_moe<2>(W, Wsh, ebytes, ids, x, y, dtype, T, nslot, nexperts, N, mx_steps(K), xrow_te, (hipStream_t)stream);
 }
 
 int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K, void* stream) {
