@@ -25,7 +25,9 @@ namespace {
 // the operand registers, by kilobytes, two steps (a pair) at a time, the next pair in flight while one is multiplied.
 // The activation rows beside them come as whole 128-byte lines (a pair of a row, eight lanes) and turn into operands in
 // LDS that is the wave's own: loaded in operand order, 16 bytes of 32 rows at a time, four loads touch each line, and the
-// vector cache holds every load up whose line is still on its way (64 rows x 17408 x 5120: 66 us that way).
+// vector cache holds every load up whose line is still on its way (24 rows x 5120 x 17408: 30 us that way, 15.2 so).
+// More than 32 rows are passes of 32, side by side: the weights of the second mostly come from caches (64 rows x 17408 x
+// 5120: 22 us; both fragments in one pass 80, 16 us up to 32 rows).
 constexpr int kGemvMaxWaves = 8, kGemvMaxRows = 64;
 
 // S for G groups: one wave a group up to 8, else the count of 4 .. 8 that leaves the least imbalance
@@ -37,18 +39,16 @@ int gemv_waves(int G) {
     return best;
 }
 
-// QN: eights of activation rows that are loaded (1, 2, 4 or 8), MF fragments of 32
-template <int QN> constexpr int gemv_mf() { return QN == 8 ? 2 : 1; }
-// LDS of one wave: a pair of 32 MF rows, and a group's scales of them (16 bytes a row)
-template <int QN> constexpr int gemv_wave_lds() { return 32 * gemv_mf<QN>() * (128 + 16); }
+// LDS of one wave: a pair of 32 rows, and a group's scales of them (16 bytes a row)
+constexpr int kGemvWaveLds = 32 * (128 + 16);
 
 // this wave's run of K: weight rows of `strip` and the next strip (sb bytes on, or 0 where there is none); row(r):
 // the activation row of tile row r, of which n are real.  No branch lies around a load (the compiler would wait for
 // every load in flight where the paths meet): the last group is a body of its own.
+// QN: eights of activation rows that are loaded (1, 2 or 4)
 template <int QN, class Row>
 __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uint32_t sb, qmm_xmx x, int n, Row row, int K128, int S, int wave,
-                                         mx_v16f (&acc)[1][gemv_mf<QN>()]) {
-    constexpr int MF = gemv_mf<QN>();
+                                         mx_v16f (&acc)[1][1]) {
     const int lane = threadIdx.x & 63, half = lane >> 5, G = mx_groups(K128), last = K128 - 1;
     const int g0 = wave * G / S, g1 = (wave + 1) * G / S;
     const uint8_t* wp = strip + ((lane & 16) ? sb : 0u);
@@ -57,8 +57,8 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
     const int cj = lane & 7;
 #pragma unroll
     for (int i = 0; i < QN; ++i) qp[i] = x.q + (size_t)row(min(8 * i + (lane >> 3), n - 1)) * K128 * 64 + (cj & 3) * 16;
-    const int er = MF == 2 ? lane : lane & 31;           // the row whose scales this lane brings
-    const uint8_t* ep = x.e + (size_t)row(min(er, n - 1)) * K128 * 4;
+    const int fr = lane & 31, sw = a_swz(fr);            // the tile row of this lane's operand, whose scales it brings
+    const uint8_t* ep = x.e + (size_t)row(min(fr, n - 1)) * K128 * 4;
     struct Pair { uint4 w[2][2], a[QN]; };
     struct Scales { uint32_t w[2], a[4]; };
     auto load = [&](Pair& r, int p) {                    // a step past the end re-reads the last one, unused
@@ -78,8 +78,8 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
 #pragma unroll
         for (int s = 0; s < 4; ++s) r.a[s] = *(const uint32_t*)(ep + 4u * (uint32_t)min(4 * g + s, last));
     };
-    const int fr = lane & 31, sw = a_swz(fr);
-    uint8_t* es = lds + 32 * MF * 128;
+    const uint8_t* d = lds + fr * 128;
+    uint8_t* es = lds + 32 * 128 + fr * 16;
     // the products of pair P of a group, `steps` (1 or 2) of them
     auto mul = [&](const Pair& r, const Scales& sc, auto pc, int steps) {
         constexpr int P = decltype(pc)::value;
@@ -91,28 +91,21 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             if (s == steps) break;
-#pragma unroll
-            for (int f = 0; f < MF; ++f) {
-                const uint8_t* d = lds + (fr + 32 * f) * 128;
-                const uint4 a0 = *(const uint4*)(d + (((4 * s + half) ^ sw) << 4)), a1 = *(const uint4*)(d + (((4 * s + 2 + half) ^ sw) << 4));
-                const uint32_t sa = *(const uint32_t*)(es + (fr + 32 * f) * 16 + 4 * (2 * P + s)) >> (8 * half);
-                if (s == 0) {
-                    acc[0][f] = mx_mfma32<2 * P, 0>(r.w[0][0], a0, acc[0][f], sc.w[0], sa);
-                    acc[0][f] = mx_mfma32<2 * P, 2>(r.w[0][1], a1, acc[0][f], sc.w[1], sa);
-                } else {
-                    acc[0][f] = mx_mfma32<2 * P + 1, 0>(r.w[1][0], a0, acc[0][f], sc.w[0], sa);
-                    acc[0][f] = mx_mfma32<2 * P + 1, 2>(r.w[1][1], a1, acc[0][f], sc.w[1], sa);
-                }
+            const uint4 a0 = *(const uint4*)(d + (((4 * s + half) ^ sw) << 4)), a1 = *(const uint4*)(d + (((4 * s + 2 + half) ^ sw) << 4));
+            const uint32_t sa = *(const uint32_t*)(es + 4 * (2 * P + s)) >> (8 * half);
+            if (s == 0) {
+                acc[0][0] = mx_mfma32<2 * P, 0>(r.w[0][0], a0, acc[0][0], sc.w[0], sa);
+                acc[0][0] = mx_mfma32<2 * P, 2>(r.w[0][1], a1, acc[0][0], sc.w[1], sa);
+            } else {
+                acc[0][0] = mx_mfma32<2 * P + 1, 0>(r.w[1][0], a0, acc[0][0], sc.w[0], sa);
+                acc[0][0] = mx_mfma32<2 * P + 1, 2>(r.w[1][1], a1, acc[0][0], sc.w[1], sa);
             }
         }
-#pragma unroll
-        for (int f = 0; f < MF; ++f) pin<false>(acc[0][f]);
+        pin<false>(acc[0][0]);
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
-    for (int f = 0; f < MF; ++f)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[0][f][e] = 0.f;
+    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
     if (g0 < g1) {
         Pair r0, r1;
         Scales sc;
@@ -120,7 +113,7 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
         load(r0, 2 * g0);
         load(r1, 2 * g0 + 1);
         for (int g = g0; g < g1 - 1; ++g) {
-            *(uint4*)(es + er * 16) = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
+            *(uint4*)es = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
             const Scales now = sc;
             load_s(sc, g + 1);
             mul(r0, now, std::integral_constant<int, 0>{}, 2);
@@ -129,47 +122,43 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
             load(r1, 2 * g + 3);
         }
         const int left = K128 - 4 * (g1 - 1);            // steps of the last group (beyond 4: whole)
-        *(uint4*)(es + er * 16) = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
+        *(uint4*)es = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
         mul(r0, sc, std::integral_constant<int, 0>{}, min(left, 2));
         if (left > 2) mul(r1, sc, std::integral_constant<int, 1>{}, min(left - 2, 2));
     }
     settle<false>(acc);
 }
 
-// The S runs' sums, added in order: item i = 4 (64 f + lane) + e of the tile, four outputs each (weight rows 8 e ..)
-template <int MF>
-__device__ __forceinline__ void gemv_reduce(mx_v4f* red, const mx_v16f (&acc)[1][MF], int wave) {
+// The S runs' sums, added in order: item i = 64 e + lane of the tile, four outputs each (weight rows 8 e ..)
+__device__ __forceinline__ void gemv_reduce(mx_v4f* red, const mx_v16f (&acc)[1][1], int wave) {
     __syncthreads();                                     // the same LDS held the waves' operands
+    const mx_v16f& a = acc[0][0];
 #pragma unroll
-    for (int f = 0; f < MF; ++f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            red[((wave * MF + f) * 4 + e) * 64 + (threadIdx.x & 63)] = mx_v4f{acc[0][f][4 * e], acc[0][f][4 * e + 1], acc[0][f][4 * e + 2], acc[0][f][4 * e + 3]};
+    for (int e = 0; e < 4; ++e) red[(wave * 4 + e) * 64 + (threadIdx.x & 63)] = mx_v4f{a[4 * e], a[4 * e + 1], a[4 * e + 2], a[4 * e + 3]};
     __syncthreads();
 }
-template <int MF>
 __device__ __forceinline__ mx_v4f gemv_sum(const mx_v4f* red, int i, int S) {
     mx_v4f v = red[i];
-    for (int w = 1; w < S; ++w) v += red[w * MF * 256 + i];
+    for (int w = 1; w < S; ++w) v += red[w * 256 + i];
     return v;
 }
 
+// Workgroup (two strips, pass): pass p takes the rows 8 QN p ..
 template <int QN, bool BF>
 __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_mxfp4(const uint8_t* __restrict__ W, qmm_xmx x, void* __restrict__ y, int N, int K128,
                                                                    int ncol, int vec) {
-    constexpr int MF = gemv_mf<QN>();
     extern __shared__ __align__(16) uint8_t smem[];
     mx_v4f* red = (mx_v4f*)smem;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = blockDim.x >> 6;
-    const int n0 = (int)blockIdx.x * 32;
+    const int n0 = (int)blockIdx.x * 32, m0 = (int)blockIdx.y * 8 * QN, m1 = min(m0 + 8 * QN, ncol);
     const uint32_t sb = mx_strip_bytes(K128);
-    mx_v16f acc[1][MF];
-    gemv_run<QN>(smem + wave * gemv_wave_lds<QN>(), W + (size_t)blockIdx.x * 2 * sb, n0 + 16 < N ? sb : 0u, x, ncol, [](int r) { return r; }, K128, S, wave,
-                 acc);
-    gemv_reduce<MF>(red, acc, wave);
-    for (int i = threadIdx.x; i < 256 * MF; i += blockDim.x) {
-        const int m = 32 * (i >> 8) + (i & 31), n = n0 + 8 * ((i >> 6) & 3) + 4 * ((i >> 5) & 1);
-        if (m < ncol && n < N) mx_store4<BF>(y, (size_t)m * N + n, gemv_sum<MF>(red, i, S), N - n, vec);
+    mx_v16f acc[1][1];
+    gemv_run<QN>(smem + wave * kGemvWaveLds, W + (size_t)blockIdx.x * 2 * sb, n0 + 16 < N ? sb : 0u, x, m1 - m0, [&](int r) { return m0 + r; }, K128, S,
+                 wave, acc);
+    gemv_reduce(red, acc, wave);
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) {
+        const int m = m0 + (i & 31), n = n0 + 8 * (i >> 6) + 4 * ((i >> 5) & 1);
+        if (m < m1 && n < N) mx_store4<BF>(y, (size_t)m * N + n, gemv_sum(red, i, S), N - n, vec);
     }
 }
 
@@ -207,14 +196,14 @@ __global__ void __launch_bounds__(64 * kGemvMaxWaves) k_gemv_moe_mxfp4(const uin
     const uint8_t* strip = (id < 0 ? Wsh : W + (size_t)id * ebytes) + (size_t)blockIdx.x * 2 * sb;
     for (int c0 = 0; c0 < n; c0 += 8 * QN) {
         mx_v16f acc[1][1];
-        gemv_run<QN>(smem + wave * gemv_wave_lds<QN>(), strip, n0 + 16 < N ? sb : 0u, x, min(n - c0, 8 * QN), [&](int r) {
+        gemv_run<QN>(smem + wave * kGemvWaveLds, strip, n0 + 16 < N ? sb : 0u, x, min(n - c0, 8 * QN), [&](int r) {
             const int slot = cols[c0 + r];
             return xrow_te ? slot : slot / per_token;
         }, K128, S, wave, acc);
-        gemv_reduce<1>(red, acc, wave);
+        gemv_reduce(red, acc, wave);
         for (int i = threadIdx.x; i < 256; i += blockDim.x) {
             const int c = c0 + (i & 31), nn = n0 + 8 * (i >> 6) + 4 * ((i >> 5) & 1);
-            if ((i & 31) < 8 * QN && c < n && nn < N) mx_store4<BF>(y, (size_t)cols[c] * N + nn, gemv_sum<1>(red, i, S), N - nn, vec);
+            if ((i & 31) < 8 * QN && c < n && nn < N) mx_store4<BF>(y, (size_t)cols[c] * N + nn, gemv_sum(red, i, S), N - nn, vec);
         }
         __syncthreads();                                 // red is written again
     }
@@ -361,8 +350,8 @@ const MxTileCost& pick_tile(int M, int N, int K128) {
 template <int QN>
 int launch_gemv(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K128, hipStream_t s) {
     const int S = gemv_waves(mx_groups(K128));
-    const dim3 grid((unsigned)((N + 31) / 32)), block(64 * S);
-    const size_t lds = (size_t)S * std::max<size_t>(gemv_mf<QN>() * 256 * sizeof(mx_v4f), gemv_wave_lds<QN>());
+    const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((ncol + 8 * QN - 1) / (8 * QN))), block(64 * S);
+    const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), kGemvWaveLds);
     if (dtype == QMM_BF16)
         hipLaunchKernelGGL((k_gemv_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
     else
@@ -376,7 +365,7 @@ int launch_gemv_moe(const void* W, const void* Wsh, size_t ebytes, const int* id
                     int K128, int xrow_te, hipStream_t s) {
     const int S = gemv_waves(mx_groups(K128));
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)(T * nslot)), block(64 * S);
-    const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), gemv_wave_lds<QN>());
+    const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), kGemvWaveLds);
     if (dtype == QMM_BF16)
         hipLaunchKernelGGL((k_gemv_moe_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
                            xrow_te, nexperts, N, K128, vec_out(y, dtype, N));
@@ -403,8 +392,7 @@ int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N
     hipStream_t s = (hipStream_t)stream;
     if (ncol <= 8) return launch_gemv<1>(W, x, y, dtype, ncol, N, K128, s);
     if (ncol <= 16) return launch_gemv<2>(W, x, y, dtype, ncol, N, K128, s);
-    if (ncol <= 32) return launch_gemv<4>(W, x, y, dtype, ncol, N, K128, s);
-    return launch_gemv<8>(W, x, y, dtype, ncol, N, K128, s);
+    return launch_gemv<4>(W, x, y, dtype, ncol, N, K128, s);
 }
 
 int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int* ids, qmm_xmx x, void* y, int dtype, int T, int nslot, int nexperts,
