@@ -242,9 +242,12 @@ __global__ void __launch_bounds__(512, 2) k_gemm_mxfp4_dma(const uint8_t* __rest
     mx_store<MF, NF, BF>(smem, acc, Dst, n0 + 32 * NF * (wave & 3), N, vec, [&](int r) { return mw + r < M ? (int64_t)(mw + r) : -1; });
 }
 
-// Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 64 at a time, with as
-// many 32-row fragments as they need.
-constexpr int kMoeNF = 1, kMoeD = 8, kMoeCols = 128 * kMoeNF, kMoeRows = 64;
+// Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 128 at a time, with as
+// many 32-row fragments as they need.  512 experts of 1024 x 2048, 10 a token and a shared one: 1024 tokens 116 us, 2048
+// 128, 4096 154, 8192 252; 64 rows at a time 118, 131, 214, 335 (weights are read again).  The 571 MB of weights take
+// 110 at a large copy's rate, and bound it up to 2048 tokens; beyond, the steps of the tiles do.  Weights three steps
+// ahead: seven take 133 at 2048, and a third workgroup on a CU (of 168 registers a wave) 147.
+constexpr int kMoeNF = 1, kMoeD = 4, kMoeCols = 128 * kMoeNF, kMoeRows = 128;
 
 template <int MF, bool BF>
 __device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_xmx x, const int* rowtab, int k0, int n, int n0, void* D, int N, int K128,
@@ -271,7 +274,9 @@ __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __rest
     for (int r = 0; r < t.ncols; r += kMoeRows) {
         const int n = min(t.ncols - r, kMoeRows);
         if (n <= 32) moe_rows<1, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+        else if (n <= 64) moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+        else if (n <= 96) moe_rows<3, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+        else moe_rows<4, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
         __syncthreads();                                 // LDS is filled again
     }
 }

@@ -369,7 +369,8 @@ def sorted_rows(ids, E, cap_rows=128):
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("T,slots,E,N,K,cap_rows", [(1, 2, 4, 16, 128, 128), (40, 5, 7, 130, 300, 128), (150, 3, 2, 257, 640, 128), (64, 4, 100, 64, 1100, 128),
-                                                    (90, 4, 3, 48, 520, 17), (500, 2, 3, 140, 256, 128)])
+                                                    (90, 4, 3, 48, 520, 17), (500, 2, 3, 140, 256, 128), (75, 2, 1, 200, 1300, 128),
+                                                    (97, 2, 1, 64, 384, 128)])
 def test_moe_gemm(gpu, T, slots, E, N, K, cap_rows, out):
     rng = np.random.default_rng(T + E + K)
     W, Wsh, vals = experts(rng, E, N, K)
