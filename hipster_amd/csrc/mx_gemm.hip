@@ -243,10 +243,10 @@ __global__ void __launch_bounds__(512, 2) k_gemm_mxfp4_dma(const uint8_t* __rest
 }
 
 // Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 128 at a time, with as
-// many 32-row fragments as they need.  512 experts of 1024 x 2048, 10 a token and a shared one: 1024 tokens 116 us, 2048
-// 128, 4096 154, 8192 252; 64 rows at a time 118, 131, 214, 335 (weights are read again).  The 571 MB of weights take
-// 110 at a large copy's rate, and bound it up to 2048 tokens; beyond, the steps of the tiles do.  Weights three steps
-// ahead: seven take 133 at 2048, and a third workgroup on a CU (of 168 registers a wave) 147.
+// many 32-row fragments as they need.  512 experts of 1024 x 2048, 10 a token and a shared one: 512 tokens 109 us, 2048
+// 125, 8192 248; 64 rows at a time 335 at 8192 (weights are read again).  The 571 MB of weights take 110 at a large
+// copy's rate, and bound it up to 2048 tokens; beyond, the steps of the tiles do.  Weights three steps ahead: seven take
+// 5 % more at 2048, a third workgroup on a CU (of 168 registers a wave) 12 %.
 constexpr int kMoeNF = 1, kMoeD = 4, kMoeCols = 128 * kMoeNF, kMoeRows = 128;
 
 template <int MF, bool BF>
@@ -329,15 +329,15 @@ int launch_dma(const GemmCall& c) {
 }
 
 // The tiles, and what a GEMM takes on each, in microseconds: a + steps (b + c (rounds - 1) + d load), rounds =
-// ceil(tiles / 256 CUs), load = tiles / 256.  Fitted to 108 shapes (M 65 .. 4096, N 512 .. 17408, K 2048, 5120, 17408; mean
-// error 2 to 10 %); the tile that it names takes 0.4 % more than the best of the seven on (geometric) average, 10 % at
-// most.  Fewer tiles cost more: without the two DMA tiles 1.6 % (22 % at 4096 x 17408 x 2048), without 96 x 128 and 64 x 256 1 %
-// (23 % at 512 x 5120 x 5120).
+// ceil(tiles / 256 CUs), load = tiles / 256.  Fitted to calls one by one (4 to 18 % off the times in a replayed
+// graph).  Over 108 shapes (M 65 .. 4096, N 512 .. 17408, K 2048, 5120, 17408) the tile that they name takes 0.4 % more
+// than the best of the seven on (geometric) average, 11 % at most; without one of the seven 0.9 to 5.7 % (14 to 37 % at
+// most).
 struct MxTileCost { int rows, cols; float a, b, c, d; int (*launch)(const GemmCall&); };
 const MxTileCost kMxTiles[] = {
     {192, 384, 7.42f, 0.736f, 1.116f, 0.254f, launch_dma<3, 3, 3>}, {192, 256, 6.49f, 0.572f, 0.850f, 0.192f, launch_dma<3, 2, 4>},
-    {128, 256, 5.48f, 0.415f, 0.558f, 0.185f, launch_reg<4, 2, 4, 1>}, {96, 128, 4.11f, 0.225f, 0.245f, 0.065f, launch_reg<3, 1, 8, 2>},
-    {64, 256, 3.64f, 0.289f, 0.265f, 0.126f, launch_reg<2, 2, 4, 2>}, {64, 128, 4.00f, 0.180f, 0.208f, 0.051f, launch_reg<2, 1, 8, 2>},
+    {128, 256, 5.48f, 0.415f, 0.558f, 0.185f, launch_reg<4, 2, 4, 1>}, {96, 128, 4.11f, 0.225f, 0.245f, 0.065f, launch_reg<3, 1, 4, 2>},
+    {64, 256, 3.64f, 0.289f, 0.265f, 0.126f, launch_reg<2, 2, 4, 2>}, {64, 128, 4.00f, 0.180f, 0.208f, 0.051f, launch_reg<2, 1, 4, 2>},
     {32, 128, 4.22f, 0.129f, 0.134f, 0.028f, launch_reg<1, 1, 8, 2>},
 };
 

@@ -9,14 +9,16 @@
 //                 fraction of one.  Weights go straight from memory to the operand registers, D - 1 steps ahead (a
 //                 strip belongs to one wave; through LDS it would take two thirds of its bandwidth).  Activations,
 //                 which the waves share, come two steps at a time (a pair: 128 bytes of a row, whole cache lines),
-//                 four steps ahead in registers, then through LDS: three buffers, so that one barrier a pair
+//                 D steps ahead in registers, then through LDS: three buffers, so that one barrier a pair
 //                 suffices.  LDS reads run two 32-row fragments ahead of their products, across steps.
-//                 65 rows x 5120 x 5120: 10.9 us (14.7 for the other core's best tile).
+//                 65 rows x 5120 x 5120: 10.8 us (29 for the other core's best tile); 300 x 17408 x 5120: 26, of which
+//                 launch, first loads, products and outputs take 18 and the weights the rest: a CU gets some 32 KB/us
+//                 of them from HBM however far ahead it asks (with loads that hit a cache: 22).
 //   mx_tile_dma   64 MF x 128 NF outputs, eight waves, for many rows.  Both operands by DMA (global_load_lds):
 //                 activations by pairs into two buffers, weights step by step into a ring of NS, scales by groups of
 //                 four steps.  The waves run as two halves (the rows' halves, one wave of each on every SIMD) half a step
 //                 apart: while one half reads its operands from LDS and starts its DMAs, the other multiplies, and a
-//                 barrier ends each phase.  2048 x 17408 x 5120, a new weight each call: 101 us (3.6 PFLOP/s) against 115
+//                 barrier ends each phase.  2048 x 17408 x 5120, a new weight each call: 104 us (3.5 PFLOP/s) against 129
 //                 for the best tile of mx_tile_reg; without its DMAs it takes 71, without products and LDS reads 72.
 //
 // LDS holds an activation row's 16-byte chunk c at chunk c ^ a_swz(row): reads of 16 rows' chunk are free of bank
@@ -92,10 +94,8 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
     }
     uint4 w[D][NF][2];
     uint32_t ws[NF][2], wsn[NF][2];
-    auto load_w = [&](uint4 (&d)[NF][2], int k) {
-        const uint8_t* p = wbase + (uint32_t)min(k, last) * 1024u;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) { d[f][0] = ld16(p + woff[f]); d[f][1] = ld16(p + woff[f] + 512u); }
+    auto load_w = [&](uint4 (&d)[NF][2], int k, int i) {                   // piece i of 2 NF
+        d[i >> 1][i & 1] = ld16(wbase + (uint32_t)min(k, last) * 1024u + woff[i >> 1] + (i & 1) * 512u);
     };
     auto load_ws = [&](uint32_t (&d)[NF][2], int g) {
         const uint8_t* p = wbase + (uint32_t)min(g, G - 1) * 256u;
@@ -103,40 +103,38 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
         for (int f = 0; f < NF; ++f) { d[f][0] = *(const uint32_t*)(p + soff[f]); d[f][1] = *(const uint32_t*)(p + soff[f] + 128u); }
     };
 
-    // activations: chunk tid % 8 of the rows tid / 8 + 32 i, and the scales of row tid
+    // activations: chunk tid % 8 of the rows tid / 8 + 32 i, and the scales of row tid / 2 in step tid % 2 of a pair
     const int cj = tid & 7;
     const uint8_t* qp[MF];
 #pragma unroll
     for (int i = 0; i < MF; ++i) qp[i] = x.q + (size_t)rows((tid >> 3) + 32 * i) * K128 * 64 + (cj & 3) * 16;
-    const uint8_t* ep = x.e + (size_t)rows(min(tid, T::kRows - 1)) * K128 * 4;
-    uint4 pa[2][MF];
-    uint32_t pe[2][2];
-    auto load_a = [&](uint4 (&d)[MF], uint32_t (&e)[2], int p) {
-        const uint32_t off = (uint32_t)min(2 * p + (cj >> 2), last) * 64u;
-#pragma unroll
-        for (int i = 0; i < MF; ++i) d[i] = ld16(qp[i] + off);
-        e[0] = *(const uint32_t*)(ep + (uint32_t)min(2 * p, last) * 4u);
-        e[1] = *(const uint32_t*)(ep + (uint32_t)min(2 * p + 1, last) * 4u);
+    const int es = min(tid, 2 * T::kRows - 1);           // beyond: the last one again
+    const uint8_t* ep = x.e + (size_t)rows(es >> 1) * K128 * 4;
+    constexpr int NP = D / 2;                            // pairs in flight
+    uint4 pa[NP][MF];
+    uint32_t pe[NP];
+    auto load_a = [&](uint4 (&d)[MF], int p, int i) { d[i] = ld16(qp[i] + (uint32_t)min(2 * p + (cj >> 2), last) * 64u); };
+    auto load_as = [&](uint32_t& e, int p) { e = *(const uint32_t*)(ep + (uint32_t)min(2 * p + (es & 1), last) * 4u); };
+    auto put_a = [&](const uint4 (&v)[MF], int buf, int i) {
+        const int row = (tid >> 3) + 32 * i;
+        *(uint4*)(smem + buf * T::kStage + row * 128 + ((cj ^ a_swz(row)) << 4)) = v[i];
     };
-    auto put_a = [&](const uint4 (&v)[MF], const uint32_t (&e)[2], int buf) {
-        uint8_t* d = smem + buf * T::kStage;
+    auto put_as = [&](uint32_t e, int buf) { *(uint32_t*)(smem + buf * T::kStage + T::kCodes + es * 4) = e; };
+    auto load_pair = [&](uint4 (&d)[MF], uint32_t& e, int p) {
 #pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            const int row = (tid >> 3) + 32 * i;
-            *(uint4*)(d + row * 128 + ((cj ^ a_swz(row)) << 4)) = v[i];
-        }
-        if (tid < T::kRows) *(uint2*)(d + T::kCodes + tid * 8) = make_uint2(e[0], e[1]);
+        for (int i = 0; i < MF; ++i) load_a(d, p, i);
+        load_as(e, p);
     };
     // this lane's part of fragment j in step parity s of a buffer: two blocks' codes, the four scale bytes
     struct Frag { uint4 c0, c1; uint32_t s; };
     const int fr = lane & 31, sw = a_swz(fr);            // rows 32 apart: the same rotation
+    const uint32_t at0 = (uint32_t)(fr * 128 + ((half ^ sw) << 4)), at1 = (uint32_t)(fr * 128 + (((half + 2) ^ sw) << 4));
     auto read_a = [&](int buf, int s, int j) {
         const uint8_t* d = smem + buf * T::kStage;
-        const int c = 4 * s + half;
         Frag r;
-        r.c0 = *(const uint4*)(d + (fr + 32 * j) * 128 + ((c ^ sw) << 4));
-        r.c1 = *(const uint4*)(d + (fr + 32 * j) * 128 + (((c + 2) ^ sw) << 4));
-        r.s = *(const uint32_t*)(d + T::kCodes + (fr + 32 * j) * 8 + 4 * s);
+        r.c0 = *(const uint4*)(d + (at0 ^ (64u * s)) + 4096 * j);
+        r.c1 = *(const uint4*)(d + (at1 ^ (64u * s)) + 4096 * j);
+        r.s = *(const uint32_t*)(d + T::kCodes + fr * 8 + 256 * j + 4 * s);
         return r;
     };
 
@@ -147,13 +145,18 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[f][j][e] = 0.f;
 
-    load_a(pa[0], pe[0], 0);
     load_ws(ws, 0);
 #pragma unroll
-    for (int k = 0; k < D - 1; ++k) load_w(w[k], k);
-    load_a(pa[1], pe[1], 1);
-    put_a(pa[0], pe[0], 0);
-    load_a(pa[0], pe[0], 2);
+    for (int k = 0; k < D; ++k) {                        // in the order of their use: loads return in the order of issue
+        if (k % 2 == 0) load_pair(pa[k / 2], pe[k / 2], k / 2);
+        if (k == D - 1) break;
+#pragma unroll
+        for (int i = 0; i < 2 * NF; ++i) load_w(w[k], k, i);
+    }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) put_a(pa[0], 0, i);
+    put_as(pe[0], 0);
+    load_pair(pa[0], pe[0], NP);
     lds_barrier();
 
     int buf = 0;                                         // of the current pair
@@ -161,34 +164,49 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
     constexpr int kAhead = MF > 1 ? 2 : 1;               // fragments read ahead (fragments of one step follow the last step's)
     Frag fa[MF + kAhead];
     static_for<0, kAhead>([&](auto jc) { fa[jc.value] = read_a(0, jc.value / MF, jc.value % MF); });
-    // step k of ring slot U (k % D)
+    // Step k of ring slot U (k % D).  A wave issues some four instructions in the time of a product, so the rest of the
+    // step lies between the products: after the first of a fragment the reads of a later one, after its last the
+    // activations' part.  The weights' loads come after the step's first product, except in a wave that is
+    // alone on its SIMD, which spreads them over the fragments (128 x 256: 44 us against 47 at 2048 x 5120 x 5120; two
+    // waves a SIMD take 35.6 that way at 100 x 5120 x 17408, 32.4 so).
+    constexpr int kMeet = MF > 2 ? MF - 3 : -1;          // the fragment of an odd step after which the waves meet
     auto step = [&](auto uc, int k) {
-        constexpr int U = decltype(uc)::value, S = U & 3, P = (U >> 1) & 1;
-        load_w(w[(U + D - 1) % D], k + D - 1);
-        if constexpr (S == 0) load_ws(wsn, (k >> 2) + 1);
-        if constexpr ((U & 1) == 0) {
-            put_a(pa[P ^ 1], pe[P ^ 1], after(buf));     // pair k / 2 + 1
-            load_a(pa[P ^ 1], pe[P ^ 1], (k >> 1) + 3);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        constexpr int U = decltype(uc)::value, S = U & 3, P = ((U >> 1) + 1) % NP;
         static_for<0, MF>([&](auto jc) {
             constexpr int j = decltype(jc)::value, n = j + kAhead;
-            // the fragment kAhead on: of this step, or of the next one (in the next buffer after the second of a pair)
-            if constexpr (n < MF) fa[n] = read_a(buf, U & 1, n);
-            else if constexpr ((U & 1) == 1) fa[n] = read_a(after(buf), 0, n - MF);
-            else if constexpr (n - MF < MF) fa[n] = read_a(buf, 1, n - MF);
             const uint32_t sa = fa[j].s >> (8 * half);   // the lane's two in bytes 0 and 2
+            static_for<0, 2 * NF>([&](auto ic) {
+                constexpr int i = decltype(ic)::value, f = i % NF, h = i / NF;
+                acc[f][j] = mx_mfma32<S, 2 * h>(w[U][f][h], h ? fa[j].c1 : fa[j].c0, acc[f][j], ws[f][h], sa);
+                pin<AGPR>(acc[f][j]);
+                __builtin_amdgcn_sched_barrier(0);
+                // the fragment kAhead on: of this step, or of the next one (in the next buffer after the second of a pair)
+                if constexpr (i == 0) {
+                    if constexpr (n < MF) fa[n] = read_a(buf, U & 1, n);
+                    else if constexpr ((U & 1) == 1) fa[n] = read_a(after(buf), 0, n - MF);
+                    else if constexpr (n - MF < MF) fa[n] = read_a(buf, 1, n - MF);
+                }
+                if constexpr (AGPR ? i == NF : i == 0 && j == 0) {
+                    constexpr int lo = AGPR ? 2 * NF * j / MF : 0, hi = AGPR ? 2 * NF * (j + 1) / MF : 2 * NF;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<S, 0>(w[U][f][0], fa[j].c0, acc[f][j], ws[f][0], sa);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f][j] = mx_mfma32<S, 2>(w[U][f][1], fa[j].c1, acc[f][j], ws[f][1], sa);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) pin<AGPR>(acc[f][j]);
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int l = lo; l < hi; ++l) load_w(w[(U + D - 1) % D], k + D - 1, l);
+                    if constexpr (S == 1 && j == 0) load_ws(wsn, (k >> 2) + 1);
+                }
+                if constexpr (i == 2 * NF - 1 && (U & 1) == 0) {
+                    put_a(pa[P], after(buf), j);         // pair k / 2 + 1
+                    load_a(pa[P], (k >> 1) + 1 + NP, j);
+                    if constexpr (j == MF - 1) {
+                        put_as(pe[P], after(buf));
+                        load_as(pe[P], (k >> 1) + 1 + NP);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr ((U & 1) == 1 && j == kMeet) lds_barrier();             // opens the next pair
         });
         static_for<0, kAhead>([&](auto jc) { fa[jc.value] = fa[MF + jc.value]; });
-        if constexpr ((U & 1) == 0) lds_barrier();       // opens the pair that was written above
-        else buf = after(buf);
+        if constexpr ((U & 1) == 1) buf = after(buf);
+        else if constexpr (kMeet < 0) lds_barrier();
         if constexpr (S == 3) {
 #pragma unroll
             for (int f = 0; f < NF; ++f) { ws[f][0] = wsn[f][0]; ws[f][1] = wsn[f][1]; }
