@@ -26,6 +26,7 @@ typedef float mx_v4f __attribute__((ext_vector_type(4)));
 typedef float mx_v16f __attribute__((ext_vector_type(16)));
 
 constexpr int kMxMaxK = 1 << 24;                 // a strip's byte offsets stay in 32 bits
+constexpr int kMxMaxRows = 0x7fffff00;                // of a weight or a GEMM: a tile past the last row stays an int
 constexpr int kMxFp4 = 4;                        // the instruction's number for e2m1
 
 __host__ __device__ __forceinline__ int mx_steps(int K) { return (K + 127) >> 7; }

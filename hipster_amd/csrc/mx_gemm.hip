@@ -287,7 +287,7 @@ bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t
 int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int N, int K) {
     if (!W || !x.q || !x.e || !y) return QMM_ERR_NULL;
     if (dtype != QMM_F32 && dtype != QMM_BF16) return QMM_ERR_FORMAT;
-    if (N <= 0 || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
+    if (N <= 0 || N > kMxMaxRows || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
     if (misaligned(W, 16) || misaligned(x.q, 16) || misaligned(x.e, 4) || misaligned(y, dtype == QMM_BF16 ? 2 : 4)) return QMM_ERR_ARG;
     return QMM_OK;
 }
@@ -415,7 +415,7 @@ int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int*
 int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K, void* stream) {
     const int st = check_operands(W, x, D, dtype, N, K);
     if (st != QMM_OK) return st;
-    if (M < 0) return QMM_ERR_SHAPE;
+    if (M < 0 || M > kMxMaxRows) return QMM_ERR_SHAPE;
     if (M == 0) return QMM_OK;
     const int K128 = mx_steps(K);
     hipStream_t s = (hipStream_t)stream;
@@ -423,7 +423,7 @@ int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, i
 }
 
 int qmm_gemm_mxfp4_tile(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
+    if (M <= 0 || M > kMxMaxRows || N <= 0 || N > kMxMaxRows || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
     return (int)(&pick_tile(M, N, mx_steps(K)) - kMxTiles);
 }
 

@@ -146,7 +146,7 @@ using namespace qmm;
 extern "C" {
 
 size_t qmm_mxfp4_weight_bytes(int N, int K) {
-    if (N <= 0 || K <= 0 || K > kMxMaxK) return 0;
+    if (N <= 0 || N > kMxMaxRows || K <= 0 || K > kMxMaxK) return 0;
     return (size_t)((N + 15) / 16) * mx_strip_bytes(mx_steps(K));
 }
 
@@ -197,7 +197,7 @@ int qmm_dequant_mxfp4(qmm_xmx x, void* out, int dtype, int rows, int K, void* st
 
 int qmm_pack_mxfp4(qmm_xmx rows, void* W, int N, int K, void* stream) {
     if (!rows.q || !rows.e || !W) return QMM_ERR_NULL;
-    if (N <= 0 || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
+    if (N <= 0 || N > kMxMaxRows || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
     if (misaligned(rows.q, 16) || misaligned(W, 16)) return QMM_ERR_ARG;
     const int K128 = mx_steps(K);
     const uint32_t groups = (uint32_t)mx_groups(K128);

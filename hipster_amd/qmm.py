@@ -484,6 +484,13 @@ def _weight(W, N, K, name="W", extra=0):
     return _in(W, extra + (N + 15) // 16 * (steps * 1024 + (steps + 3) // 4 * 256), name, torch.uint8)
 
 
+def _experts(W, N, K, ebytes, n):
+    """The address of n packed weights of N rows of K values, `ebytes` apart."""
+    if ebytes < 0:
+        raise QmmError(f"W: weights {ebytes} bytes apart")
+    return _weight(W, N, K, "W", (n - 1) * ebytes)
+
+
 def pack_mxfp4(q, e, W, N, K, stream=None):
     """MXFP4 rows q [N][64 per step], e [N][4 per step] (an XMXBuf's tensors) -> W, the layout the products read."""
     for t, per, name in ((q, 64, "q"), (e, 4, "e")):
@@ -523,14 +530,14 @@ def gemm_mxfp4_tile(M, N, K):
 def gemv_moe_mxfp4(W, Wsh, ebytes, ids, x, y, T, nslot, nexperts, N, K, xrow_te=False, stream=None):
     """y[te][n] = W_{ids[te]}[n] . x[te if xrow_te else t] for T <= 16 tokens (ids int32 [T][nslot], below 0: Wsh)."""
     slots = T * nslot
-    check(_lib.lib().qmm_gemv_moe_mxfp4(_weight(W, N, K, "W", (nexperts - 1) * ebytes), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
+    check(_lib.lib().qmm_gemv_moe_mxfp4(_experts(W, N, K, ebytes, nexperts), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
                                         _in(ids, slots, "ids", torch.int32), _xmx(x, slots if xrow_te else T, K, "x"), _in(y, slots * N, "y"),
                                         _dtype(y, "y"), T, nslot, nexperts, N, K, int(xrow_te), _handle(stream)), "gemv_moe_mxfp4")
 
 
 def moe_gemm_mxfp4(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, N, K, stream=None):
     """D[k] = W_e . x[rowtab[k]] over rows sorted by expert (moe_sort's tiles, counts, rowtok; rowtab None: x[k])."""
-    check(_lib.lib().qmm_moe_gemm_mxfp4(_weight(W, N, K), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
+    check(_lib.lib().qmm_moe_gemm_mxfp4(_experts(W, N, K, ebytes, 1), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
                                         _in(tiles, 3 * max_tiles, "tiles", torch.int32), _in(counts, 2, "counts", torch.int32), max_tiles,
                                         None if rowtab is None else _in(rowtab, 0, "rowtab", torch.int32), _xmx(x, 0, K, "x"), _in(D, 0, "D"),
                                         _dtype(D, "D"), N, K, _handle(stream)), "moe_gemm_mxfp4")

@@ -142,3 +142,23 @@ def test_python_refusals_on_host_tensors():
         qmm.moe_route_groups(t, t.int(), t, 4, 64, 4)
     with pytest.raises(QmmError):
         qmm.postnorm_add_rmsnorm_bf16(t, t, None, t[0], t.bfloat16(), 4, 64, 1e-6)
+
+
+def test_sizes_near_the_int_limit():
+    """A tile past the last row would leave the ints that count rows: refused."""
+    L, big = _lib.lib(), (1 << 31) - 1
+    assert qmm.mxfp4_weight_bytes(big, 32) == 0 and qmm.mxfp4_weight_bytes(big - 255, 32) > 0
+    assert L.qmm_pack_mxfp4(X, D, big, 32, None) == SHAPE
+    assert L.qmm_gemv_mxfp4(D, X, D, 0, 1, big, 32, None) == SHAPE
+    assert L.qmm_gemm_mxfp4(D, X, D, 0, 1, big, 32, None) == SHAPE
+    assert L.qmm_gemm_mxfp4(D, X, D, 0, big, 32, 32, None) == SHAPE
+    assert L.qmm_gemm_mxfp4_tile(big, 32, 32) == SHAPE and L.qmm_gemm_mxfp4_tile(32, big, 32) == SHAPE
+    assert L.qmm_moe_gemm_mxfp4(D, None, 1 << 20, D, D, 1, None, X, D, 0, big, 32, None) == SHAPE
+    assert L.qmm_gemv_moe_mxfp4(D, None, 1 << 20, D, X, D, 0, 1, 1, 1, big, 32, 0, None) == SHAPE
+
+
+def test_experts_a_negative_distance_apart():
+    W = torch.zeros(4096, dtype=torch.uint8)
+    for call in (lambda: qmm.gemv_moe_mxfp4(W, None, -16, None, None, None, 1, 1, 2, 16, 32), lambda: qmm.moe_gemm_mxfp4(W, None, -16, None, None, 1, None, None, None, 16, 32)):
+        with pytest.raises(QmmError, match="apart"):
+            call()
