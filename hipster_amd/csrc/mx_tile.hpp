@@ -12,8 +12,9 @@
 //                 D steps ahead in registers, then through LDS: three buffers, so that one barrier a pair
 //                 suffices.  LDS reads run two 32-row fragments ahead of their products, across steps.
 //                 65 rows x 5120 x 5120: 10.8 us (29 for the other core's best tile); 300 x 17408 x 5120: 26, of which
-//                 launch, first loads, products and outputs take 18 and the weights the rest: a CU gets some 32 KB/us
-//                 of them from HBM however far ahead it asks (with loads that hit a cache: 22).
+//                 launch, first loads, products and outputs take 18; it is bound by what a CU fetches past its L1, at
+//                 most 50 KB/us from HBM (a plain read by 8 to 80 workgroups, however much is in flight), where a tile
+//                 of 128 x 256 needs 960 KB (with weights that hit the L1: 22 us).
 //   mx_tile_dma   64 MF x 128 NF outputs, eight waves, for many rows.  Both operands by DMA (global_load_lds):
 //                 activations by pairs into two buffers, weights step by step into a ring of NS, scales by groups of
 //                 four steps.  The waves run as two halves (the rows' halves, one wave of each on every SIMD) half a step
