@@ -10,6 +10,10 @@
 // read once and xo and xn written once; HBM bounds it (one row: the two reductions' latency).  A thread
 // holds C pieces of V values, 4 (16-byte accesses) or 1 (rows that 16-byte accesses do not fit); every load is
 // issued before the first sum.  Sums are f32 in a fixed order: per thread, by halves of the wave, wave by wave.
+//
+// 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 29 from caches; 4096 rows 69; one row
+// 6.7, one after another.  Threads go by n alone, since they set the sums' order: 640 of them with two pieces each
+// take 5.0 for one row and 9.5 instead of 11.1 for 300, but 41 for 2048 (448 with three 40, 320 with four 53).
 #include "mx.hpp"
 
 namespace qmm {
