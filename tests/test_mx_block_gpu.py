@@ -146,6 +146,21 @@ def test_expert_block_replayed(gpu, T):
         assert torch.equal(got, b.xb2)
 
 
+def test_two_blocks_at_once(gpu):
+    """Two streams, the runs in flight together: nothing is shared between calls."""
+    blocks = [(Block(T, 30 + T), torch.cuda.Stream()) for T in (60, 5)]
+    for i, (b, s) in enumerate(blocks):
+        b.feed(i)
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for b, s in blocks:
+            with torch.cuda.stream(s):
+                b.run()
+    torch.cuda.synchronize()
+    for b, _ in blocks:
+        b.check()
+
+
 @pytest.mark.parametrize("T", [1, 40, 64, 65, 300])
 def test_dense_block(gpu, T):
     """norm -> MXFP4 in one call, gate and up, silu, down, norm; the same codes from the two ways to them."""
