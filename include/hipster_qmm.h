@@ -427,7 +427,7 @@ int qmm_pack_mxfp4(qmm_xmx rows, void* W, int N, int K, void* stream);
 int qmm_repack_row_mxfp4(const uint8_t* src, uint8_t* q, uint8_t* e, int K);
 /* y[m][n] = W[n] . x[m] for m < ncol <= 64, y [ncol][N] f32 or bf16 (dtype), W packed: decode and draft
  * verification.  Products and block scales are exact, sums f32 in an order set by K alone: a row's bits do not
- * depend on ncol or N.  Any N, K. */
+ * depend on ncol or N.  Any K <= 2^24; N (and the GEMM's M) <= 2^31 - 256. */
 int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K, void* stream);
 /* the same for the experts of T <= 16 tokens: slot te = t * nslot + s uses expert ids[te] (W + id * ebytes, a packed
  * weight of N rows; below 0: Wsh, or expert 0 where Wsh is NULL; beyond the last: the last), x row te if xrow_te,
