@@ -332,15 +332,15 @@ int launch_dma(const GemmCall& c) {
 
 // The tiles, and what a GEMM takes on each, in microseconds: a + steps (b + c (rounds - 1) + d load), rounds =
 // ceil(tiles / 256 CUs), load = tiles / 256.  Fitted to calls one by one (4 to 18 % off the times in a replayed
-// graph).  Over 108 shapes (M 65 .. 4096, N 512 .. 17408, K 2048, 5120, 17408) the tile that they name takes 0.4 % more
-// than the best of the seven on (geometric) average, 11 % at most; without one of the seven 0.9 to 5.7 % (14 to 37 % at
-// most).
+// graph).  Over 108 shapes (M 65 .. 4096, N 512 .. 17408, K 2048, 5120, 17408) the tile that they name takes 0.3 % more
+// than the best of the eight on (geometric) average, 11 % at most; without one of the first seven 0.9 to 5.7 % (14 to
+// 37 % at most), without 192 x 128 0.6 % (1024 x 5120 x 5120 takes 26 us instead of 22).
 struct MxTileCost { int rows, cols; float a, b, c, d; int (*launch)(const GemmCall&); };
 const MxTileCost kMxTiles[] = {
     {192, 384, 7.42f, 0.736f, 1.116f, 0.254f, launch_dma<3, 3, 3>}, {192, 256, 6.49f, 0.572f, 0.850f, 0.192f, launch_dma<3, 2, 4>},
     {128, 256, 5.48f, 0.415f, 0.558f, 0.185f, launch_reg<4, 2, 4, 1>}, {96, 128, 4.11f, 0.225f, 0.245f, 0.065f, launch_reg<3, 1, 4, 2>},
     {64, 256, 3.64f, 0.289f, 0.265f, 0.126f, launch_reg<2, 2, 4, 2>}, {64, 128, 4.00f, 0.180f, 0.208f, 0.051f, launch_reg<2, 1, 4, 2>},
-    {32, 128, 4.22f, 0.129f, 0.134f, 0.028f, launch_reg<1, 1, 8, 2>},
+    {32, 128, 4.22f, 0.129f, 0.134f, 0.028f, launch_reg<1, 1, 8, 2>}, {192, 128, 5.10f, 0.339f, 0.433f, 0.201f, launch_reg<6, 1, 4, 1>},
 };
 
 const MxTileCost& pick_tile(int M, int N, int K128) {

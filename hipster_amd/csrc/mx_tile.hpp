@@ -104,24 +104,37 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
         for (int f = 0; f < NF; ++f) { d[f][0] = *(const uint32_t*)(p + soff[f]); d[f][1] = *(const uint32_t*)(p + soff[f] + 128u); }
     };
 
-    // activations: chunk tid % 8 of the rows tid / 8 + 32 i, and the scales of row tid / 2 in step tid % 2 of a pair
+    // activations: chunk tid % 8 of the rows tid / 8 + 32 i, and the scales of row tid / 2 in step tid % 2 of a pair,
+    // and of row 128 + tid / 2 where the tile has more than 128
     const int cj = tid & 7;
     const uint8_t* qp[MF];
 #pragma unroll
     for (int i = 0; i < MF; ++i) qp[i] = x.q + (size_t)rows((tid >> 3) + 32 * i) * K128 * 64 + (cj & 3) * 16;
-    const int es = min(tid, 2 * T::kRows - 1);           // beyond: the last one again
-    const uint8_t* ep = x.e + (size_t)rows(es >> 1) * K128 * 4;
+    constexpr int NE = (2 * T::kRows + 255) / 256;
+    int es[NE];
+    const uint8_t* ep[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        es[i] = min(tid + 256 * i, 2 * T::kRows - 1);    // beyond: the last one again
+        ep[i] = x.e + (size_t)rows(es[i] >> 1) * K128 * 4;
+    }
     constexpr int NP = D / 2;                            // pairs in flight
     uint4 pa[NP][MF];
-    uint32_t pe[NP];
+    uint32_t pe[NP][NE];
     auto load_a = [&](uint4 (&d)[MF], int p, int i) { d[i] = ld16(qp[i] + (uint32_t)min(2 * p + (cj >> 2), last) * 64u); };
-    auto load_as = [&](uint32_t& e, int p) { e = *(const uint32_t*)(ep + (uint32_t)min(2 * p + (es & 1), last) * 4u); };
+    auto load_as = [&](uint32_t (&e)[NE], int p) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) e[i] = *(const uint32_t*)(ep[i] + (uint32_t)min(2 * p + (es[i] & 1), last) * 4u);
+    };
     auto put_a = [&](const uint4 (&v)[MF], int buf, int i) {
         const int row = (tid >> 3) + 32 * i;
         *(uint4*)(smem + buf * T::kStage + row * 128 + ((cj ^ a_swz(row)) << 4)) = v[i];
     };
-    auto put_as = [&](uint32_t e, int buf) { *(uint32_t*)(smem + buf * T::kStage + T::kCodes + es * 4) = e; };
-    auto load_pair = [&](uint4 (&d)[MF], uint32_t& e, int p) {
+    auto put_as = [&](const uint32_t (&e)[NE], int buf) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) *(uint32_t*)(smem + buf * T::kStage + T::kCodes + es[i] * 4) = e[i];
+    };
+    auto load_pair = [&](uint4 (&d)[MF], uint32_t (&e)[NE], int p) {
 #pragma unroll
         for (int i = 0; i < MF; ++i) load_a(d, p, i);
         load_as(e, p);

@@ -225,7 +225,7 @@ TILES = [(0, 6000, 20000, 130), (0, 4000, 12300, 260), (0, 2000, 16400, 400), (0
          (1, 385, 20000, 1160), (1, 769, 10000, 2050), (2, 6000, 12300, 400), (2, 6000, 12300, 513), (2, 6000, 6200, 900), (2, 577, 10000, 1160),
          (2, 700, 8200, 2050), (3, 769, 10000, 260), (3, 769, 5000, 400), (3, 200, 16400, 640), (3, 200, 8200, 1025), (4, 200, 1000, 32),
          (4, 200, 8200, 513), (4, 200, 12300, 1160), (5, 385, 4100, 300), (5, 200, 5000, 900), (5, 200, 5000, 2050), (6, 200, 1000, 513),
-         (6, 200, 1000, 1025), (6, 200, 1000, 2180)]
+         (6, 200, 1000, 1025), (6, 200, 1000, 2180), (7, 769, 5000, 2050), (7, 961, 4900, 2180), (7, 1000, 4100, 2400), (7, 1153, 4100, 2433)]
 
 
 @pytest.mark.parametrize("tile,M,N,K", TILES)
