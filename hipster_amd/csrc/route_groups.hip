@@ -90,7 +90,7 @@ __device__ __forceinline__ double fma_c(double a, double b, double c) {
     return d;
 }
 __device__ __forceinline__ double exp64(double x) {
-    x = fmin(fmax(x, -800.0), 800.0);                    // 0 and inf from there on; NaN is masked before
+    x = fmin(fmax(x, -800.0), 800.0);                    // 0 and inf from there on; a NaN becomes -800: the callers keep theirs out
     const double n = __builtin_rint(x * 1.4426950408889634);
     const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, x));
     double p = 1.0 / 6227020800.0;
@@ -294,7 +294,8 @@ __global__ void __launch_bounds__(256) k_route_groups(const float* __restrict__ 
     }
     if (lane == 0 && r.shared) {
         idt[topk] = -1;
-        wt[topk] = r.shared == 1 ? (float)(1.0 / (1.0 + exp64(-(double)gate))) : 1.f;
+        const float sig = (float)(1.0 / (1.0 + exp64(-(double)gate)));
+        wt[topk] = r.shared != 1 ? 1.f : gate == gate ? sig : gate;        // a NaN stays one
     }
 }
 
