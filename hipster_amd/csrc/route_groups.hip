@@ -6,7 +6,7 @@
 //   the topk largest c of their experts, ties to the lower index;  w = s (renormalised over them) * scale
 //
 // Scores, sums and comparisons are in 64 bits: which of two experts is taken is a decision, and in 32 bits a
-// rounding of exp could make it otherwise than the definition does.  A logit of -inf or NaN masks its expert.
+// rounding of exp could make it otherwise than the definition does.  A logit or bias of -inf or NaN masks its expert.
 //
 // One wave routes a token; lane i holds the experts VPL i .. VPL i + VPL - 1.  The top-k without a step per expert:
 // the k-th largest of the largest keys of the 32 pairs of lanes (their upper 32 bits; found by a ballot for each) is
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256) k_route_groups(const float* __restrict__ 
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         c[j] = r.bias ? p[j] + (double)b[j] : p[j];
-        in[j] &= c[j] == c[j];                   // a NaN bias masks too
+        in[j] &= c[j] > -INFINITY;               // a bias of -inf or NaN masks too
     }
     const int per = E / r.groups;
     if (r.keep < r.groups) {

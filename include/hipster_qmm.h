@@ -447,7 +447,8 @@ int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_
                        qmm_xmx x, void* D, int dtype, int N, int K, void* stream);
 /* Experts of each token from logits [T][stride] by rule (above): ids / w [T][topk + (shared != 0)] in falling order of
  * the choice value, ties to the lower id.  Scores and comparisons are in 64 bits, a weight is rounded once.  An
- * expert whose logit is -inf or NaN is never chosen; a slot without an expert gets id -1, weight 0.
+ * expert whose logit or bias is -inf or NaN is never chosen and counts in no group; a slot without an expert gets id
+ * -1, weight 0.  The shared expert's weight is the sigmoid of its logit whatever that is (NaN: NaN).
  * nexp <= 1024, topk <= 16, groups <= 64 dividing nexp, topk <= keep * (nexp / groups), stride >= nexp (+ 1 for
  * shared 1). */
 int qmm_moe_route_groups(const float* logits, int stride, const qmm_route_rule* rule, int* ids, float* w, int T, int nexp, int topk, void* stream);

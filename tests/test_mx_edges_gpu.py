@@ -41,3 +41,23 @@ def test_route_shared_gate_that_is_not_finite(gpu, score, T):
             l[0] = np.nan
             ids, w = route(l, 64, 6, score=score, shared="gate")
         assert (ids[0] == -1).all() and (w[0, :6] == 0).all() and np.isnan(w[0, 6])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_bias_that_masks(gpu, score):
+    """A bias of -inf masks an expert as a logit of -inf does, also where too few experts are left."""
+    rng = np.random.default_rng(1)
+    l = rng.standard_normal((7, 64)).astype(np.float32)
+    l[0, :60] = np.nan
+    l[1, 4:] = -np.inf
+    b = (rng.standard_normal(64) * 0.1).astype(np.float32)
+    b[[0, 2, 61, 63]] = -np.inf, np.nan, -np.inf, np.inf
+    ids, w = route(l, 64, 6, score=score, bias=b)
+    assert not np.isin(ids, (0, 2, 61)).any() and (ids[0, 3:] == -1).all() and (ids[1, 2:] == -1).all() and (w[ids < 0] == 0).all()
+    route(l, 64, 6, score=score, bias=b, groups=8, keep=2, best=2, shared="one")
+    b[:] = -np.inf                                                       # every expert
+    ids, w = route(l, 64, 6, score=score, bias=b, groups=8, keep=2, best=2)
+    assert (ids == -1).all() and (w == 0).all()
+    b[32:] = 0.0                                                         # groups without an expert lose
+    ids, _ = route(l[2:], 64, 6, score=score, bias=b, groups=8, keep=4, best=2)
+    assert (ids >= 32).all()
