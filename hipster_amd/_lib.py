@@ -146,6 +146,7 @@ SIGNATURES = {
     "qmm_gemv_moe_mxfp4": (c_int, [c_vp, c_vp, ctypes.c_size_t, c_vp, XMX, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_mxfp4": (c_int, [c_vp, XMX, c_vp, c_int, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_mxfp4_tile": (c_int, [c_int, c_int, c_int]),
+    "qmm_moe_gemm_mxfp4_n": (c_int, [c_vp, c_vp, ctypes.c_size_t, c_int, c_vp, c_vp, c_int, c_vp, c_int, XMX, c_int, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_moe_gemm_mxfp4": (c_int, [c_vp, c_vp, ctypes.c_size_t, c_vp, c_vp, c_int, c_vp, XMX, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_moe_route_groups": (c_int, [c_vp, c_int, ctypes.POINTER(RouteRule), c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_postnorm_add_rmsnorm_bf16": (c_int, _POSTNORM + [c_vp, c_int, c_int, ctypes.c_float, c_vp]),

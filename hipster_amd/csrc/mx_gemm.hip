@@ -3,7 +3,7 @@
 //   qmm_gemv_mxfp4       y[m][n] = W[n] . x[m], m < 64: decode and draft verification
 //   qmm_gemv_moe_mxfp4   the same for the routed experts of up to 16 tokens, by ids
 //   qmm_gemm_mxfp4       any number of rows: prompts
-//   qmm_moe_gemm_mxfp4   rows sorted by expert (qmm_moe_sort)
+//   qmm_moe_gemm_mxfp4   rows sorted by expert (qmm_moe_sort); _n with the sizes of its buffers
 //
 // v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 32 weight rows by 32 activation rows over 64 values with their block
 // scales and adds to f32 (16 x 16 over 128 reads twice the operand bytes per product: 5.4 against 6.4 PFLOP/s from
@@ -16,6 +16,7 @@
 #include "mx_tile.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 namespace qmm {
@@ -251,13 +252,18 @@ __global__ void __launch_bounds__(512, 2) k_gemm_mxfp4_dma(const uint8_t* __rest
 // 5 % more at 2048, a third workgroup on a CU (of 168 registers a wave) 12 %.
 constexpr int kMoeNF = 1, kMoeD = 4, kMoeCols = 128 * kMoeNF, kMoeRows = 128;
 
+//
+// The tiles and the table come from the device, where no host check sees them: an expert or a row beyond what the caller says
+// the buffers hold is taken as the last one, and rows of D beyond its end are left out.
+struct MoeBounds { int experts, rows, xrows; };
+
 template <int MF, bool BF>
-__device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_xmx x, const int* rowtab, int k0, int n, int n0, void* D, int N, int K128,
-                                         int vec) {
+__device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_xmx x, const int* rowtab, int xrows, int k0, int n, int n0, void* D, int N,
+                                         int K128, int vec) {
     mx_v16f acc[kMoeNF][MF];
     mx_tile_reg<MF, kMoeNF, kMoeD, false>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
         const int k = k0 + min(r, n - 1);
-        return rowtab ? rowtab[k] : k;
+        return rowtab ? min(max(rowtab[k], 0), xrows - 1) : k;
     }, acc);
     mx_store<MF, kMoeNF, BF>(smem, acc, D, n0 + 32 * kMoeNF * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return r < n ? (int64_t)(k0 + r) : -1; });
 }
@@ -266,19 +272,20 @@ template <bool BF>
 __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __restrict__ W, const uint8_t* __restrict__ Wsh, size_t ebytes,
                                                            const qmm_moe_tile* __restrict__ tiles, const int* __restrict__ counts,
                                                            const int* __restrict__ rowtab, qmm_xmx x, void* __restrict__ D, int N, int K128,
-                                                           uint32_t nblocks, int vec) {
+                                                           uint32_t nblocks, int vec, MoeBounds b) {
     extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t ti = blockIdx.x / nblocks;
     if (ti >= (uint32_t)(counts[0] + counts[1])) return;
     const qmm_moe_tile t = tiles[ti];
     const int n0 = (int)(blockIdx.x - ti * nblocks) * kMoeCols;
-    const uint8_t* We = t.expert < 0 ? (Wsh ? Wsh : W) : W + (size_t)t.expert * ebytes;
-    for (int r = 0; r < t.ncols; r += kMoeRows) {
-        const int n = min(t.ncols - r, kMoeRows);
-        if (n <= 32) moe_rows<1, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else if (n <= 64) moe_rows<2, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else if (n <= 96) moe_rows<3, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
-        else moe_rows<4, BF>(smem, We, x, rowtab, t.k0 + r, n, n0, D, N, K128, vec);
+    const uint8_t* We = t.expert < 0 ? (Wsh ? Wsh : W) : W + (size_t)min(t.expert, b.experts - 1) * ebytes;
+    const int rows = t.k0 < 0 ? 0 : min(t.ncols, b.rows - t.k0);
+    for (int r = 0; r < rows; r += kMoeRows) {
+        const int n = min(rows - r, kMoeRows);
+        if (n <= 32) moe_rows<1, BF>(smem, We, x, rowtab, b.xrows, t.k0 + r, n, n0, D, N, K128, vec);
+        else if (n <= 64) moe_rows<2, BF>(smem, We, x, rowtab, b.xrows, t.k0 + r, n, n0, D, N, K128, vec);
+        else if (n <= 96) moe_rows<3, BF>(smem, We, x, rowtab, b.xrows, t.k0 + r, n, n0, D, N, K128, vec);
+        else moe_rows<4, BF>(smem, We, x, rowtab, b.xrows, t.k0 + r, n, n0, D, N, K128, vec);
         __syncthreads();                                 // LDS is filled again
     }
 }
@@ -383,6 +390,25 @@ int launch_gemv_moe(const void* W, const void* Wsh, size_t ebytes, const int* id
     return QMM_OK;
 }
 
+int launch_moe_gemm(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
+                    qmm_xmx x, void* D, int dtype, int N, int K, MoeBounds b, hipStream_t s) {
+    if (ebytes % 16 != 0 || misaligned(Wsh, 16) || misaligned(tiles, 4) || misaligned(counts, 4) || misaligned(rowtab, 4)) return QMM_ERR_ARG;
+    if (max_tiles == 0 || b.rows == 0) return QMM_OK;
+    const uint32_t nblocks = ((uint32_t)N + kMoeCols - 1) / kMoeCols;
+    if ((uint64_t)nblocks * max_tiles > 0x7fffffffu) return QMM_ERR_SHAPE;
+    const int K128 = mx_steps(K);
+    const dim3 grid(nblocks * (uint32_t)max_tiles);
+    constexpr size_t lds = MxReg<kMoeRows / 32, kMoeNF>::kLds;
+    if (dtype == QMM_BF16)
+        hipLaunchKernelGGL(k_moe_gemm_mxfp4<true>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
+                           K128, nblocks, vec16_out(D, dtype, N), b);
+    else
+        hipLaunchKernelGGL(k_moe_gemm_mxfp4<false>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
+                           K128, nblocks, vec16_out(D, dtype, N), b);
+    QMM_LAUNCH_CHECK();
+    return QMM_OK;
+}
+
 }  // namespace
 }  // namespace qmm
 
@@ -429,28 +455,23 @@ int qmm_gemm_mxfp4_tile(int M, int N, int K) {
     return (int)(&pick_tile(M, N, mx_steps(K)) - kMxTiles);
 }
 
+int qmm_moe_gemm_mxfp4_n(const void* W, const void* Wsh, size_t ebytes, int nexperts, const qmm_moe_tile* tiles, const int* counts, int max_tiles,
+                         const int* rowtab, int rows, qmm_xmx x, int xrows, void* D, int dtype, int N, int K, void* stream) {
+    const int st = check_operands(W, x, D, dtype, N, K);
+    if (st != QMM_OK) return st;
+    if (!tiles || !counts) return QMM_ERR_NULL;
+    if (max_tiles < 0 || nexperts < 1 || rows < 0 || xrows < (rowtab ? (rows > 0) : rows)) return QMM_ERR_SHAPE;
+    if (nexperts > 1 && ebytes < qmm_mxfp4_weight_bytes(N, K)) return QMM_ERR_ARG;
+    return launch_moe_gemm(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, dtype, N, K, MoeBounds{nexperts, rows, xrows}, (hipStream_t)stream);
+}
+
 int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
                        qmm_xmx x, void* D, int dtype, int N, int K, void* stream) {
     const int st = check_operands(W, x, D, dtype, N, K);
     if (st != QMM_OK) return st;
     if (!tiles || !counts) return QMM_ERR_NULL;
     if (max_tiles < 0) return QMM_ERR_SHAPE;
-    if (ebytes % 16 != 0 || misaligned(Wsh, 16) || misaligned(tiles, 4) || misaligned(counts, 4) || misaligned(rowtab, 4)) return QMM_ERR_ARG;
-    if (max_tiles == 0) return QMM_OK;
-    const uint32_t nblocks = ((uint32_t)N + kMoeCols - 1) / kMoeCols;
-    if ((uint64_t)nblocks * max_tiles > 0x7fffffffu) return QMM_ERR_SHAPE;
-    const int K128 = mx_steps(K);
-    const dim3 grid(nblocks * (uint32_t)max_tiles);
-    constexpr size_t lds = MxReg<kMoeRows / 32, kMoeNF>::kLds;
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == QMM_BF16)
-        hipLaunchKernelGGL(k_moe_gemm_mxfp4<true>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
-                           K128, nblocks, vec16_out(D, dtype, N));
-    else
-        hipLaunchKernelGGL(k_moe_gemm_mxfp4<false>, grid, dim3(256), lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, tiles, counts, rowtab, x, D, N,
-                           K128, nblocks, vec16_out(D, dtype, N));
-    QMM_LAUNCH_CHECK();
-    return QMM_OK;
+    return launch_moe_gemm(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, dtype, N, K, MoeBounds{INT_MAX, INT_MAX, INT_MAX}, (hipStream_t)stream);
 }
 
 }  // extern "C"

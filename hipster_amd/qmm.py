@@ -385,6 +385,7 @@ def moe_gemm(fmt, shared_fmt, W, Wsh, ebytes, tiles, ntiles, stiles, nstiles, ct
 # ---- MXFP4 decoder blocks ----
 # These calls answer in a few microseconds on the device, so their checks are kept to one pass over each
 # tensor and the arguments go to the library as plain integers.
+_INT_MAX = (1 << 31) - 1
 _DTYPE = {torch.float32: _lib.QMM_F32, torch.bfloat16: _lib.QMM_BF16}
 _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda d: torch.cuda.current_stream(d).cuda_stream)
@@ -478,10 +479,14 @@ def mxfp4_weight_bytes(N, K):
     return _lib.lib().qmm_mxfp4_weight_bytes(N, K)
 
 
+def _wbytes(N, K):
+    steps = (K + 127) // 128
+    return (N + 15) // 16 * (steps * 1024 + (steps + 3) // 4 * 256)
+
+
 def _weight(W, N, K, name="W", extra=0):
     """The address of a packed weight of N rows of K values, `extra` bytes into its buffer."""
-    steps = (K + 127) // 128
-    return _in(W, extra + (N + 15) // 16 * (steps * 1024 + (steps + 3) // 4 * 256), name, torch.uint8)
+    return _in(W, extra + _wbytes(N, K), name, torch.uint8)
 
 
 def _experts(W, N, K, ebytes, n):
@@ -535,12 +540,21 @@ def gemv_moe_mxfp4(W, Wsh, ebytes, ids, x, y, T, nslot, nexperts, N, K, xrow_te=
                                         _dtype(y, "y"), T, nslot, nexperts, N, K, int(xrow_te), _handle(stream)), "gemv_moe_mxfp4")
 
 
-def moe_gemm_mxfp4(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, N, K, stream=None):
-    """D[k] = W_e . x[rowtab[k]] over rows sorted by expert (moe_sort's tiles, counts, rowtok; rowtab None: x[k])."""
-    check(_lib.lib().qmm_moe_gemm_mxfp4(_experts(W, N, K, ebytes, 1), None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes,
-                                        _in(tiles, 3 * max_tiles, "tiles", torch.int32), _in(counts, 2, "counts", torch.int32), max_tiles,
-                                        None if rowtab is None else _in(rowtab, 0, "rowtab", torch.int32), _xmx(x, 0, K, "x"), _in(D, 0, "D"),
-                                        _dtype(D, "D"), N, K, _handle(stream)), "moe_gemm_mxfp4")
+def moe_gemm_mxfp4(W, Wsh, ebytes, tiles, counts, max_tiles, rowtab, x, D, N, K, stream=None, rows=None, nexperts=None):
+    """D[k] = W_e . x[rowtab[k]] over rows sorted by expert (moe_sort's tiles, counts, rowtok; rowtab None: x[k]).
+
+    rows: how many the tiles hold at most, which D and rowtab must have room for (None: as many as rowtab has, or without
+    it x); nexperts: of W (None: as many as it holds).  Tiles that name others reach nothing outside the tensors."""
+    pw = _experts(W, N, K, ebytes, 1 if nexperts is None else nexperts)
+    if nexperts is None:
+        nexperts = min(1 + (W.numel() - _wbytes(N, K)) // ebytes, _INT_MAX) if ebytes else 1
+    xrows = min(x.q.numel() // (64 * max(1, (K + 127) // 128)), _INT_MAX)
+    if rows is None:
+        rows = xrows if rowtab is None else rowtab.numel()
+    check(_lib.lib().qmm_moe_gemm_mxfp4_n(pw, None if Wsh is None else _weight(Wsh, N, K, "Wsh"), ebytes, nexperts,
+                                          _in(tiles, 3 * max_tiles, "tiles", torch.int32), _in(counts, 2, "counts", torch.int32), max_tiles,
+                                          None if rowtab is None else _in(rowtab, rows, "rowtab", torch.int32), rows, _xmx(x, xrows, K, "x"), xrows,
+                                          _in(D, rows * N, "D"), _dtype(D, "D"), N, K, _handle(stream)), "moe_gemm_mxfp4")
 
 
 _SCORE = {"softmax": 0, "sigmoid": 1}

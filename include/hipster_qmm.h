@@ -445,6 +445,12 @@ int qmm_gemm_mxfp4_tile(int M, int N, int K);
  * is NULL) for expert -1.  max_tiles bounds the grid.  A row has the bits of qmm_gemm_mxfp4. */
 int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
                        qmm_xmx x, void* D, int dtype, int N, int K, void* stream);
+/* the same with what the buffers hold: nexperts weights at W, `rows` rows of D (and entries of rowtab), xrows rows of x.
+ * Tiles and table are device data that no host check sees; here they cannot lead out of the buffers: an expert
+ * or an x row beyond the last is the last, and rows of D from `rows` on are left as they were.  ebytes at least one weight where
+ * nexperts > 1; without a table xrows >= rows. */
+int qmm_moe_gemm_mxfp4_n(const void* W, const void* Wsh, size_t ebytes, int nexperts, const qmm_moe_tile* tiles, const int* counts, int max_tiles,
+                         const int* rowtab, int rows, qmm_xmx x, int xrows, void* D, int dtype, int N, int K, void* stream);
 /* Experts of each token from logits [T][stride] by rule (above): ids / w [T][topk + (shared != 0)] in falling order of
  * the choice value, ties to the lower id.  Scores and comparisons are in 64 bits, a weight is rounded once.  An
  * expert whose logit or bias is -inf or NaN is never chosen and counts in no group; a slot without an expert gets id

@@ -1,0 +1,94 @@
+"""What the MXFP4 block operators refuse before a device is asked: status codes of the library, and the checks of the Python
+mirror on stand-ins for device tensors.  No call below reaches a device."""
+import ctypes
+
+import pytest
+import torch
+
+from hipster_amd import _lib, qmm
+from hipster_amd._lib import QmmError, XMX
+
+FORMAT, SHAPE, NULL, ARG = -1, -2, -3, -6
+D = ctypes.c_void_p(64)                       # a non-null, aligned pointer that nothing dereferences
+X = XMX(64, 64)
+
+
+class OnDevice:
+    """A tensor as the checks see one: on device 0, contiguous, its address nothing that is read."""
+    is_cuda = True
+
+    def __init__(self, n, dtype):
+        self.n, self.dtype, self.device = n, dtype, "cuda:0"
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def numel(self):
+        return self.n
+
+    def data_ptr(self):
+        return 4096
+
+
+class Rows:
+    """An XMXBuf of such tensors."""
+
+    def __init__(self, rows, K):
+        self.rows, self.K = rows, K
+        self.q, self.e = (OnDevice(rows * per * qmm.mxfp4_steps(K), torch.uint8) for per in (64, 4))
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The arguments of the library calls that get through, which do nothing."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or 0
+
+    monkeypatch.setattr(qmm, "_device", lambda: 0)
+    monkeypatch.setattr(qmm, "_raw_stream", lambda d: 0)
+    monkeypatch.setattr(_lib, "lib", lambda: Lib())
+    return calls
+
+
+def test_sorted_experts_sizes(launched):
+    """D, the table, x and the experts' weights hold what the tiles may name, or the call is refused."""
+    E, TS, N, K, cap = 4, 24, 40, 300, 9
+    one = 3 * (3 * 1024 + 256)
+    i32, u8, f32 = torch.int32, torch.uint8, torch.float32
+
+    def call(w=E * one, tab=TS, d=TS * N, xr=6, eb=one, **kw):
+        qmm.moe_gemm_mxfp4(OnDevice(w, u8), None, eb, OnDevice(3 * cap, i32), OnDevice(2, i32), cap, None if tab is None else OnDevice(tab, i32),
+                           Rows(xr, K), OnDevice(d, f32), N, K, **kw)
+
+    call()
+    call(tab=None, xr=TS)
+    call(tab=None, xr=TS + 8, rows=TS)
+    call(tab=TS + 8, rows=TS)
+    call(nexperts=E)
+    assert len(launched) == 5
+    for kw, what in ((dict(d=TS * N - 1), "D holds"), (dict(d=6 * N), "D holds"), (dict(tab=None, xr=TS, d=TS * N - N), "D holds"),
+                     (dict(tab=TS - 1, rows=TS), "rowtab holds"), (dict(nexperts=E + 1), "W holds"), (dict(w=one - 16), "W holds")):
+        with pytest.raises(QmmError, match=what):
+            call(**kw)
+    assert len(launched) == 5
+    # the bounds that the device gets
+    name, a = launched[0]
+    assert name == "qmm_moe_gemm_mxfp4_n" and (a[3], a[8], a[10]) == (E, TS, 6)
+
+
+def test_sorted_experts_refusals():
+    L, one = _lib.lib(), qmm.mxfp4_weight_bytes(32, 64)
+
+    def f(W=D, eb=one, E=2, tiles=D, counts=D, n=4, tab=D, rows=8, xrows=8, N=32, K=64, dtype=0):
+        return L.qmm_moe_gemm_mxfp4_n(W, None, eb, E, tiles, counts, n, tab, rows, X, xrows, D, dtype, N, K, None)
+
+    assert f(W=None) == NULL and f(tiles=None) == NULL and f(counts=None) == NULL and f(dtype=2) == FORMAT
+    assert f(E=0) == SHAPE and f(rows=-1) == SHAPE and f(xrows=0) == SHAPE and f(tab=None, xrows=7) == SHAPE and f(n=-1) == SHAPE
+    assert f(eb=one - 16) == ARG and f(eb=0) == ARG and f(eb=one + 8) == ARG and f(tab=ctypes.c_void_p(66)) == ARG
+    assert f(rows=0) == 0 and f(rows=0, xrows=0) == 0 and f(n=0) == 0

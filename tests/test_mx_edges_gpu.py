@@ -61,3 +61,55 @@ def test_route_bias_that_masks(gpu, score):
     b[32:] = 0.0                                                         # groups without an expert lose
     ids, _ = route(l[2:], 64, 6, score=score, bias=b, groups=8, keep=4, best=2)
     assert (ids >= 32).all()
+
+
+def packed(rng, n, N, K):
+    """n weights packed one after another, and their values."""
+    W, vals = torch.empty(n, qmm.mxfp4_weight_bytes(N, K), dtype=torch.uint8, device="cuda"), []
+    for i in range(n):
+        c, b = mx_ref.random_rows(rng, N, K)
+        qmm.pack_mxfp4(dev(mx_ref.pack(c)), dev(b), W[i], N, K)
+        vals.append(mx_ref.values(c, b))
+    return W, vals
+
+
+def rows_of(code, byte):
+    b = qmm.XMXBuf(*code.shape)
+    b.q.copy_(dev(mx_ref.pack(code)))
+    b.e.copy_(dev(byte))
+    return b
+
+
+def test_sorted_experts_stay_inside_their_buffers(gpu):
+    """Tiles and a table of another model: experts and rows beyond the last are the last, rows past the end of D stay."""
+    rng = np.random.default_rng(2)
+    E, N, K, TX, ROWS, ALL = 3, 72, 200, 5, 40, 64
+    W, vals = packed(rng, E, N, K)
+    ac, ab = mx_ref.random_rows(rng, TX, K)
+    a = mx_ref.values(ac, ab)
+    tab = rng.integers(-2, TX + 3, ALL).astype(np.int32)
+    tab[[3, 9]] = 2 ** 31 - 1, -2 ** 31
+    tiles = np.array([(0, 0, 10), (7, 10, 20), (1, 30, 10 ** 9), (2, ROWS, 8), (2 ** 31 - 1, 2 ** 31 - 1, 128), (0, -8, 4), (1, 2, -5)], np.int32)
+    counts = dev(np.array([2 ** 30, 5], np.int32))                       # more tiles than there are
+    D = torch.full((ALL, N), -7.0, device="cuda")
+    qmm.moe_gemm_mxfp4(W, None, W.shape[1], dev(tiles), counts, len(tiles), dev(tab), rows_of(ac, ab), D, N, K, rows=ROWS)
+    got = host(D)
+    expert = np.repeat([0, E - 1, 1], [10, 20, ROWS - 30])
+    ref, bound = np.empty((ROWS, N)), np.empty((ROWS, N))
+    for r in range(ROWS):
+        ref[r], bound[r] = (v[0] for v in mx_ref.product_bound(a[[min(max(tab[r], 0), TX - 1)]], vals[expert[r]], K))
+    assert (np.abs(got[:ROWS] - ref) <= bound).all()
+    assert (got[ROWS:] == -7).all()
+
+
+def test_sorted_experts_refuse_short_buffers(gpu):
+    W, _ = packed(np.random.default_rng(3), 2, 32, 128)
+    tiles, counts, tab = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((4, 3), 2, 12))
+    x, D = qmm.XMXBuf(4, 128), torch.full((12, 32), -7.0, device="cuda")
+    f = lambda D=D, tab=tab, **kw: qmm.moe_gemm_mxfp4(W, None, W.shape[1], tiles, counts, 4, tab, x, D, 32, 128, **kw)      # noqa: E731
+    f()
+    f(D=D[:11], rows=11)
+    for bad in (lambda: f(D=D[:4]), lambda: f(D=D[:11]), lambda: f(tab=tab[:11], rows=12), lambda: f(nexperts=3), lambda: f(tab=None, rows=5)):
+        with pytest.raises(QmmError):
+            bad()
+    assert (host(D) == -7).all()
