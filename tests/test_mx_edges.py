@@ -20,8 +20,13 @@ class OnDevice:
     def __init__(self, n, dtype):
         self.n, self.dtype, self.device = n, dtype, "cuda:0"
 
+        self.shape = (n,)
+
     def is_contiguous(self):
         return True
+
+    def stride(self, dim):
+        return 1
 
     def get_device(self):
         return 0
@@ -92,3 +97,25 @@ def test_sorted_experts_refusals():
     assert f(E=0) == SHAPE and f(rows=-1) == SHAPE and f(xrows=0) == SHAPE and f(tab=None, xrows=7) == SHAPE and f(n=-1) == SHAPE
     assert f(eb=one - 16) == ARG and f(eb=0) == ARG and f(eb=one + 8) == ARG and f(tab=ctypes.c_void_p(66)) == ARG
     assert f(rows=0) == 0 and f(rows=0, xrows=0) == 0 and f(n=0) == 0
+
+
+@pytest.mark.parametrize("ds", [False, True])
+def test_norm_to_q8_elsewhere(launched, ds):
+    """The q8 rows of a norm are on the device that it runs on, as its other tensors are."""
+    n, v = 64, OnDevice(64, torch.float32)
+    good = qmm.XQ8Buf(1, n, device="cpu", with_ds=ds)
+    good.q, good.d, good.s = OnDevice(n, torch.int8), OnDevice(2, torch.float32), OnDevice(2, torch.float32)
+    good.ds = OnDevice(4, torch.float32) if ds else None
+    qmm.postnorm_add_rmsnorm_quant(v, v, v, v, v, good, 1, n, 1e-6)
+    assert len(launched) == 1
+    for part in ("q", "d", "s") + (("ds",) if ds else ()):
+        for wrong in (getattr(qmm.XQ8Buf(1, n, device="cpu", with_ds=ds), part), "other"):
+            bad = qmm.XQ8Buf(1, n, device="cpu", with_ds=ds)
+            bad.q, bad.d, bad.s, bad.ds = good.q, good.d, good.s, good.ds
+            if wrong == "other":                                         # of another device
+                wrong = OnDevice(getattr(good, part).n, getattr(good, part).dtype)
+                wrong.get_device = lambda: 1
+            setattr(bad, part, wrong)
+            with pytest.raises(QmmError, match="xq"):
+                qmm.postnorm_add_rmsnorm_quant(v, v, v, v, v, bad, 1, n, 1e-6)
+    assert len(launched) == 1
