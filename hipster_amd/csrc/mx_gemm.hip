@@ -45,6 +45,10 @@ int gemv_waves(int G) {
 // LDS of one wave: a pair of 32 rows, and a group's scales of them (16 bytes a row)
 constexpr int kGemvWaveLds = 32 * (128 + 16);
 
+// LDS accesses of a wave before it stay before those after it (no instruction: a wave's LDS accesses are carried out in order,
+// but the compiler may swap a lane's own read and write of different addresses, which are another lane's same ones)
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // this wave's run of K: weight rows of `strip` and the next strip (sb bytes on, or 0 where there is none); row(r):
 // the activation row of tile row r, of which n are real.  No branch lies around a load (the compiler would wait for
 // every load in flight where the paths meet): the last group is a body of its own.
@@ -91,6 +95,7 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
             const int q = 8 * i + (lane >> 3);
             *(uint4*)(lds + q * 128 + ((cj ^ a_swz(q)) << 4)) = r.a[i];
         }
+        wave_lds_fence();                                // other lanes read what this one wrote
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             if (s == steps) break;
@@ -104,6 +109,7 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
                 acc[0][0] = mx_mfma32<2 * P + 1, 2>(r.w[1][1], a1, acc[0][0], sc.w[1], sa);
             }
         }
+        wave_lds_fence();                                // the reads come before the next pair's writes
         pin<false>(acc[0][0]);
         __builtin_amdgcn_sched_barrier(0);
     };
