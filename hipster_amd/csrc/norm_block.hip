@@ -8,8 +8,9 @@
 //
 // rms(v) = sqrt(sum(v^2) / n + eps).  A row is held in registers between its two sums, so x, y and the gate are
 // read once and xo and xn written once; HBM bounds it (one row: the two reductions' latency).  A thread
-// holds C pieces of V values, 4 (16-byte accesses) or 1 (rows that 16-byte accesses do not fit); every load is
-// issued before the first sum.  Sums are f32 in a fixed order: per thread, by halves of the wave, wave by wave.
+// holds C pieces of V values, 4 (n % 4 == 0) or 1; every load is issued before the first sum.  Sums are f32 in a fixed
+// order: per thread, by halves of the wave, wave by wave.  Threads and V go by n alone, so a row's bits depend on
+// nothing but the row, whatever the alignment of its arrays and their strides.
 //
 // 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 29 from caches; 4096 rows 69; one row
 // 6.7, one after another.  Threads go by n alone, since they set the sums' order: 640 of them with two pieces each
@@ -32,23 +33,35 @@ struct NbArgs {
     float alpha, eps;
 };
 
+// four values in memory, at the alignment of one: a vector access may have any (the compiler emits the same
+// instructions as for aligned ones)
+typedef uint32_t nb_u4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t nb_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t nb_u1 __attribute__((aligned(1)));
+typedef uint16_t nb_h1 __attribute__((aligned(1)));
+
 // V values at p + i (16-byte or 8-byte access, or one value); past the row: the address clamped, the value unused
 template <int V>
 __device__ __forceinline__ void nb_load(float (&v)[V], const void* p, int i, int n, bool bf) {
     if constexpr (V == 4) {
         const int k = min(i, n - 4);
         if (bf) {
-            const uint2 r = *(const uint2*)((const uint16_t*)p + k);
+            const nb_u2 r = *(const nb_u2*)((const uint16_t*)p + k);
             v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
             v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
         } else {
-            const float4 r = *(const float4*)((const float*)p + k);
-            v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+            const nb_u4 r = *(const nb_u4*)((const float*)p + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[j]);
         }
     } else {
         const int k = min(i, n - 1);
         v[0] = bf ? bf2f(((const uint16_t*)p)[k]) : ((const float*)p)[k];
     }
+}
+
+__device__ __forceinline__ void nb_store(float* p, const float (&v)[4]) {
+    *(nb_u4*)p = nb_u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
 
 __device__ __forceinline__ float nb_act(float z, int act) {
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(NT) k_norm_block(NbArgs a) {
             ss = fmaf(xv[c][k], xv[c][k], ss);
         }
         if (i < n) {
-            if constexpr (V == 4) *(float4*)(a.xo + t * n + i) = make_float4(xv[c][0], xv[c][1], xv[c][2], xv[c][3]);
+            if constexpr (V == 4) nb_store(a.xo + t * n + i, xv[c]);
             else a.xo[t * n + i] = xv[c][0];
         }
     }
@@ -128,7 +141,7 @@ __global__ void __launch_bounds__(NT) k_norm_block(NbArgs a) {
         if constexpr (OUT == kNbBf16) {
             if (i < n) {
                 if constexpr (V == 4)
-                    *(uint2*)(a.xb + t * n + i) = make_uint2(mx_bf16x2(o[0], o[1]), mx_bf16x2(o[2], o[3]));
+                    *(nb_u2*)(a.xb + t * n + i) = nb_u2{mx_bf16x2(o[0], o[1]), mx_bf16x2(o[2], o[3])};
                 else a.xb[t * n + i] = (uint16_t)mx_bf16x2(o[0], 0.f);
             }
         } else if constexpr (OUT == kNbQ8) {             // n % 32 == 0: a block's lanes are in the row together
@@ -143,8 +156,8 @@ __global__ void __launch_bounds__(NT) k_norm_block(NbArgs a) {
             sum = V == 4 ? g8_isum(sum) : g32_isum(sum);
             if (i < n) {
                 if constexpr (V == 4) {
-                    *(float4*)(a.xn + t * n + i) = make_float4(o[0], o[1], o[2], o[3]);
-                    *(uint32_t*)(a.q8.q + t * n + i) = (uint32_t)(q[0] & 0xff) | ((uint32_t)(q[1] & 0xff) << 8) | ((uint32_t)(q[2] & 0xff) << 16) |
+                    nb_store(a.xn + t * n + i, o);
+                    *(nb_u1*)(a.q8.q + t * n + i) = (uint32_t)(q[0] & 0xff) | ((uint32_t)(q[1] & 0xff) << 8) | ((uint32_t)(q[2] & 0xff) << 16) |
                                                        ((uint32_t)q[3] << 24);
                 } else {
                     a.xn[t * n + i] = o[0];
@@ -175,7 +188,7 @@ __global__ void __launch_bounds__(NT) k_norm_block(NbArgs a) {
                 if constexpr (V == 4) {
                     uint32_t b = 0;
                     if (byte != 255) b = mx_codes2<1>(mx_codes2<0>(0u, o[0] * inv, o[1] * inv), o[2] * inv, o[3] * inv);
-                    *(uint16_t*)q = (uint16_t)b;
+                    *(nb_h1*)q = (uint16_t)b;
                 } else {
                     const float u = o[0] * inv, u1 = __int_as_float(dpp_i<kDppXor1>(__float_as_int(u)));
                     if ((i & 1) == 0) *q = (uint8_t)(byte == 255 ? 0u : mx_codes2<0>(0u, u, u1));
@@ -207,32 +220,21 @@ int nb_args(const float* x, const void* y, int y_dtype, size_t ldy, const float*
     return QMM_OK;
 }
 
-// whether every row of every array takes accesses of four values
-bool nb_vec(const NbArgs& a) {
-    const bool rows = a.n % 4 == 0 && !misaligned(a.x, 16) && !misaligned(a.xo, 16) && !misaligned(a.w, 16) && !misaligned(a.wy, 16) &&
-                      a.ldy % 4 == 0 && !misaligned(a.y, a.y_bf ? 8 : 16);
-    const bool gate = !a.gate || !a.per_value || (a.ldg % 4 == 0 && !misaligned(a.gate, a.gate_bf ? 8 : 16));
-    const bool out = !misaligned(a.xb, 8) && !misaligned(a.xn, 16) && !misaligned(a.q8.q, 4) && !misaligned(a.mx.q, 2);
-    return rows && gate && out;
-}
-
 template <NbOut OUT>
 int nb_launch(const NbArgs& a, int T, hipStream_t s) {
     if (T == 0) return QMM_OK;
     const int len = OUT == kNbMx ? mx_steps(a.n) * 128 : a.n;      // values written per row
     const dim3 grid((unsigned)T);
 #define QMM_NB(NT, V, C) hipLaunchKernelGGL((k_norm_block<NT, V, C, OUT>), grid, dim3(NT), 0, s, a)
-    if (nb_vec(a)) {
-        if (len <= 1024) QMM_NB(256, 4, 1);
-        else if (len <= 2048) QMM_NB(256, 4, 2);
-        else if (len <= 4096) QMM_NB(256, 4, 4);
-        else if (len <= 5120) QMM_NB(256, 4, 5);
-        else if (len <= 8192) QMM_NB(512, 4, 4);
-        else QMM_NB(1024, 4, 4);
-    } else {
+    if (a.n % 4 != 0) {
         if (len <= 4096) QMM_NB(1024, 1, 4);
         else QMM_NB(1024, 1, 16);
-    }
+    } else if (len <= 1024) QMM_NB(256, 4, 1);
+    else if (len <= 2048) QMM_NB(256, 4, 2);
+    else if (len <= 4096) QMM_NB(256, 4, 4);
+    else if (len <= 5120) QMM_NB(256, 4, 5);
+    else if (len <= 8192) QMM_NB(512, 4, 4);
+    else QMM_NB(1024, 4, 4);
 #undef QMM_NB
     QMM_LAUNCH_CHECK();
     return QMM_OK;

@@ -113,3 +113,52 @@ def test_sorted_experts_refuse_short_buffers(gpu):
         with pytest.raises(QmmError):
             bad()
     assert (host(D) == -7).all()
+
+
+def shifted(t, by):
+    """t's values in rows that start `by` elements off an aligned address and lie an odd number of elements apart (2-d)."""
+    if t.dim() == 1:
+        out = torch.zeros(len(t) + 8, dtype=t.dtype, device="cuda")[by:by + len(t)]
+    else:
+        out = torch.zeros(t.shape[0], t.shape[1] + 9 - t.shape[1] % 2, dtype=t.dtype, device="cuda")[:, by:by + t.shape[1]]
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("ydt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [4, 32, 640, 2880, 4100, 5120, 5632, 8192, 12288, 16384])
+def test_norm_bits_do_not_depend_on_alignment(gpu, n, ydt):
+    """A row has the same bits wherever its arrays lie, and whether it is one of many or alone."""
+    g = torch.Generator().manual_seed(n)
+    T, eps = 3, 1e-6
+    x, y, gate = (torch.randn(T, n, generator=g).cuda() for _ in range(3))
+    y, gate = y.to(ydt), gate.to(ydt)
+    wy, w = ((1 + 0.2 * torch.randn(n, generator=g)).cuda() for _ in range(2))
+
+    def run(x, y, wy, w, gate, off, rows=T):
+        flat = lambda dt: torch.full((rows * n + 8,), 7.0, device="cuda").to(dt)     # noqa: E731
+        xo, xb, xn = flat(torch.float32)[off:], flat(torch.bfloat16)[off:], flat(torch.float32)[off:]
+        kw = dict(gate=gate, act="silu", xo=xo, alpha=0.5)
+        qmm.postnorm_add_rmsnorm_bf16(x, y, wy, w, xb, rows, n, eps, **kw)
+        out = [xo[:rows * n].clone(), xb[:rows * n]]
+        m = qmm.XMXBuf(rows, n)
+        if off:
+            m.q = torch.zeros(m.q.numel() + 8, dtype=torch.uint8, device="cuda")[off:off + m.q.numel()].view(m.q.shape)
+        qmm.postnorm_add_rmsnorm_mxfp4(x, y, wy, w, m, rows, n, eps, **kw)
+        out += [xo[:rows * n].clone(), m.q, m.e]
+        if n % 32 == 0:
+            q8 = qmm.XQ8Buf(rows, n)
+            if off:
+                q8.q = torch.zeros(rows * n + 8, dtype=torch.int8, device="cuda")[off:off + rows * n].view(rows, n)
+            qmm.postnorm_add_rmsnorm_quant(x, y, wy, w, xn, q8, rows, n, eps, **kw)
+            out += [xo[:rows * n].clone(), xn[:rows * n], q8.q, q8.d, q8.s]
+        assert (xo[rows * n:] == 7).all() and (xb[rows * n:] == 7).all() and (n % 32 or (xn[rows * n:] == 7).all())
+        return [t.clone() for t in out]
+
+    want = run(x, y, wy, w, gate, 0)
+    xs = torch.zeros(T * n + 8, device="cuda")[1:1 + T * n].view(T, n).copy_(x)
+    for got in (run(x, shifted(y, 0), wy, w, gate, 0), run(x, shifted(y, 3), wy, w, shifted(gate, 1), 0), run(xs, y, shifted(wy, 1), shifted(w, 2), gate, 0),
+                run(x, y, wy, w, gate, 1), run(xs, shifted(y, 1), shifted(wy, 3), shifted(w, 3), shifted(gate, 5), 3)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = run(x[2:], shifted(y, 3)[2:], wy, w, shifted(gate, 1)[2:], 0, rows=1)
+    assert torch.equal(one[0], want[0][2 * n:]) and torch.equal(one[1], want[1][2 * n:]) and torch.equal(one[3][0], want[3][2])
