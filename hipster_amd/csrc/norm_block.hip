@@ -12,9 +12,15 @@
 // order: per thread, by halves of the wave, wave by wave.  Threads and V go by n alone, so a row's bits depend on
 // nothing but the row, whatever the alignment of its arrays and their strides.
 //
-// 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 29 from caches; 4096 rows 69; one row
-// 6.7, one after another.  Threads go by n alone, since they set the sums' order: 640 of them with two pieces each
-// take 5.0 for one row and 9.5 instead of 11.1 for 300, but 41 for 2048 (448 with three 40, 320 with four 53).
+// 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 29 from caches; one row 6.6, one
+// after another.  Rows that start anywhere and lie an odd number of values apart: the same.
+//
+// Threads go by the row's length alone, since they set the order of its sums; pieces are as few as cover it (2048 rows, us):
+//   256 threads up to five pieces: 5120 values 37.5 (512 threads with three: 41.3); with a sixth a wave has more
+//     than 128 registers, three a SIMD instead of four: 5248 values 49.4, 512 threads with three 41.8
+//   512 threads up to 8192 values: 55.5 (1024 with two: 68)
+//   1024 beyond: 8320 values 82 (512 with five would take 65, in another order of sums)
+// One row alone would like more threads (5120 values: 640 with two 4.8 against 6.6), 300 rows too (9.3 against 10.7).
 #include "mx.hpp"
 
 namespace qmm {
@@ -231,9 +237,12 @@ int nb_launch(const NbArgs& a, int T, hipStream_t s) {
         else QMM_NB(1024, 1, 16);
     } else if (len <= 1024) QMM_NB(256, 4, 1);
     else if (len <= 2048) QMM_NB(256, 4, 2);
+    else if (len <= 3072) QMM_NB(256, 4, 3);
     else if (len <= 4096) QMM_NB(256, 4, 4);
     else if (len <= 5120) QMM_NB(256, 4, 5);
+    else if (len <= 6144) QMM_NB(512, 4, 3);
     else if (len <= 8192) QMM_NB(512, 4, 4);
+    else if (len <= 12288) QMM_NB(1024, 4, 3);
     else QMM_NB(1024, 4, 4);
 #undef QMM_NB
     QMM_LAUNCH_CHECK();

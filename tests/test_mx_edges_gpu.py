@@ -162,3 +162,26 @@ def test_norm_bits_do_not_depend_on_alignment(gpu, n, ydt):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     one = run(x[2:], shifted(y, 3)[2:], wy, w, shifted(gate, 1)[2:], 0, rows=1)
     assert torch.equal(one[0], want[0][2 * n:]) and torch.equal(one[1], want[1][2 * n:]) and torch.equal(one[3][0], want[3][2])
+
+
+@pytest.mark.parametrize("n", [1024, 1028, 2048, 2052, 3072, 3076, 4096, 4100, 5120, 5124, 6144, 6148, 8192, 8196, 12288, 12292, 16384])
+def test_norm_widths_around_its_launches(gpu, n):
+    """Both sides of every width at which the launch changes, all outputs."""
+    g = torch.Generator().manual_seed(n)
+    T, eps = 2, 1e-6
+    x, y = torch.randn(T, n, generator=g).cuda() * 3, torch.randn(T, n, generator=g).cuda()
+    wy, w = ((1 + 0.2 * torch.randn(n, generator=g)).cuda() for _ in range(2))
+    xo, xn, bo, bn = mx_ref.postnorm(host(x), host(y), host(wy), host(w), None, "none", 1.0, eps)
+    out, xb, m = torch.empty_like(x), torch.full((T + 1, n), 7.0, device="cuda").bfloat16(), qmm.XMXBuf(T, n)
+    qmm.postnorm_add_rmsnorm_bf16(x, y, wy, w, xb, T, n, eps, xo=out)
+    assert (np.abs(host(out) - xo) <= bo).all()
+    assert (np.abs(host(xb[:T].float()) - xn) <= bn + 2.0 ** -8 * (np.abs(xn) + bn)).all() and (xb[T] == 7).all()
+    out2 = torch.empty_like(x)
+    qmm.postnorm_add_rmsnorm_mxfp4(x, y, wy, w, m, T, n, eps, xo=out2)
+    assert torch.equal(out2, out)
+    if n % 32 == 0:
+        f, q8, mq = torch.empty_like(x), qmm.XQ8Buf(T, n), qmm.XMXBuf(T, n)
+        qmm.postnorm_add_rmsnorm_quant(x, y, wy, w, f, q8, T, n, eps, xo=out2)
+        assert torch.equal(out2, out) and (np.abs(host(f) - xn) <= bn).all() and torch.equal(f.bfloat16(), xb[:T])
+        qmm.quantize_mxfp4(f, mq, T, n)
+        assert torch.equal(mq.q, m.q) and torch.equal(mq.e, m.e)
