@@ -298,9 +298,9 @@ __global__ void __launch_bounds__(256, 2) k_moe_gemm_mxfp4(const uint8_t* __rest
 
 bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
-// what every product checks of its operands
-int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int N, int K) {
-    if (!W || !x.q || !x.e || !y) return QMM_ERR_NULL;
+// what every product checks of its operands (rows: 0 if it has none, and then needs no buffers of them)
+int check_operands(const void* W, qmm_xmx x, const void* y, int dtype, int rows, int N, int K) {
+    if (!W || (rows != 0 && (!x.q || !x.e || !y))) return QMM_ERR_NULL;
     if (dtype != QMM_F32 && dtype != QMM_BF16) return QMM_ERR_FORMAT;
     if (N <= 0 || N > kMxMaxRows || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
     if (misaligned(W, 16) || misaligned(x.q, 16) || misaligned(x.e, 4) || misaligned(y, dtype == QMM_BF16 ? 2 : 4)) return QMM_ERR_ARG;
@@ -423,7 +423,7 @@ using namespace qmm;
 extern "C" {
 
 int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K, void* stream) {
-    const int st = check_operands(W, x, y, dtype, N, K);
+    const int st = check_operands(W, x, y, dtype, ncol, N, K);
     if (st != QMM_OK) return st;
     if (ncol < 0 || ncol > kGemvMaxRows) return QMM_ERR_SHAPE;
     if (ncol == 0) return QMM_OK;
@@ -436,9 +436,9 @@ int qmm_gemv_mxfp4(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N
 
 int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int* ids, qmm_xmx x, void* y, int dtype, int T, int nslot, int nexperts,
                        int N, int K, int xrow_te, void* stream) {
-    const int st = check_operands(W, x, y, dtype, N, K);
+    const int st = check_operands(W, x, y, dtype, T, N, K);
     if (st != QMM_OK) return st;
-    if (!ids) return QMM_ERR_NULL;
+    if (T != 0 && !ids) return QMM_ERR_NULL;
     if (T < 0 || T > kMoeGemvMaxT || nslot < 1 || nslot > kMoeMaxSlots || nexperts < 1) return QMM_ERR_SHAPE;
     if (ebytes % 16 != 0 || (nexperts > 1 && ebytes < qmm_mxfp4_weight_bytes(N, K)) || misaligned(Wsh, 16) || misaligned(ids, 4)) return QMM_ERR_ARG;
     if (T == 0) return QMM_OK;
@@ -447,7 +447,7 @@ int qmm_gemv_moe_mxfp4(const void* W, const void* Wsh, size_t ebytes, const int*
 }
 
 int qmm_gemm_mxfp4(const void* W, qmm_xmx x, void* D, int dtype, int M, int N, int K, void* stream) {
-    const int st = check_operands(W, x, D, dtype, N, K);
+    const int st = check_operands(W, x, D, dtype, M, N, K);
     if (st != QMM_OK) return st;
     if (M < 0 || M > kMxMaxRows) return QMM_ERR_SHAPE;
     if (M == 0) return QMM_OK;
@@ -463,7 +463,7 @@ int qmm_gemm_mxfp4_tile(int M, int N, int K) {
 
 int qmm_moe_gemm_mxfp4_n(const void* W, const void* Wsh, size_t ebytes, int nexperts, const qmm_moe_tile* tiles, const int* counts, int max_tiles,
                          const int* rowtab, int rows, qmm_xmx x, int xrows, void* D, int dtype, int N, int K, void* stream) {
-    const int st = check_operands(W, x, D, dtype, N, K);
+    const int st = check_operands(W, x, D, dtype, rows, N, K);
     if (st != QMM_OK) return st;
     if (!tiles || !counts) return QMM_ERR_NULL;
     if (max_tiles < 0 || nexperts < 1 || rows < 0 || xrows < (rowtab ? (rows > 0) : rows)) return QMM_ERR_SHAPE;
@@ -473,7 +473,7 @@ int qmm_moe_gemm_mxfp4_n(const void* W, const void* Wsh, size_t ebytes, int nexp
 
 int qmm_moe_gemm_mxfp4(const void* W, const void* Wsh, size_t ebytes, const qmm_moe_tile* tiles, const int* counts, int max_tiles, const int* rowtab,
                        qmm_xmx x, void* D, int dtype, int N, int K, void* stream) {
-    const int st = check_operands(W, x, D, dtype, N, K);
+    const int st = check_operands(W, x, D, dtype, 1, N, K);
     if (st != QMM_OK) return st;
     if (!tiles || !counts) return QMM_ERR_NULL;
     if (max_tiles < 0) return QMM_ERR_SHAPE;

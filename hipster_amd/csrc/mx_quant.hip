@@ -152,7 +152,7 @@ size_t qmm_mxfp4_weight_bytes(int N, int K) {
 }
 
 int qmm_quantize_mxfp4(const void* x, int dtype, size_t ldx, qmm_xmx out, int rows, int K, void* stream) {
-    if (!x || !out.q || !out.e) return QMM_ERR_NULL;
+    if (rows != 0 && (!x || !out.q || !out.e)) return QMM_ERR_NULL;
     if (dtype != QMM_F32 && dtype != QMM_BF16) return QMM_ERR_FORMAT;
     if (rows < 0 || K <= 0 || K > kMxMaxK || ldx < (size_t)K) return QMM_ERR_SHAPE;
     if (misaligned(out.q, 16) || misaligned(out.e, 4) || misaligned(x, dtype == QMM_BF16 ? 2 : 4)) return QMM_ERR_ARG;
@@ -174,7 +174,7 @@ int qmm_quantize_mxfp4(const void* x, int dtype, size_t ldx, qmm_xmx out, int ro
 }
 
 int qmm_dequant_mxfp4(qmm_xmx x, void* out, int dtype, int rows, int K, void* stream) {
-    if (!x.q || !x.e || !out) return QMM_ERR_NULL;
+    if (rows != 0 && (!x.q || !x.e || !out)) return QMM_ERR_NULL;
     if (dtype != QMM_F32 && dtype != QMM_BF16) return QMM_ERR_FORMAT;
     if (rows < 0 || K <= 0 || K > kMxMaxK) return QMM_ERR_SHAPE;
     if (misaligned(x.q, 4) || misaligned(out, dtype == QMM_BF16 ? 2 : 4)) return QMM_ERR_ARG;

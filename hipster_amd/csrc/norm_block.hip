@@ -210,7 +210,7 @@ bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t
 // the checks that every output form shares, and the arguments laid out
 int nb_args(const float* x, const void* y, int y_dtype, size_t ldy, const float* wy, const qmm_gate* gate, float alpha, float* xo, const float* w,
             int T, int n, float eps, NbArgs& a) {
-    if (!x || !y || !xo || !w) return QMM_ERR_NULL;
+    if (!w || (T != 0 && (!x || !y || !xo))) return QMM_ERR_NULL;
     if (y_dtype != QMM_F32 && y_dtype != QMM_BF16) return QMM_ERR_FORMAT;
     if (T < 0 || n < 1 || n > kNbMaxN || ldy < (size_t)n) return QMM_ERR_SHAPE;
     a = NbArgs{};
@@ -261,7 +261,7 @@ int qmm_postnorm_add_rmsnorm_bf16(const float* x, const void* y, int y_dtype, si
     NbArgs a;
     const int st = nb_args(x, y, y_dtype, ldy, wy, gate, alpha, xo, w, T, n, eps, a);
     if (st != QMM_OK) return st;
-    if (!xb) return QMM_ERR_NULL;
+    if (T != 0 && !xb) return QMM_ERR_NULL;
     if (misaligned(xb, 2)) return QMM_ERR_ARG;
     a.xb = xb;
     return nb_launch<kNbBf16>(a, T, (hipStream_t)stream);
@@ -272,7 +272,7 @@ int qmm_postnorm_add_rmsnorm_quant(const float* x, const void* y, int y_dtype, s
     NbArgs a;
     const int st = nb_args(x, y, y_dtype, ldy, wy, gate, alpha, xo, w, T, n, eps, a);
     if (st != QMM_OK) return st;
-    if (!xn || !xq.q || !xq.d || !xq.s) return QMM_ERR_NULL;
+    if (T != 0 && (!xn || !xq.q || !xq.d || !xq.s)) return QMM_ERR_NULL;
     if (n % 32 != 0) return QMM_ERR_SHAPE;
     if (misaligned(xn, 4) || misaligned(xq.d, 4) || misaligned(xq.s, 4) || misaligned(xq.ds, 8)) return QMM_ERR_ARG;
     a.xn = xn; a.q8 = xq;
@@ -284,7 +284,7 @@ int qmm_postnorm_add_rmsnorm_mxfp4(const float* x, const void* y, int y_dtype, s
     NbArgs a;
     const int st = nb_args(x, y, y_dtype, ldy, wy, gate, alpha, xo, w, T, n, eps, a);
     if (st != QMM_OK) return st;
-    if (!xq.q || !xq.e) return QMM_ERR_NULL;
+    if (T != 0 && (!xq.q || !xq.e)) return QMM_ERR_NULL;
     a.mx = xq;
     return nb_launch<kNbMx>(a, T, (hipStream_t)stream);
 }

@@ -306,7 +306,7 @@ using namespace qmm;
 
 extern "C" int qmm_moe_route_groups(const float* logits, int stride, const qmm_route_rule* rule, int* ids, float* w, int T, int nexp, int topk,
                                     void* stream) {
-    if (!logits || !rule || !ids || !w) return QMM_ERR_NULL;
+    if (!rule || (T != 0 && (!logits || !ids || !w))) return QMM_ERR_NULL;
     const qmm_route_rule r = *rule;
     if (r.score < 0 || r.score > 1 || r.shared < 0 || r.shared > 2 || r.best < 1 || r.best > 2) return QMM_ERR_ARG;
     if (T < 0 || nexp < 1 || nexp > kRgMaxExp || topk < 1 || topk > kRgMaxK || stride < nexp + (r.shared == 1)) return QMM_ERR_SHAPE;

@@ -119,3 +119,20 @@ def test_norm_to_q8_elsewhere(launched, ds):
             with pytest.raises(QmmError, match="xq"):
                 qmm.postnorm_add_rmsnorm_quant(v, v, v, v, v, bad, 1, n, 1e-6)
     assert len(launched) == 1
+
+
+def test_calls_for_no_rows():
+    """Nothing to do, and no buffers to do it in (an empty tensor has no address); the other arguments are checked as ever."""
+    L, no, eb = _lib.lib(), XMX(None, None), qmm.mxfp4_weight_bytes(32, 64)
+    r = _lib.RouteRule(None, 1.0, 0, 1, 1, 1, 1, 0)
+    q8 = _lib.XQ8(None, None, None, None)
+    calls = [lambda t, n=64: L.qmm_quantize_mxfp4(None, 0, 64, no, t, n, None), lambda t, n=64: L.qmm_dequant_mxfp4(no, None, 0, t, n, None),
+             lambda t, n=64: L.qmm_gemv_mxfp4(D, no, None, 0, t, 32, n, None), lambda t, n=64: L.qmm_gemm_mxfp4(D, no, None, 0, t, 32, n, None),
+             lambda t, n=64: L.qmm_gemv_moe_mxfp4(D, None, eb, None, no, None, 0, t, 4, 8, 32, n, 0, None),
+             lambda t, n=64: L.qmm_moe_gemm_mxfp4_n(D, None, eb, 8, D, D, 4, None, t, no, t, None, 0, 32, n, None),
+             lambda t, n=64: L.qmm_moe_route_groups(None, n, ctypes.byref(r), None, None, t, n, 4, None),
+             lambda t, n=64: L.qmm_postnorm_add_rmsnorm_bf16(None, None, 0, n, None, None, 1.0, None, D, None, t, n, 1e-6, None),
+             lambda t, n=64: L.qmm_postnorm_add_rmsnorm_quant(None, None, 0, n, None, None, 1.0, None, D, None, q8, t, n, 1e-6, None),
+             lambda t, n=64: L.qmm_postnorm_add_rmsnorm_mxfp4(None, None, 0, n, None, None, 1.0, None, D, no, t, n, 1e-6, None)]
+    for i, call in enumerate(calls):
+        assert call(0) == 0 and call(1) == NULL and call(0, 0) == SHAPE, i

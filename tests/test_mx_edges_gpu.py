@@ -185,3 +185,23 @@ def test_norm_widths_around_its_launches(gpu, n):
         assert torch.equal(out2, out) and (np.abs(host(f) - xn) <= bn).all() and torch.equal(f.bfloat16(), xb[:T])
         qmm.quantize_mxfp4(f, mq, T, n)
         assert torch.equal(mq.q, m.q) and torch.equal(mq.e, m.e)
+
+
+def test_no_rows(gpu):
+    """A batch without tokens: every call takes its empty tensors."""
+    T, E, k, n = 0, 8, 2, 64
+    e = lambda *s, dt=torch.float32: torch.empty(s, dtype=dt, device="cuda")         # noqa: E731
+    (W, _), x, xq, w = packed(np.random.default_rng(5), E, 32, n), e(T, n), qmm.XMXBuf(T, n), torch.ones(n, device="cuda")
+    ids, tiles, counts = e(T, k, dt=torch.int32), torch.zeros(E + 2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    qmm.quantize_mxfp4(x, xq, T, n)
+    qmm.dequant_mxfp4(xq, x, T, n)
+    qmm.gemv_mxfp4(W[0], xq, e(T, 32), T, 32, n)
+    qmm.gemm_mxfp4(W[0], xq, e(T, 32), T, 32, n)
+    qmm.moe_route_groups(e(T, E), ids, e(T, k), T, E, k)
+    qmm.gemv_moe_mxfp4(W, None, W.shape[1], ids, xq, e(T * k, 32), T, k, E, 32, n)
+    qmm.moe_gemm_mxfp4(W, None, W.shape[1], tiles, counts, E + 2, e(T * k, dt=torch.int32), xq, e(T * k, 32), 32, n)
+    qmm.postnorm_add_rmsnorm_bf16(x, e(T, n), w, w, e(T, n, dt=torch.bfloat16), T, n, 1e-6)
+    qmm.postnorm_add_rmsnorm_quant(x, e(T, n), w, w, e(T, n), qmm.XQ8Buf(T, n), T, n, 1e-6)
+    qmm.postnorm_add_rmsnorm_mxfp4(x, e(T, n), w, w, xq, T, n, 1e-6, gate=e(T, n), act="silu")
+    with pytest.raises(QmmError):
+        qmm.quantize_mxfp4(x, xq, 1, n)
