@@ -315,7 +315,7 @@ struct GemmCall { const uint8_t* W; qmm_xmx x; void* D; int dtype, M, N, K128; h
 template <class T, class F>
 int launch_tiles(const GemmCall& c, F f) {
     const int64_t mt = ((int64_t)c.M + T::kRows - 1) / T::kRows, nt = ((int64_t)c.N + T::kCols - 1) / T::kCols;
-    if (mt * nt > 0x7fffffff) return QMM_ERR_SHAPE;
+    if (!grid_fits((uint64_t)(mt * nt), T::kThreads)) return QMM_ERR_SHAPE;
     f(dim3((unsigned)(mt * nt)), (int)mt, vec16_out(c.D, c.dtype, c.N));
     QMM_LAUNCH_CHECK();
     return QMM_OK;
@@ -371,6 +371,7 @@ template <int QN>
 int launch_gemv(const void* W, qmm_xmx x, void* y, int dtype, int ncol, int N, int K128, hipStream_t s) {
     const int S = gemv_waves(mx_groups(K128));
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((ncol + 8 * QN - 1) / (8 * QN))), block(64 * S);
+    if (!grid_fits(grid.x, block.x)) return QMM_ERR_SHAPE;
     const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), kGemvWaveLds);
     if (dtype == QMM_BF16)
         hipLaunchKernelGGL((k_gemv_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, x, y, N, K128, ncol, vec_out(y, dtype, N));
@@ -385,6 +386,7 @@ int launch_gemv_moe(const void* W, const void* Wsh, size_t ebytes, const int* id
                     int K128, int xrow_te, hipStream_t s) {
     const int S = gemv_waves(mx_groups(K128));
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)(T * nslot)), block(64 * S);
+    if (!grid_fits(grid.x, block.x)) return QMM_ERR_SHAPE;
     const size_t lds = (size_t)S * std::max<size_t>(256 * sizeof(mx_v4f), kGemvWaveLds);
     if (dtype == QMM_BF16)
         hipLaunchKernelGGL((k_gemv_moe_mxfp4<QN, true>), grid, block, lds, s, (const uint8_t*)W, (const uint8_t*)Wsh, ebytes, ids, x, y, T * nslot, nslot,
@@ -401,7 +403,7 @@ int launch_moe_gemm(const void* W, const void* Wsh, size_t ebytes, const qmm_moe
     if (ebytes % 16 != 0 || misaligned(Wsh, 16) || misaligned(tiles, 4) || misaligned(counts, 4) || misaligned(rowtab, 4)) return QMM_ERR_ARG;
     if (max_tiles == 0 || b.rows == 0) return QMM_OK;
     const uint32_t nblocks = ((uint32_t)N + kMoeCols - 1) / kMoeCols;
-    if ((uint64_t)nblocks * max_tiles > 0x7fffffffu) return QMM_ERR_SHAPE;
+    if (!grid_fits((uint64_t)nblocks * max_tiles, 256)) return QMM_ERR_SHAPE;
     const int K128 = mx_steps(K);
     const dim3 grid(nblocks * (uint32_t)max_tiles);
     constexpr size_t lds = MxReg<kMoeRows / 32, kMoeNF>::kLds;

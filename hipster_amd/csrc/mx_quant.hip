@@ -203,7 +203,7 @@ int qmm_pack_mxfp4(qmm_xmx rows, void* W, int N, int K, void* stream) {
     const int K128 = mx_steps(K);
     const uint32_t groups = (uint32_t)mx_groups(K128);
     const uint64_t blocks = (uint64_t)((N + 15) / 16) * groups;
-    if (blocks > 0x7fffffffu) return QMM_ERR_SHAPE;
+    if (!grid_fits(blocks, 64)) return QMM_ERR_SHAPE;
     hipLaunchKernelGGL(k_pack_mxfp4, dim3((unsigned)blocks), dim3(64), 0, (hipStream_t)stream, rows.q, rows.e, (uint8_t*)W, N, K128, groups);
     QMM_LAUNCH_CHECK();
     return QMM_OK;

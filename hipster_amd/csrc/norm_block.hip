@@ -231,7 +231,10 @@ int nb_launch(const NbArgs& a, int T, hipStream_t s) {
     if (T == 0) return QMM_OK;
     const int len = OUT == kNbMx ? mx_steps(a.n) * 128 : a.n;      // values written per row
     const dim3 grid((unsigned)T);
-#define QMM_NB(NT, V, C) hipLaunchKernelGGL((k_norm_block<NT, V, C, OUT>), grid, dim3(NT), 0, s, a)
+#define QMM_NB(NT, V, C) do { \
+        if (!grid_fits((uint64_t)T, NT)) return QMM_ERR_SHAPE; \
+        hipLaunchKernelGGL((k_norm_block<NT, V, C, OUT>), grid, dim3(NT), 0, s, a); \
+    } while (0)
     if (a.n % 4 != 0) {
         if (len <= 4096) QMM_NB(1024, 1, 4);
         else QMM_NB(1024, 1, 16);

@@ -352,6 +352,9 @@ __device__ __forceinline__ qmm_bf16x8 q4_bf16x8_mix(uint32_t u0, uint32_t u1, ui
 
 }  // namespace qmm
 
+// whether a launch of `blocks` workgroups stays within the 2^32 - 1 threads and 2^31 - 1 workgroups that one may have
+inline bool grid_fits(uint64_t blocks, uint32_t threads) { return blocks <= 0x7fffffffu && blocks * threads <= 0xffffffffu; }
+
 // Host-side launch check shared by the C-ABI wrappers.
 #define QMM_LAUNCH_CHECK()                                                   \
     do {                                                                     \

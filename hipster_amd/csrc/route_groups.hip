@@ -320,6 +320,7 @@ extern "C" int qmm_moe_route_groups(const float* logits, int stride, const qmm_r
     // a single token: one wave; else four tokens a workgroup
     const int waves = T == 1 ? 1 : 4;
     const dim3 grid((unsigned)((T + waves - 1) / waves)), block(64 * waves);
+    if (!grid_fits(grid.x, block.x)) return QMM_ERR_SHAPE;
     const int per_wave = rg_lds_doubles(nexp, r.keep < r.groups);
     const size_t lds = (size_t)waves * per_wave * sizeof(double);
     hipStream_t s = (hipStream_t)stream;

@@ -410,7 +410,8 @@ int qmm_silu_mul_quant(const float* gate, const float* up, qmm_xq8 xq, int n, vo
 int qmm_silu_mul_bf16(const float* gate, const float* up, uint16_t* out, size_t n, void* stream);
 
 /* ---- MXFP4 decoder blocks (no reference counterpart) ---- */
-/* A call for no rows does nothing and needs no buffers of them (the pointers may be NULL, as an empty tensor's are). */
+/* A call for no rows does nothing and needs no buffers of them (the pointers may be NULL, as an empty tensor's are).  A
+ * call whose launch would have 2^32 threads or more is refused (QMM_ERR_SHAPE); only far more rows than a model has make one. */
 /* rows of x (dtype QMM_F32 or QMM_BF16, row stride ldx >= K values) -> MXFP4.  A block's scale is 2^E,
  * E = max(floor(log2 amax) - 2, -127); a code is x * 2^-E rounded to nearest, ties to even, saturating at 6.  A block
  * with a NaN or an infinity gets scale byte 255 (NaN).  Any K >= 1 up to 2^24 (values past K count as 0); x needs

@@ -136,3 +136,18 @@ def test_calls_for_no_rows():
              lambda t, n=64: L.qmm_postnorm_add_rmsnorm_mxfp4(None, None, 0, n, None, None, 1.0, None, D, no, t, n, 1e-6, None)]
     for i, call in enumerate(calls):
         assert call(0) == 0 and call(1) == NULL and call(0, 0) == SHAPE, i
+
+
+def test_launches_beyond_the_grid():
+    """More threads than a launch may have: refused before anything is launched."""
+    L, eb = _lib.lib(), 1 << 40
+    assert L.qmm_pack_mxfp4(X, D, (1 << 30) + 16, 32, None) == SHAPE                                  # 2^26 strips and one, a wave each
+    assert L.qmm_gemv_mxfp4(D, X, D, 0, 1, (1 << 28) + 32, 1 << 15, None) == SHAPE                    # 2^23 pairs of strips, eight waves each
+    assert L.qmm_gemv_moe_mxfp4(D, None, eb, D, X, D, 0, 1, 1, 1, (1 << 28) + 32, 1 << 15, 0, None) == SHAPE
+    assert L.qmm_gemm_mxfp4(D, X, D, 0, 1 << 30, 1 << 20, 32, None) == SHAPE
+    assert L.qmm_moe_gemm_mxfp4_n(D, None, eb, 1, D, D, 1 << 24, None, 1, X, 1, D, 0, 129, 32, None) == SHAPE
+    big = ((1 << 24) + 1, (1 << 23) + 1, (1 << 22) + 1)
+    for T, n in zip(big, (128, 5632, 8320)):
+        assert L.qmm_postnorm_add_rmsnorm_bf16(D, D, 0, n, None, None, 1.0, D, D, D, T, n, 1e-6, None) == SHAPE
+    r = _lib.RouteRule(None, 1.0, 0, 1, 1, 1, 1, 0)
+    assert L.qmm_moe_route_groups(D, 8, ctypes.byref(r), D, D, (1 << 26) + 4, 8, 2, None) == SHAPE
