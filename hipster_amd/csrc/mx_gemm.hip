@@ -269,8 +269,8 @@ __device__ __forceinline__ void moe_rows(uint8_t* smem, const uint8_t* We, qmm_x
     mx_v16f acc[kMoeNF][MF];
     mx_tile_reg<MF, kMoeNF, kMoeD, false>(smem, We, x, n0 / 16, (N + 15) / 16, K128, [&](int r) {
         const int k = k0 + min(r, n - 1);
-        return rowtab ? min(max(rowtab[k], 0), xrows - 1) : k;
-    }, acc);
+        return rowtab ? rowtab[k] : k;
+    }, acc, [&](int row) { return min(max(row, 0), xrows - 1); });
     mx_store<MF, kMoeNF, BF>(smem, acc, D, n0 + 32 * kMoeNF * (int)(threadIdx.x >> 6), N, vec, [&](int r) { return r < n ? (int64_t)(k0 + r) : -1; });
 }
 

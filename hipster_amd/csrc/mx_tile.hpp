@@ -74,9 +74,13 @@ struct MxReg {
     static constexpr int kLds = 3 * kStage > kStoreLds ? 3 * kStage : kStoreLds;
 };
 
-// rows(r): the activation row of tile row r.  acc[f][j]: weight rows 32 f.., activation rows 32 j.. of this wave
-template <int MF, int NF, int D, bool AGPR, class Rows>
-__device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm_xmx x, int strip0, int nstrips, int K128, Rows rows, mx_v16f (&acc)[NF][MF]) {
+struct AsItIs { __device__ int operator()(int r) const { return r; } };
+
+// fit(rows(r)): the activation row of tile row r (rows may load from a table: all of them first, then what fit does with them,
+// or each load would be waited for by itself).  acc[f][j]: weight rows 32 f.., activation rows 32 j.. of this wave
+template <int MF, int NF, int D, bool AGPR, class Rows, class Fit = AsItIs>
+__device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm_xmx x, int strip0, int nstrips, int K128, Rows rows, mx_v16f (&acc)[NF][MF],
+                                            Fit fit = Fit{}) {
     using T = MxReg<MF, NF>;
     static_assert(D == 4 || D == 8, "the ring of weights turns with the groups of four steps");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -108,16 +112,21 @@ __device__ __forceinline__ void mx_tile_reg(uint8_t* smem, const uint8_t* W, qmm
     // and of row 128 + tid / 2 where the tile has more than 128
     const int cj = tid & 7;
     const uint8_t* qp[MF];
+    int qr[MF];
 #pragma unroll
-    for (int i = 0; i < MF; ++i) qp[i] = x.q + (size_t)rows((tid >> 3) + 32 * i) * K128 * 64 + (cj & 3) * 16;
+    for (int i = 0; i < MF; ++i) qr[i] = rows((tid >> 3) + 32 * i);
     constexpr int NE = (2 * T::kRows + 255) / 256;
-    int es[NE];
+    int es[NE], er[NE];
     const uint8_t* ep[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
         es[i] = min(tid + 256 * i, 2 * T::kRows - 1);    // beyond: the last one again
-        ep[i] = x.e + (size_t)rows(es[i] >> 1) * K128 * 4;
+        er[i] = rows(es[i] >> 1);
     }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) qp[i] = x.q + (size_t)fit(qr[i]) * K128 * 64 + (cj & 3) * 16;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) ep[i] = x.e + (size_t)fit(er[i]) * K128 * 4;
     constexpr int NP = D / 2;                            // pairs in flight
     uint4 pa[NP][MF];
     uint32_t pe[NP][NE];
