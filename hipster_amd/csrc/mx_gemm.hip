@@ -124,8 +124,8 @@ __device__ __forceinline__ void gemv_run(uint8_t* lds, const uint8_t* strip, uin
         for (int g = g0; g < g1 - 1; ++g) {
             *(uint4*)es = make_uint4(sc.a[0], sc.a[1], sc.a[2], sc.a[3]);
             const Scales now = sc;
-            load_s(sc, g + 1);
             mul(r0, now, std::integral_constant<int, 0>{}, 2);
+            load_s(sc, g + 1);
             load(r0, 2 * g + 2);
             mul(r1, now, std::integral_constant<int, 1>{}, 2);
             load(r1, 2 * g + 3);
