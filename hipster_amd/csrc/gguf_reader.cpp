@@ -46,7 +46,7 @@ namespace {
 // ---------------------------------------------------------------------------------- block shapes
 // elements and bytes per block, indexed by ggml type number; {0, 0} = a type this library does not size
 struct BlockShape { uint16_t elems, bytes; };
-constexpr int kMaxGType = 31;
+constexpr int kMaxGType = 40;
 constexpr BlockShape kBlockShape[kMaxGType] = {
     /* 0 F32    */ {1, 4},    /* 1 F16   */ {1, 2},    /* 2 Q4_0  */ {32, 18},   /* 3 Q4_1   */ {32, 20},
     /* 4        */ {0, 0},    /* 5       */ {0, 0},    /* 6 Q5_0  */ {32, 22},   /* 7 Q5_1   */ {32, 24},
@@ -55,7 +55,8 @@ constexpr BlockShape kBlockShape[kMaxGType] = {
     /* 16..19   */ {0, 0}, {0, 0}, {0, 0}, {0, 0},
     /* 20 IQ4_NL*/ {32, 18},  /* 21 IQ3_S*/ {256, 110},/* 22      */ {0, 0},     /* 23 IQ4_XS*/ {256, 136},
     /* 24 I8    */ {1, 1},    /* 25      */ {0, 0},    /* 26 I32  */ {1, 4},     /* 27..29   */ {0, 0}, {0, 0}, {0, 0},
-    /* 30 BF16  */ {1, 2},
+    /* 30 BF16  */ {1, 2},    /* 31..38   */ {0, 0}, {0, 0}, {0, 0}, {0, 0}, {0, 0}, {0, 0}, {0, 0}, {0, 0},
+    /* 39 MXFP4 */ {32, 17},
 };
 
 BlockShape block_shape(uint32_t t) { return t < (uint32_t)kMaxGType ? kBlockShape[t] : BlockShape{0, 0}; }

@@ -18,7 +18,7 @@ from ._lib import GgufTensor, QmmError, check
 
 # ggml tensor types (the reference's GType numbering, gguf.h:12-17)
 GType = type("GType", (), dict(F32=0, F16=1, Q4_0=2, Q4_1=3, Q5_0=6, Q5_1=7, Q8_0=8, Q8_1=9, Q2_K=10, Q3_K=11, Q4_K=12,
-                               Q5_K=13, Q6_K=14, Q8_K=15, IQ4_NL=20, IQ3_S=21, IQ4_XS=23, I8=24, I32=26, BF16=30))
+                               Q5_K=13, Q6_K=14, Q8_K=15, IQ4_NL=20, IQ3_S=21, IQ4_XS=23, I8=24, I32=26, BF16=30, MXFP4=39))
 KV_UINT, KV_INT, KV_FLOAT, KV_BOOL, KV_STRING, KV_ARRAY = range(6)
 
 

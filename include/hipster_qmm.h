@@ -100,12 +100,12 @@ typedef struct {
 typedef struct { const void* g; size_t ld; int32_t dtype, act, per_value; } qmm_gate;
 
 /* ---- GGUF (the on-disk format of the weights; reference: engine/src/gguf.h, gguf.cpp) ---- */
-/* ggml tensor types (the reference's GType numbering, gguf.h:12-17) */
+/* ggml tensor types (the reference's GType numbering, gguf.h:12-17; MXFP4, which it does not read, is ggml's) */
 enum {
     QMM_GGML_F32 = 0, QMM_GGML_F16 = 1, QMM_GGML_Q4_0 = 2, QMM_GGML_Q4_1 = 3, QMM_GGML_Q5_0 = 6, QMM_GGML_Q5_1 = 7,
     QMM_GGML_Q8_0 = 8, QMM_GGML_Q8_1 = 9, QMM_GGML_Q2_K = 10, QMM_GGML_Q3_K = 11, QMM_GGML_Q4_K = 12, QMM_GGML_Q5_K = 13,
     QMM_GGML_Q6_K = 14, QMM_GGML_Q8_K = 15, QMM_GGML_IQ4_NL = 20, QMM_GGML_IQ3_S = 21, QMM_GGML_IQ4_XS = 23,
-    QMM_GGML_I8 = 24, QMM_GGML_I32 = 26, QMM_GGML_BF16 = 30
+    QMM_GGML_I8 = 24, QMM_GGML_I32 = 26, QMM_GGML_BF16 = 30, QMM_GGML_MXFP4 = 39
 };
 /* kinds of KV values (the reference's GValue kinds, gguf.h:37-41: every integer width collapses to one
  * signed and one unsigned kind, f32/f64 to FLOAT) */
@@ -142,7 +142,8 @@ int qmm_gguf_kv_array_len(const qmm_gguf* g, const char* key, uint64_t* out);
 int qmm_gguf_read_tensor(const qmm_gguf* g, const char* name, void* dst, size_t dst_bytes);
 /* the layout the kernels read for a GGUF weight type, and its row bytes (reference: to_lin,
  * qwen4exp.cpp:34-65): Q4_K, Q5_K, IQ4_XS as stored; Q6_K -> QMM_Q6_K_SOA; Q8_0 -> QMM_Q8_0_SOA;
- * Q5_1 and Q5_0 -> QMM_Q5_1_SOA; F32, F16, BF16 -> QMM_Q8_0_SOA (requantised); others QMM_ERR_FORMAT */
+ * Q5_1 and Q5_0 -> QMM_Q5_1_SOA; F32, F16, BF16 -> QMM_Q8_0_SOA (requantised); others QMM_ERR_FORMAT (MXFP4 weights
+ * go through qmm_repack_row_mxfp4 and qmm_pack_mxfp4) */
 int qmm_weight_format(int gtype, int K, int* wfmt, size_t* row_bytes);
 /* N rows of K weights of GGUF type gtype -> that layout in dst (N * row_bytes bytes): a copy, the row
  * repacks above, or for F32/F16/BF16 the reference's quantize_row_q8_0_soa (quant.h:174-183: d =

@@ -2,10 +2,13 @@
 mirror on stand-ins for device tensors.  No call below reaches a device."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
-from hipster_amd import _lib, qmm
+import mx_ref
+from gguf_writer import STR, write_gguf
+from hipster_amd import _lib, gguf, qmm
 from hipster_amd._lib import QmmError, XMX
 
 FORMAT, SHAPE, NULL, ARG = -1, -2, -3, -6
@@ -151,3 +154,34 @@ def test_launches_beyond_the_grid():
         assert L.qmm_postnorm_add_rmsnorm_bf16(D, D, 0, n, None, None, 1.0, D, D, D, T, n, 1e-6, None) == SHAPE
     r = _lib.RouteRule(None, 1.0, 0, 1, 1, 1, 1, 0)
     assert L.qmm_moe_route_groups(D, 8, ctypes.byref(r), D, D, (1 << 26) + 4, 8, 2, None) == SHAPE
+
+
+def test_weights_of_a_model_file(tmp_path):
+    """A file with MXFP4 tensors opens (ggml type 39, 17 bytes a block), and its rows go to the rows that are packed."""
+    E, N, K = 2, 3, 160
+    blocks = np.random.default_rng(1).integers(0, 255, (E * N, K // 32, 17), dtype=np.uint8)
+    path = str(tmp_path / "m.gguf")
+    write_gguf(path, [("a", 0, (8,), np.arange(8, dtype=np.float32)), ("w", gguf.GType.MXFP4, (K, N, E), blocks), ("b", 0, (4,), np.ones(4, np.float32))],
+               {"general.architecture": (STR, "x")})
+    assert gguf.gtype_block(gguf.GType.MXFP4) == (32, 17) and gguf.gtype_row_bytes(gguf.GType.MXFP4, K) == K // 32 * 17
+    with gguf.GGUF(path) as g:
+        assert g.get("b").array().view(np.float32).tolist() == [1.0] * 4
+        t = g.get("w")
+        assert t.type == 39 and t.ne == (K, N, E, 1) and t.nbytes == blocks.size
+        for raw in (t.array(), g.read_tensor(t)):
+            for row, want in zip(raw.reshape(E * N, -1), blocks):
+                q, e = qmm.repack_row_mxfp4(row, K)
+                code = np.stack([q & 15, q >> 4], 1).reshape(1, -1)
+                byte = np.zeros((1, 8), np.uint8)
+                byte[0, :K // 32] = want[:, 0]
+                assert np.array_equal(e, byte[0])
+                # ggml: weight i of a block is the low half of byte i, weight i + 16 the high half, times 2^(byte - 127)
+                level = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6])
+                vals = level[np.concatenate([want[:, 1:] & 15, want[:, 1:] >> 4], 1)] * np.exp2(want[:, :1].astype(np.float64) - 127)
+                assert np.array_equal(mx_ref.values(code, byte)[0, :K], vals.reshape(-1))
+        with pytest.raises(QmmError, match="QMM_ERR_FORMAT"):           # no layout of the q8 products
+            gguf.upload_lin(g, "w", device="cpu")
+    for other in (31, 38, 40):
+        write_gguf(path, [("t", other, (32,), np.zeros(32, np.uint8))])
+        with pytest.raises(QmmError, match="QMM_ERR_FORMAT"):
+            gguf.GGUF(path)
