@@ -13,9 +13,11 @@
 //
 // The strip is in the order of the scaled matrix instructions: a lane supplies 32 codes of one row, a block, and the
 // block's scale in one byte of a register (which byte, the instruction says).  So a wave reads half a step of two
-// strips as two runs of 512 bytes and four steps' scales as one dword per lane, with no shuffle.  The instruction's sum of 128 products is exact to f32 rounding for fp4 operands
-// (measured: within 1.3 * 2^-24 of the sum of magnitudes with block scales spread over 2^+-40); fp8 operands
-// are not (products 2^15 below a group's largest are dropped), which is why activations are fp4 too.
+// strips as two runs of 512 bytes and four steps' scales as one dword per lane, with no shuffle.
+//
+// The instruction's sum of products is exact to f32 rounding for fp4 operands (measured: within 1.3 * 2^-24 of the sum of
+// magnitudes with block scales spread over 2^+-40); for fp8 operands it is not (products 2^15 below a group's largest
+// are dropped), which is why activations are fp4 too.
 #pragma once
 #include "qmm_common.hpp"
 

@@ -27,10 +27,11 @@ namespace {
 // the operand registers, by kilobytes, two steps (a pair) at a time, the next pair in flight while one is multiplied.
 // The activation rows beside them come as whole 128-byte lines (a pair of a row, eight lanes) and turn into operands in
 // LDS that is the wave's own: loaded in operand order, 16 bytes of 32 rows at a time, four loads touch each line, and the
-// vector cache holds every load up whose line is still on its way (24 rows x 5120 x 17408: 30 us that way, 15.2 so).
-// More than 32 rows are passes of 32, side by side: the weights of the second mostly come from caches (64 rows x 17408 x
-// 5120: 22 us; both fragments in one pass 80, 16 us up to 32 rows).  1 row x 17408 x 5120, weights from memory: 12 us,
-// 3.9 TB/s.
+// vector cache holds every load up whose line is still on its way (24 rows x 5120 x 17408 took twice the time).
+// More than 32 rows are passes of 32, side by side: the weights of the second mostly come from caches (both fragments in one
+// pass took 80 us at 64 rows x 17408 x 5120, for a cause not found).  With weights from memory / from the last-level cache: 1 row x
+// 17408 x 5120 13.5 / 10.4 us (3.5 / 4.6 TB/s), 33 rows 22 / 20, 64 rows 25 / 22; 24 rows x 5120 x 17408 18 / 12.5, whose 160
+// workgroups leave CUs idle.
 constexpr int kGemvMaxWaves = 8, kGemvMaxRows = 64;
 
 // S for G groups: one wave a group up to 8, else the count of 4 .. 8 that leaves the least imbalance
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(512, 2) k_gemm_mxfp4_dma(const uint8_t* __rest
 
 // Grouped: workgroup (tile of one expert's rows, block of 128 outputs); a tile's rows 128 at a time, with as
 // many 32-row fragments as they need.  512 experts of 1024 x 2048, 10 a token and a shared one: 512 tokens 109 us, 2048
-// 125, 8192 248; 64 rows at a time 335 at 8192 (weights are read again).  The 571 MB of weights take 110 at a large
+// 127, 8192 248; 64 rows at a time 335 at 8192 (weights are read again).  The 571 MB of weights take 110 at a large
 // copy's rate, and bound it up to 2048 tokens; beyond, the steps of the tiles do.  Weights three steps ahead: seven take
 // 5 % more at 2048, a third workgroup on a CU (of 168 registers a wave) 12 %.
 constexpr int kMoeNF = 1, kMoeD = 4, kMoeCols = 128 * kMoeNF, kMoeRows = 128;

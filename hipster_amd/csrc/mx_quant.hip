@@ -12,7 +12,7 @@
 //
 // All three move each byte once and are bound by HBM: a thread takes one 16-byte load of input (4 f32 or
 // 8 bf16), 8 or 4 neighbouring lanes make a block and find amax by DPP.  2048 x 17408 bf16 (90 MB, 17 us at a
-// large copy's rate): quantisation 26 us from memory, 16 from caches; the values back as bf16 16.
+// large copy's rate): quantisation 23 us from memory, 16 from caches; the values back as bf16 16.
 #include "mx.hpp"
 
 namespace qmm {

@@ -11,16 +11,16 @@
 //                 which the waves share, come two steps at a time (a pair: 128 bytes of a row, whole cache lines),
 //                 D steps ahead in registers, then through LDS: three buffers, so that one barrier a pair
 //                 suffices.  LDS reads run two 32-row fragments ahead of their products, across steps.
-//                 65 rows x 5120 x 5120: 10.8 us (29 for the other core's best tile); 300 x 17408 x 5120: 26, of which
-//                 launch, first loads, products and outputs take 18; it is bound by what a CU fetches past its L1, at
-//                 most 50 KB/us from HBM (a plain read by 8 to 80 workgroups, however much is in flight), where a tile
-//                 of 128 x 256 needs 960 KB (with weights that hit the L1: 22 us).
+//                 65 rows x 5120 x 5120: 10.8 us (29 for the other core's best tile); 300 x 17408 x 5120: 26 with weights
+//                 from memory, 23.5 from the last-level cache.  Taken apart when it took 28.5: 23.9 with weights that hit the L1,
+//                 20.7 without LDS reads too, 19.7 without LDS writes, 17.7 with products, launch and outputs alone: 204 tiles
+//                 of 128 x 256 on 256 CUs, 384 rows multiplied for 300, one wave a SIMD.
 //   mx_tile_dma   64 MF x 128 NF outputs, eight waves, for many rows.  Both operands by DMA (global_load_lds):
 //                 activations by pairs into two buffers, weights step by step into a ring of NS, scales by groups of
 //                 four steps.  The waves run as two halves (the rows' halves, one wave of each on every SIMD) half a step
 //                 apart: while one half reads its operands from LDS and starts its DMAs, the other multiplies, and a
-//                 barrier ends each phase.  2048 x 17408 x 5120, a new weight each call: 104 us (3.5 PFLOP/s) against 129
-//                 for the best tile of mx_tile_reg; without its DMAs it takes 71, without products and LDS reads 72.
+//                 barrier ends each phase.  2048 x 17408 x 5120, a new weight each call: 101 to 105 us (3.5 PFLOP/s) against
+//                 129 for the best tile of mx_tile_reg; without its DMAs it takes 71, without products and LDS reads 72.
 //
 // LDS holds an activation row's 16-byte chunk c at chunk c ^ a_swz(row): reads of 16 rows' chunk are free of bank
 // conflicts for any row alignment of 32.

@@ -12,8 +12,8 @@
 // order: per thread, by halves of the wave, wave by wave.  Threads and V go by n alone, so a row's bits depend on
 // nothing but the row, whatever the alignment of its arrays and their strides.
 //
-// 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 29 from caches; one row 6.6, one
-// after another.  Rows that start anywhere and lie an odd number of values apart: the same.
+// 2048 x 5120 with a bf16 gate per value: 37 us (28 for its 147 MB at a large copy's rate), 30 from caches, 45 with f32 and q8
+// out; one row 6.6, one after another (4.3 with one gate).  Rows that start anywhere and lie an odd number of values apart: the same.
 //
 // Threads go by the row's length alone, since they set the order of its sums; pieces are as few as cover it (2048 rows, us):
 //   256 threads up to five pieces: 5120 values 37.5 (512 threads with three: 41.3); with a sixth a wave has more
