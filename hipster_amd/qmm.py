@@ -612,9 +612,9 @@ def postnorm_add_rmsnorm_quant(x, y, wy, w, xn, xq, T, n, eps, gate=None, act="n
     a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
     if xq.ncol < T or xq.K != n:
         raise QmmError(f"xq holds {xq.ncol} rows of {xq.K} values, {T} of {n} are needed")
-    for t, dt in ((xq.q, torch.int8), (xq.d, torch.float32), (xq.s, torch.float32), (xq.ds, torch.float32)):
-        if t is not None:
-            _in(t, 0, "xq", dt)
+    dev = _device()
+    if xq.q.get_device() != dev or xq.d.get_device() != dev or xq.s.get_device() != dev or (xq.ds is not None and xq.ds.get_device() != dev):
+        raise QmmError(f"xq is on {xq.q.device}, the current device is cuda:{dev}")
     check(_lib.lib().qmm_postnorm_add_rmsnorm_quant(*a, _in(xn, T * n, "xn", torch.float32), xq.c(), T, n, eps, _handle(stream)),
           "postnorm_add_rmsnorm_quant")
 
