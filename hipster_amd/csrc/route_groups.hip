@@ -14,10 +14,10 @@
 // the experts' order, a lane each, and their rank among them is their slot.  More than 64 (many equal scores) are taken
 // one at a time.
 //
-// 4096 tokens of 256 experts (8 groups, 4 kept, 8 chosen, sigmoid): 9.2 us (replayed), 512 of them 5.9; a single token of 512
-// (10 chosen, softmax) 5.0, 64 tokens 6.3; with a step per chosen expert, the library's exp and a branch around each 12.5 and 7.8.  The 4 MB of logits
-// would take 0.8: it is bound by its instructions (of a wave some 650 vector ones, four waves a SIMD) and, at a
-// few tokens, by their latency.
+// 4096 tokens of 256 experts (8 groups, 4 kept, 8 chosen, sigmoid): 9.2 us (replayed), 512 of them 5.9; a single token of
+// 512 (10 chosen, softmax) 5.0, 64 tokens 6.3; with a step per chosen expert, the library's exp and a branch around each 12.5
+// for the first and 7.8 for the single token.  The 4 MB of logits would take 0.8: it is bound by its instructions (of a wave some
+// 650 vector ones, four waves a SIMD) and, at a few tokens, by their latency.
 
 #include "qmm_common.hpp"
 
@@ -81,9 +81,10 @@ __device__ __forceinline__ float wave_fmax(float v) {
     const uint32_t k = wave_umax(order_key32(v));
     return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
-// exp in 64 bits: x = n ln 2 + r (ln 2 in two parts, the ones that fdlibm's e_exp.c gives), the Taylor series of e^r to r^13 (|r| <= 0.347: the next term is
-// 4e-18 of the sum) and a scaling by 2^n.  The products are written out: with the constant as the addend in scalar
-// registers a term is one instruction, where the library's exp moves each constant first.
+// exp in 64 bits: x = n ln 2 + r, the Taylor series of e^r to r^13 (|r| <= 0.347: the next term is 4e-18 of the sum) and a
+// scaling by 2^n.  ln 2 is its nearest double and what is left of it: an fma rounds x - n ln 2 only once, however long
+// n ln 2 is.  The products are written out: with the constant as the addend in scalar registers a term is one instruction,
+// where the library's exp moves each constant first.
 __device__ __forceinline__ double fma_c(double a, double b, double c) {
     double d;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
@@ -92,7 +93,7 @@ __device__ __forceinline__ double fma_c(double a, double b, double c) {
 __device__ __forceinline__ double exp64(double x) {
     x = fmin(fmax(x, -800.0), 800.0);                    // 0 and inf from there on; a NaN becomes -800: the callers keep theirs out
     const double n = __builtin_rint(x * 1.4426950408889634);
-    const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, x));
+    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));
     double p = 1.0 / 6227020800.0;
     p = fma_c(p, r, 1.0 / 479001600.0);
     p = fma_c(p, r, 1.0 / 39916800.0);
