@@ -235,18 +235,25 @@ int nb_launch(const NbArgs& a, int T, hipStream_t s) {
         if (!grid_fits((uint64_t)T, NT)) return QMM_ERR_SHAPE; \
         hipLaunchKernelGGL((k_norm_block<NT, V, C, OUT>), grid, dim3(NT), 0, s, a); \
     } while (0)
+    const auto pieces = [&](int threads) { return (len + 4 * threads - 1) / (4 * threads); };
     if (a.n % 4 != 0) {
         if (len <= 4096) QMM_NB(1024, 1, 4);
         else QMM_NB(1024, 1, 16);
-    } else if (len <= 1024) QMM_NB(256, 4, 1);
-    else if (len <= 2048) QMM_NB(256, 4, 2);
-    else if (len <= 3072) QMM_NB(256, 4, 3);
-    else if (len <= 4096) QMM_NB(256, 4, 4);
-    else if (len <= 5120) QMM_NB(256, 4, 5);
-    else if (len <= 6144) QMM_NB(512, 4, 3);
-    else if (len <= 8192) QMM_NB(512, 4, 4);
-    else if (len <= 12288) QMM_NB(1024, 4, 3);
-    else QMM_NB(1024, 4, 4);
+    } else if (len <= 5120) {
+        switch (pieces(256)) {
+            case 1: QMM_NB(256, 4, 1); break;
+            case 2: QMM_NB(256, 4, 2); break;
+            case 3: QMM_NB(256, 4, 3); break;
+            case 4: QMM_NB(256, 4, 4); break;
+            default: QMM_NB(256, 4, 5);
+        }
+    } else if (len <= 8192) {
+        if (pieces(512) <= 3) QMM_NB(512, 4, 3);
+        else QMM_NB(512, 4, 4);
+    } else {
+        if (pieces(1024) <= 3) QMM_NB(1024, 4, 3);
+        else QMM_NB(1024, 4, 4);
+    }
 #undef QMM_NB
     QMM_LAUNCH_CHECK();
     return QMM_OK;
