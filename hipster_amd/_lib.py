@@ -17,6 +17,7 @@ QMM_Q4_K, QMM_Q5_K, QMM_IQ4_XS, QMM_Q6_K_SOA, QMM_Q8_0_SOA, QMM_Q5_1_SOA, QMM_Q6
 
 c_vp = ctypes.c_void_p
 c_int = ctypes.c_int
+c_sz = ctypes.c_size_t
 
 
 class XQ8(ctypes.Structure):
@@ -64,6 +65,28 @@ class RouteRule(ctypes.Structure):
 class Gate(ctypes.Structure):
     """qmm_gate: the gate of a block's output."""
     _fields_ = [("g", c_vp), ("ld", ctypes.c_size_t), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("per_value", ctypes.c_int32)]
+
+
+class KVMX(ctypes.Structure):
+    """qmm_kv_mxfp4: a paged cache of keys and values in MXFP4."""
+    _fields_ = [("kq", c_vp), ("ke", c_vp), ("vq", c_vp), ("ve", c_vp), ("pages", ctypes.c_int32), ("page", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class Seqs(ctypes.Structure):
+    """qmm_seqs: the sequences of a call."""
+    _fields_ = [("cu", c_vp), ("lens", c_vp), ("table", c_vp), ("n", ctypes.c_int32), ("ld", ctypes.c_int32)]
+
+
+class Attn(ctypes.Structure):
+    """qmm_attn: scale, window and sinks of attention."""
+    _fields_ = [("sinks", c_vp), ("scale", ctypes.c_float), ("window", ctypes.c_int32)]
+
+
+class Rope(ctypes.Structure):
+    """qmm_rope: rotary positions with several axes."""
+    _fields_ = [("freq", c_vp), ("axis", c_vp), ("pos", c_vp), ("ldp", ctypes.c_size_t), ("axes", ctypes.c_int32), ("pairs", ctypes.c_int32),
+                ("style", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 # element types (include/hipster_qmm.h)
@@ -152,6 +175,14 @@ SIGNATURES = {
     "qmm_postnorm_add_rmsnorm_bf16": (c_int, _POSTNORM + [c_vp, c_int, c_int, ctypes.c_float, c_vp]),
     "qmm_postnorm_add_rmsnorm_quant": (c_int, _POSTNORM + [c_vp, XQ8, c_int, c_int, ctypes.c_float, c_vp]),
     "qmm_postnorm_add_rmsnorm_mxfp4": (c_int, _POSTNORM + [XMX, c_int, c_int, ctypes.c_float, c_vp]),
+    "qmm_rope_axes": (c_int, [c_vp, c_int, c_sz, c_vp, c_int, c_sz, ctypes.POINTER(Rope), c_int, c_int, c_int, c_vp]),
+    "qmm_kv_write_mxfp4": (c_int, [c_vp, c_sz, c_vp, c_sz, c_int, ctypes.POINTER(KVMX), ctypes.POINTER(Seqs), c_int, c_vp]),
+    "qmm_kv_read_mxfp4": (c_int, [ctypes.POINTER(KVMX), ctypes.POINTER(Seqs), c_vp, c_sz, c_vp, c_sz, c_int, c_int, c_vp]),
+    "qmm_attn_kv_mxfp4": (c_int, [c_vp, c_int, c_sz, ctypes.POINTER(KVMX), ctypes.POINTER(Seqs), ctypes.POINTER(Attn), c_vp, c_int, c_sz,
+                                  c_int, c_int, c_int, c_int, c_vp, c_sz, c_vp]),
+    "qmm_attn_kv_ws_bytes": (c_sz, [c_int, c_int, c_int, c_int]),
+    "qmm_attn_prompt_bf16": (c_int, [c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp, c_vp, c_int, ctypes.POINTER(Attn), c_int, c_int,
+                                     c_int, c_int, c_int, c_vp]),
     "qmm_gemm_wq": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16_ld": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp]),

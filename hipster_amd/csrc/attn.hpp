@@ -1,0 +1,69 @@
+// attn.hpp -- what the kernels of attention share: a call's sequences, a paged MXFP4 cache, bf16 matrix instructions.
+#pragma once
+#include "mx.hpp"
+
+namespace qmm {
+
+typedef __bf16 at_bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 at_bf8 __attribute__((ext_vector_type(8)));
+typedef short at_s4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float neg_inf() { return __uint_as_float(0xff800000u); }
+
+// other lanes of the wave read what this one wrote to LDS (which the hardware does in order), or write what it read
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// The transposing LDS read of 16-bit values: in each 16 lanes, lane i supplies the address of four values, values 4 (i % 4) .. + 3 of
+// row i / 4, and gets value i of the four rows.
+__device__ __forceinline__ at_s4 tr_read(const void* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(const __attribute__((address_space(3))) at_s4*)p);
+}
+
+// ---- a call's sequences (qmm_seqs) ----
+// Offsets and lengths are device data.  Both ends of a span are brought into [0, rows] before they are subtracted (a difference of
+// arbitrary ints wraps round), so that whatever they hold, rows r0 .. r0 + m - 1 are rows; positions are checked by the callers.
+__host__ __device__ __forceinline__ int within(int v, int rows) { return v < 0 ? 0 : v > rows ? rows : v; }
+struct SeqSpan { int r0, m, len; };               // first row, rows, tokens
+
+__device__ __forceinline__ SeqSpan seq_span(const int* __restrict__ cu, const int* __restrict__ lens, int b, int rows) {
+    const int r0 = within(cu[b], rows), r1 = within(cu[b + 1], rows);
+    return {r0, max(r1 - r0, 0), max(lens[b], 0)};
+}
+
+// The sequence that row r (the same in all lanes) belongs to, -1: none.  The wave compares 64 offsets at a time, so that up to 64
+// sequences cost one load's latency.
+__device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, int n, int r) {
+    const int lane = threadIdx.x & 63;
+    int b = -1;
+    for (int base = 0; base < n; base += 64) {
+        const int at = base + lane;
+        const int c = at < n ? cu[at] : 0x7fffffff;
+        const int below = __popcll(__ballot(c <= r));
+        if (below) b = base + below - 1;
+        if (below < 64) break;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    return b >= 0 && r < cu[b + 1] && r >= cu[b] ? b : -1;
+}
+
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// what the entry points ask of a cache and of the sequences; *lg: log2 of the page
+inline int kv_check(const qmm_kv_mxfp4* kv, const qmm_seqs* s, int* lg) {
+    if (!kv || !s || !kv->kq || !kv->ke || !kv->vq || !kv->ve || !s->cu || !s->lens || !s->table) return QMM_ERR_NULL;
+    if (kv->dim != 64 && kv->dim != 128 && kv->dim != 256) return QMM_ERR_SHAPE;
+    if (kv->heads < 1 || kv->heads > 4096 || kv->pages < 1 || kv->page < 16 || kv->page > 4096 || (kv->page & (kv->page - 1))) return QMM_ERR_SHAPE;
+    if (s->n < 1 || s->ld < 1 || (int64_t)s->ld * kv->page > 0x7fffffff) return QMM_ERR_SHAPE;
+    if (!aligned(kv->kq, 16) || !aligned(kv->vq, 16) || !aligned(kv->ke, 8) || !aligned(kv->ve, 8)) return QMM_ERR_ARG;
+    if (!aligned(s->cu, 4) || !aligned(s->lens, 4) || !aligned(s->table, 4)) return QMM_ERR_ARG;
+    for (*lg = 4; 1 << *lg != kv->page;) ++*lg;
+    return QMM_OK;
+}
+inline int attn_check(const qmm_attn* a) {
+    if (!a) return QMM_ERR_NULL;
+    if (a->window < 0) return QMM_ERR_SHAPE;
+    return aligned(a->sinks, 4) ? QMM_OK : QMM_ERR_ARG;
+}
+
+}  // namespace qmm

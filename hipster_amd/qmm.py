@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import Gate, GemvSeg, MoeSegs, MoeTile, QmmError, RouteRule, XMX, XQ8, XQ8K, check  # noqa: F401
+from ._lib import KVMX, XMX, XQ8, XQ8K, Attn, Gate, GemvSeg, MoeSegs, MoeTile, QmmError, Rope, RouteRule, Seqs, check  # noqa: F401
 
 WFmt = type("WFmt", (), {"Q4_K": _lib.QMM_Q4_K, "Q5_K": _lib.QMM_Q5_K, "IQ4_XS": _lib.QMM_IQ4_XS,
                          "Q6_K_SOA": _lib.QMM_Q6_K_SOA, "Q8_0_SOA": _lib.QMM_Q8_0_SOA,
@@ -623,3 +623,129 @@ def postnorm_add_rmsnorm_mxfp4(x, y, wy, w, xq, T, n, eps, gate=None, act="none"
     """The same with rmsnorm(xo) * w as MXFP4 rows (XMXBuf of T x n)."""
     a = _postnorm(x, y, wy, w, gate, act, alpha, xo, T, n)
     check(_lib.lib().qmm_postnorm_add_rmsnorm_mxfp4(*a, _xmx(xq, T, n, "xq"), T, n, eps, _handle(stream)), "postnorm_add_rmsnorm_mxfp4")
+
+
+# ---- attention between a block's q, k, v products and its output product ----
+class KVMXBuf:
+    """A cache of keys and values in MXFP4, in pages of `page` tokens: kq, vq [pages][heads][page][dim / 2] uint8 (codes), ke, ve
+    [pages][heads][page][dim / 32] uint8 (scale bytes)."""
+
+    def __init__(self, pages, page, heads, dim, device="cuda"):
+        self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
+        self.kq, self.vq = (torch.zeros((pages, heads, page, dim // 2), dtype=torch.uint8, device=device) for _ in range(2))
+        self.ke, self.ve = (torch.zeros((pages, heads, page, dim // 32), dtype=torch.uint8, device=device) for _ in range(2))
+
+    def c(self):
+        return KVMX(self.kq.data_ptr(), self.ke.data_ptr(), self.vq.data_ptr(), self.ve.data_ptr(), self.pages, self.page, self.heads, self.dim)
+
+
+def _kv(kv):
+    n = kv.pages * kv.heads * kv.page
+    return KVMX(_in(kv.kq, n * (kv.dim // 2), "kv.kq", torch.uint8), _in(kv.ke, n * (kv.dim // 32), "kv.ke", torch.uint8),
+                _in(kv.vq, n * (kv.dim // 2), "kv.vq", torch.uint8), _in(kv.ve, n * (kv.dim // 32), "kv.ve", torch.uint8),
+                kv.pages, kv.page, kv.heads, kv.dim)
+
+
+def _seqs(cu, lens, table):
+    n = lens.numel()
+    if table.dim() != 2 or table.shape[0] < n:
+        raise QmmError(f"table must have a row of pages for each of {n} sequences, got shape {tuple(table.shape)}")
+    return Seqs(_in(cu, n + 1, "cu", torch.int32), _in(lens, n, "lens", torch.int32), _in(table, 0, "table", torch.int32), n, table.shape[1])
+
+
+def _heads(t, rows, heads, dim, name):
+    """The row stride of t, `rows` rows of heads * dim contiguous values: [rows][heads * dim] or [rows][heads][dim], or one such row."""
+    if t is not None and t.is_cuda and t.dim() == 3:
+        if t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+            raise QmmError(f"{name} must be rows of {heads} heads of {dim} contiguous values, got shape {tuple(t.shape)}, strides {tuple(t.stride())}")
+        if t.get_device() != _device():
+            raise QmmError(f"{name} is on {t.device}, the current device is cuda:{_device()}")
+        if t.shape[0] < rows:
+            raise QmmError(f"{name} has {t.shape[0]} rows, {rows} are needed")
+        ld = t.stride(0) if t.shape[0] > 1 else heads * dim
+        if ld < heads * dim:
+            raise QmmError(f"{name}: rows overlap (stride {ld}, {heads * dim} values)")
+        return ld
+    return _rows(t, rows, heads * dim, name)
+
+
+_STYLE = {"halves": 0, "neighbours": 1}
+
+
+def rope_axes(x, out, pos, freq, axis, rows, heads, dim, style="halves", scale=1.0, stream=None):
+    """Rotary positions with several axes: pair i of every head of row t of x turns by pos[axis[i]][t] * freq[i], times scale.
+
+    x, out: rows of heads * dim values, f32 or bf16 each (out may be x); pos int32 [axes][rows] or [rows]; freq f32 [pairs]; axis uint8
+    [pairs] or None (axis 0 for all); style "halves" (values i and i + pairs are a pair) or "neighbours" (2 i and 2 i + 1).  Values
+    from 2 pairs on are copied."""
+    if style not in _STYLE:
+        raise QmmError(f"style {style!r}: halves or neighbours")
+    pairs = freq.numel()
+    axes, ldp = (1, 0) if pos.dim() == 1 else (pos.shape[0], pos.shape[-1])
+    if pos.dim() > 2 or (pos.shape[-1] < rows):
+        raise QmmError(f"pos must be [axes][rows] or [rows] with {rows} rows, got shape {tuple(pos.shape)}")
+    ldx, ldo = _heads(x, rows, heads, dim, "x"), _heads(out, rows, heads, dim, "out")
+    r = Rope(_in(freq, pairs, "freq", torch.float32), None if axis is None else _in(axis, pairs, "axis", torch.uint8),
+             _in(pos, 0, "pos", torch.int32), ldp, axes, pairs, _STYLE[style], scale)
+    check(_lib.lib().qmm_rope_axes(x.data_ptr(), _dtype(x, "x"), ldx, out.data_ptr(), _dtype(out, "out"), ldo, r, rows, heads, dim, _handle(stream)),
+          "rope_axes")
+
+
+def _same(k, v, what):
+    if k.dtype is not v.dtype:
+        raise QmmError(f"{what} must be of one type, got {k.dtype} and {v.dtype}")
+    return _dtype(k, "k")
+
+
+def kv_write_mxfp4(k, v, kv, cu, lens, table, rows, stream=None):
+    """k, v (f32 or bf16, `rows` rows of the cache's heads * dim) -> their tokens' places in kv (KVMXBuf), as MXFP4.
+
+    Rows cu[b] .. cu[b + 1] - 1 are the last ones of sequence b, which has lens[b] tokens with them; table[b] are its pages (int32,
+    all on the device).  Rows from the last cu on, and tokens outside the table or the cache, are not written."""
+    ldk, ldv = _heads(k, rows, kv.heads, kv.dim, "k"), _heads(v, rows, kv.heads, kv.dim, "v")
+    check(_lib.lib().qmm_kv_write_mxfp4(k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), _kv(kv), _seqs(cu, lens, table), rows,
+                                        _handle(stream)), "kv_write_mxfp4")
+
+
+def kv_read_mxfp4(kv, cu, lens, table, k, v, rows, stream=None):
+    """The values that kv holds for the tokens of these rows (as kv_write_mxfp4 places them) -> k, v, f32 or bf16 (exact in both)."""
+    ldk, ldv = _heads(k, rows, kv.heads, kv.dim, "k"), _heads(v, rows, kv.heads, kv.dim, "v")
+    check(_lib.lib().qmm_kv_read_mxfp4(_kv(kv), _seqs(cu, lens, table), k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), rows,
+                                       _handle(stream)), "kv_read_mxfp4")
+
+
+def attn_kv_ws_bytes(rows, heads, dim, max_len):
+    """Bytes of attn_kv_mxfp4's workspace (0: it needs none)."""
+    return _lib.lib().qmm_attn_kv_ws_bytes(rows, heads, dim, max_len)
+
+
+def _attn(scale, dim, window, sinks, heads):
+    return Attn(None if sinks is None else _in(sinks, heads, "sinks", torch.float32), dim ** -0.5 if scale is None else scale, window)
+
+
+def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, ws, scale=None, window=0, sinks=None, stream=None):
+    """Attention of up to max_rows (<= 16) new rows a sequence over the cache kv, which holds their keys and values already.
+
+    q, out: `rows` rows of heads * kv.dim values, f32 or bf16 each; heads / kv.heads (<= 16) successive heads share one of the cache;
+    max_len: at least the longest of lens; ws: a uint8 tensor of attn_kv_ws_bytes(rows, heads, kv.dim, max_len) bytes (None where that
+    is 0); scale None: dim ** -0.5; window: keys a row sees with its own (0: all); sinks f32 [heads]: a logit beside the keys'."""
+    ldq, ldo = _heads(q, rows, heads, kv.dim, "q"), _heads(out, rows, heads, kv.dim, "out")
+    check(_lib.lib().qmm_attn_kv_mxfp4(q.data_ptr(), _dtype(q, "q"), ldq, _kv(kv), _seqs(cu, lens, table), _attn(scale, kv.dim, window, sinks, heads),
+                                       out.data_ptr(), _dtype(out, "out"), ldo, rows, heads, max_rows, max_len,
+                                       None if ws is None else _in(ws, 0, "ws", torch.uint8), 0 if ws is None else ws.numel(), _handle(stream)),
+          "attn_kv_mxfp4")
+
+
+def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None, window=0, sinks=None, stream=None):
+    """Causal attention of packed sequences: rows cu_q[b] .. cu_q[b + 1] - 1 of q, the last ones of the tokens cu_k[b] .. cu_k[b + 1] - 1
+    of k and v (cu_k None: cu_q).  q, out rows of heads * dim values, k, v of kv_heads * dim, all bf16 (row strides multiples of 8);
+    scale, window and sinks as in attn_kv_mxfp4."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        if t.dtype is not torch.bfloat16:
+            raise QmmError(f"{name} must be torch.bfloat16, got {t.dtype}")
+    rows, krows, n = q.shape[0], k.shape[0], cu_q.numel() - 1
+    ldq, ldo = _heads(q, rows, heads, dim, "q"), _heads(out, rows, heads, dim, "out")
+    ldk, ldv = _heads(k, krows, kv_heads, dim, "k"), _heads(v, krows, kv_heads, dim, "v")
+    check(_lib.lib().qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _in(cu_q, n + 1, "cu_q", torch.int32),
+                                          None if cu_k is None else _in(cu_k, n + 1, "cu_k", torch.int32), n, _attn(scale, dim, window, sinks, heads),
+                                          rows, krows, heads, kv_heads, dim, _handle(stream)), "attn_prompt_bf16")

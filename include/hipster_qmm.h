@@ -99,6 +99,21 @@ typedef struct {
  * 1: n values per token at g + t * ld (ld 0: the same n for every token) */
 typedef struct { const void* g; size_t ld; int32_t dtype, act, per_value; } qmm_gate;
 
+/* a cache of keys and values in MXFP4, in pages of `page` tokens (a power of two, 16 .. 4096): codes kq, vq [pages][heads][page][dim / 2]
+ * (value 2i in the low half of byte i), scale bytes ke, ve [pages][heads][page][dim / 32]; dim 64, 128 or 256.  kq and vq are
+ * 16-byte aligned, ke and ve 8-byte. */
+typedef struct { uint8_t* kq; uint8_t* ke; uint8_t* vq; uint8_t* ve; int32_t pages, page, heads, dim; } qmm_kv_mxfp4;
+/* the n sequences of a call, all on the device: rows cu[b] .. cu[b + 1] - 1 of the call's row tensors are the last ones of sequence b,
+ * which has lens[b] tokens with them: of m rows, row i is the token at position lens[b] - m + i.  Token p is in the cache at
+ * page table[b * ld + p / page], place p % page. */
+typedef struct { const int32_t* cu; const int32_t* lens; const int32_t* table; int32_t n, ld; } qmm_seqs;
+/* how far and how a row of attention sees: score = scale * q . k; keys of the positions (p - window, p] (window 0: all up to p); sinks
+ * [heads of q] f32 or NULL: a logit per head that takes part in the softmax and has no value */
+typedef struct { const float* sinks; float scale; int32_t window; } qmm_attn;
+/* rotary positions: pair i < pairs of a head turns by pos[axis[i] * ldp + t] * freq[i] (pos int32 [axes][ldp], axis NULL: axis 0 for all);
+ * style 0: values i and i + pairs are a pair, 1: values 2i and 2i + 1.  Turned values are multiplied by scale. */
+typedef struct { const float* freq; const uint8_t* axis; const int32_t* pos; size_t ldp; int32_t axes, pairs, style; float scale; } qmm_rope;
+
 /* ---- GGUF (the on-disk format of the weights; reference: engine/src/gguf.h, gguf.cpp) ---- */
 /* ggml tensor types (the reference's GType numbering, gguf.h:12-17; MXFP4, which it does not read, is ggml's) */
 enum {
@@ -472,6 +487,44 @@ int qmm_postnorm_add_rmsnorm_quant(const float* x, const void* y, int y_dtype, s
 /* ... or as MXFP4 rows, the codes that qmm_quantize_mxfp4 gives for the f32 xn (any n) */
 int qmm_postnorm_add_rmsnorm_mxfp4(const float* x, const void* y, int y_dtype, size_t ldy, const float* wy, const qmm_gate* gate, float alpha,
                                    float* xo, const float* w, qmm_xmx xq, int T, int n, float eps, void* stream);
+
+/* ---- attention between a block's q, k, v products and its output product (no reference counterpart) ---- */
+/* What lies on the device is not seen by a host check, so the kernels keep inside the buffers whatever it holds: rows from cu[n] on
+ * belong to no sequence and are left as they were; rows at negative positions (lens[b] below the rows given) are not written, and as
+ * queries see nothing; positions from ld * page on are not written and not seen; a page number outside the cache is not written, and
+ * makes what reads it NaN.  Two sequences that share a page may read it at once, but may not write it in one call.
+ * A call for no rows does nothing and needs no buffers. */
+/* x [rows][heads][dim] (row stride ldx values, a row's heads one after the other) -> out, f32 or bf16 each, out = x allowed where types
+ * and strides are the same.  dim <= 1024, 2 * pairs <= dim, axes <= 255, values from 2 * pairs on are copied.  The angle is exact
+ * before its reduction, whatever the position; its sine and cosine are within 2^-22. */
+int qmm_rope_axes(const void* x, int dtype, size_t ldx, void* out, int out_dtype, size_t ldo, const qmm_rope* rope, int rows, int heads, int dim,
+                  void* stream);
+/* k and v [rows][heads][dim] (f32 or bf16, row strides ldk, ldv) -> their sequences' places in the cache, the codes that
+ * qmm_quantize_mxfp4 gives */
+int qmm_kv_write_mxfp4(const void* k, size_t ldk, const void* v, size_t ldv, int dtype, const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, int rows,
+                       void* stream);
+/* the values that the cache holds for these rows' tokens -> k and v (f32 or bf16, exact in both; row strides ldk, ldv): what
+ * qmm_kv_write_mxfp4 was given, quantised.  cu of the whole sequences reads them whole. */
+int qmm_kv_read_mxfp4(const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, void* k, size_t ldk, void* v, size_t ldv, int dtype, int rows, void* stream);
+/* attention of up to 16 new rows a sequence over the cache (which holds their own keys and values): out[r][h] = sum_j w_j v_j / (sum_j w_j +
+ * exp(sink)), w_j = exp(scale q[r][h] . k_j), over the keys that row r sees; no key (or scores of -inf alone): 0.
+ * q (16-byte aligned, ldq a multiple of 16 bytes) and out [rows][heads][dim], f32 or bf16 each, row
+ * strides ldq, ldo; heads a multiple of the cache's, at most 16 times as many, successive heads sharing one.  max_rows (<= 16): the
+ * most rows of a sequence, later ones are left as they were; max_len (<= 2^30): at least the longest lens[b] (later keys are not seen).  ws:
+ * qmm_attn_kv_ws_bytes(...) bytes, 16-byte aligned; calls that overlap need one each, calls one after another may share it.
+ * A row's bits depend on q, its sequence, max_len and whether q or out is f32 (then the matrix products carry more bits): not
+ * on the other sequences or rows of the call. */
+int qmm_attn_kv_mxfp4(const void* q, int q_dtype, size_t ldq, const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, const qmm_attn* attn, void* out,
+                      int out_dtype, size_t ldo, int rows, int heads, int max_rows, int max_len, void* ws, size_t ws_bytes, void* stream);
+/* bytes of its workspace (0: nothing needed, or a size out of range) */
+size_t qmm_attn_kv_ws_bytes(int rows, int heads, int dim, int max_len);
+/* causal attention of packed sequences, bf16: q and out [rows][heads][dim], k and v [krows][kv_heads][dim] with row strides in values
+ * (multiples of 8, 16-byte aligned).  Sequence b has the q rows cuq[b] .. cuq[b + 1] - 1 and the keys cuk[b] .. cuk[b + 1] - 1
+ * (cuk NULL: cuq); of m rows and n keys, row i is at position n - m + i.  The formula of qmm_attn_kv_mxfp4; dim 64, 128 or 256; heads
+ * a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were. */
+int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
+                         const int32_t* cuq, const int32_t* cuk, int nseq, const qmm_attn* attn, int rows, int krows, int heads, int kv_heads, int dim,
+                         void* stream);
 
 #ifdef __cplusplus
 }
