@@ -21,10 +21,14 @@
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
 #include "attn.hpp"
 
+#include <algorithm>
+#include <cstdlib>
+
 namespace qmm {
 namespace {
 
-constexpr int kWaves = 4, kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kChunk = 256, kMaxLen = 1 << 30;
+constexpr int kWaves = 4, kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kChunk = 256, kMaxLen = 1 << 30, kNone = 0x7fff0000;
+constexpr float kSlack = 8.f;
 
 struct AttnArgs {
     const void* q;
@@ -37,6 +41,7 @@ struct AttnArgs {
     size_t ldq, ldo;
     float scale;                                         // times log2(e)
     int lg, window, rows, heads, share, max_rows, max_len, chunk, chunks, groups;   // groups: of 16 NT rows
+    int lgc;                                             // log2 of chunk
     int q_bf, out_bf;
 };
 
@@ -66,6 +71,70 @@ __device__ __forceinline__ float sum_xor32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The units of work, in order: sequence, kv head, group of 16 NT rows, chunk.  What a call has of them is known on the device alone;
+// each workgroup counts them and takes its share.  A unit's place: its sequence, that one's chunks (from `first` on) and groups, and
+// the unit's number in it (`units`); past the last unit: `units` is how many there are.  The wave adds up 64 sequences at a time.
+struct Place { int b, first, chunks, groups; uint32_t units; };
+struct Counts { int first, chunks, groups; uint32_t mine, upto; };           // a lane's sequence; upto: of the sequences to it
+
+template <int NT>
+__device__ __forceinline__ Counts count(const AttnArgs& a, int base) {
+    const int lane = threadIdx.x & 63;
+    Counts c = {0, 0, 0, 0, 0};
+    if (base + lane < a.s.n) {
+        const SeqSpan q = seq_span(a.s.cu, a.s.lens, base + lane, a.rows);
+        const int m = min(q.m, a.max_rows);
+        if (m > 0) {
+            const int lo = sight(a, q.len - q.m).lo, hi = sight(a, q.len - q.m + m - 1).hi;
+            c.first = a.chunks == 1 ? 0 : lo >> a.lgc;
+            c.chunks = a.chunks == 1 ? 1 : hi < lo ? 0 : (hi >> a.lgc) - c.first + 1;
+            c.groups = (m * a.share + 16 * NT - 1) / (16 * NT);
+        }
+    }
+    c.mine = c.upto = (uint32_t)(c.chunks * c.groups * a.kv.heads);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const uint32_t v = (uint32_t)__shfl_up((int)c.upto, k, 64);
+        if (lane >= k) c.upto += v;
+    }
+    return c;
+}
+// the place of a unit that lies in the 64 sequences counted in c, `before` units lying in front of them
+__device__ __forceinline__ bool pick(const Counts& c, int base, uint32_t before, uint32_t unit, Place& p) {
+    const unsigned long long behind = __ballot(before + c.upto > unit);
+    if (!behind) return false;
+    const int l = __builtin_ctzll(behind);
+    p = {base + l, __builtin_amdgcn_readlane(c.first, l), __builtin_amdgcn_readlane(c.chunks, l), __builtin_amdgcn_readlane(c.groups, l),
+         unit - before - (uint32_t)__builtin_amdgcn_readlane((int)(c.upto - c.mine), l)};
+    return true;
+}
+template <int NT>
+__device__ __forceinline__ Place locate(const AttnArgs& a, uint32_t unit) {
+    Place p = {-1, 0, 1, 1, 0};
+    for (int base = 0; base < a.s.n; base += 64) {
+        const Counts c = count<NT>(a, base);
+        if (pick(c, base, p.units, unit, p)) return p;
+        p.units += (uint32_t)__builtin_amdgcn_readlane((int)c.upto, 63);
+    }
+    return p;
+}
+// the workgroup's first unit and the one after its last, and the first one's place: as many as any other's, one more at most
+template <int NT>
+__device__ __forceinline__ Place share(const AttnArgs& a, uint32_t& unit, uint32_t& end) {
+    Place p = {-1, 0, 1, 1, 0};
+    const bool once = a.s.n <= 64;
+    Counts c;
+    if (once) c = count<NT>(a, 0);
+    const uint64_t total = once ? (uint32_t)__builtin_amdgcn_readlane((int)c.upto, 63) : locate<NT>(a, 0xffffffffu).units;
+    unit = (uint32_t)(total * blockIdx.x / gridDim.x);
+    end = (uint32_t)(total * (blockIdx.x + 1) / gridDim.x);
+    if (unit < end) {
+        if (once) pick(c, 0, 0, unit, p);
+        else p = locate<NT>(a, unit);
+    }
+    return p;
+}
+
 // 2^(x - m), 0 for x = -inf whatever m
 __device__ __forceinline__ float weight(float x, float m) { return __builtin_amdgcn_exp2f(x - (m == neg_inf() ? 0.f : m)); }
 
@@ -83,6 +152,28 @@ __device__ __forceinline__ float finish(float o, float l, float m, const float* 
 __device__ __forceinline__ void put(const AttnArgs& a, size_t at, float v) {
     if (a.out_bf) ((uint16_t*)a.out)[at] = (uint16_t)mx_bf16x2(v, 0.f);
     else ((float*)a.out)[at] = v;
+}
+
+// v, an f32, as three bf16 that add up to it: its leading 8 significant bits, the next 8 and the last 8 (dropping bits, not rounding,
+// keeps each rest exact and costs one instruction).  Not finite: the first alone.
+__device__ __forceinline__ void split3(const float (&v)[8], at_bf8 (&f)[3]) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t x[2][3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = __float_as_uint(v[2 * j + i]);
+            const float a = __uint_as_float(u & 0xffff0000u), r = v[2 * j + i] - a, b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+            x[i][0] = u;
+            x[i][1] = __float_as_uint(r);
+            x[i][2] = __float_as_uint(r - b);
+        }
+#pragma unroll
+        for (int t = 0; t < 3; ++t) w[t][j] = __builtin_amdgcn_perm(x[1][t], x[0][t], 0x07060302u);      // the upper halves
+    }
+#pragma unroll
+    for (int t = 0; t < 3; ++t) f[t] = __builtin_bit_cast(at_bf8, make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]));
 }
 
 __device__ __forceinline__ uint32_t fp4x2(uint32_t code, int byte, float s) {
@@ -104,37 +195,42 @@ template <int D>
 struct Tile {
     static constexpr int W = D / 32;                     // words of codes = matrix steps of 32 dims
     static constexpr int S = D == 256 ? 2 : 1;           // scales
-    uint32_t c[W];
+    static constexpr int V = W / S;                      // words of a load
+    typedef uint32_t Codes __attribute__((ext_vector_type(V)));
+    Codes c[S];
     uint32_t e[S];
-    __device__ __forceinline__ float scale(int w) const { return __uint_as_float(e[D == 256 ? w / 4 : 0] << 23); }
+    __device__ __forceinline__ uint32_t word(int w) const { return c[w / V][w % V]; }
+    __device__ __forceinline__ float scale(int w) const { return __uint_as_float(e[w / V] << 23); }
+    __device__ __forceinline__ void clear(int i) {       // to values of 0
+        c[i] = Codes(0);
+        e[i] = 127;
+    }
     // dim of the first of the eight values of word w, lane group kg
     static __device__ __forceinline__ int dim(int w, int kg) { return D == 64 ? kg * 16 + w * 8 : D == 128 ? kg * 32 + w * 8 : (w / 4) * 128 + kg * 32 + (w % 4) * 8; }
 
     __device__ __forceinline__ void load(const uint8_t* __restrict__ q, const uint8_t* __restrict__ se, size_t token, int kg) {
         const uint8_t* p = q + token * (D / 2);
         const uint8_t* s = se + token * (D / 32);
-        if constexpr (D == 64) {
-            const uint2 v = *(const uint2*)(p + kg * 8);
-            c[0] = v.x; c[1] = v.y;
-            e[0] = s[kg / 2];
-        } else {
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const uint4 v = *(const uint4*)(p + i * 64 + kg * 16);
-                c[4 * i] = v.x; c[4 * i + 1] = v.y; c[4 * i + 2] = v.z; c[4 * i + 3] = v.w;
-                e[i] = s[i * 4 + kg];
-            }
+        for (int i = 0; i < S; ++i) {
+            c[i] = *(const Codes*)(p + i * 64 + kg * (4 * V));
+            e[i] = s[D == 64 ? kg / 2 : i * 4 + kg];
         }
     }
 };
 
-template <int D>
-struct Step { Tile<D> k[2], v[2]; };
+// workgroups of a CU (waves of a SIMD) that the registers are cut for
+__host__ __device__ constexpr int occupancy(int D, int NT, bool wide) {
+    return D == 64 ? (NT == 1 ? 4 : NT == 2 && !wide ? 3 : 2) : D == 128 ? (NT == 1 ? (wide ? 2 : 3) : NT == 2 && !wide ? 2 : 1) : NT == 1 && !wide ? 2 : 1;
+}
 
-// WIDE: q in f32 as three bf16 that add up to it, P as two (the second what the first's rounding missed: 2^-17 of a weight).
+template <int D>
+struct Step { Tile<D> k[2], v[2]; bool bad[2]; };      // bad: on a page outside the cache
+
+// WIDE: q in f32 as three bf16 that add up to it, P as three too.
 // Else q is bf16 and P rounded to it (2^-9 of a weight at most), as the output is.
 template <int D, int NT, bool WIDE>
-__global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv(AttnArgs a) {
     constexpr int W = Tile<D>::W, QT = WIDE ? 3 : 1, DT = D / 16;
     constexpr int kVBytes = kStep * v_stride(D), kOBytes = 16 * (D + 4) * 4, kOwn = kVBytes > kOBytes ? kVBytes : kOBytes;
     __shared__ __align__(16) uint8_t lds[kWaves * kOwn];
@@ -142,18 +238,28 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
 
-    const uint32_t id = blockIdx.x, chunk = id % (uint32_t)a.chunks, rest = id / (uint32_t)a.chunks;
-    const uint32_t ny = (uint32_t)(a.kv.heads * a.groups), b = rest / ny, y = rest - b * ny;
-    const int hk = (int)(y / (uint32_t)a.groups), group = (int)(y - hk * a.groups);
+    uint32_t unit, end;
+    for (Place at_unit = share<NT>(a, unit, end); unit < end;) {
+    const int b = at_unit.b;
+    const uint32_t y = at_unit.units / (uint32_t)at_unit.chunks;
+    const int c_off = (int)(at_unit.units - y * at_unit.chunks);
+    const int hk = (int)(y / (uint32_t)at_unit.groups), group = (int)(y - hk * at_unit.groups);
+    const int c_end = min(at_unit.chunks - c_off, (int)(end - unit));        // units of this group here
+    unit += (uint32_t)c_end;
+    const int c_first = at_unit.first + c_off;
+    if (unit < end) at_unit = locate<NT>(a, unit);       // the next group's
 
-    const SeqSpan q = seq_span(a.s.cu, a.s.lens, (int)b, a.rows);
+    const SeqSpan q = seq_span(a.s.cu, a.s.lens, b, a.rows);
     const int m = min(q.m, a.max_rows);                  // rows of this call
     const int f0 = group * 16 * NT, fn = min(m * a.share - f0, 16 * NT);     // the group's first (token, head), and how many
-    if (fn <= 0) return;
     const int first_pos = q.len - q.m;
     const int kmin = sight(a, first_pos + f0 / a.share).lo, kmax = sight(a, first_pos + (f0 + fn - 1) / a.share).hi;
-    const int c0 = (int)chunk * a.chunk, c1 = min(c0 + a.chunk - 1, kmax);   // the chunk's keys, [c0, c1]; chunks * chunk < 2^31
-    if (a.chunks > 1 && (c0 > kmax || c0 + a.chunk <= kmin)) return;         // the join does not look at it
+    const int lmax = sight(a, first_pos + (f0 + fn - 1) / a.share).lo, hmin = sight(a, first_pos + f0 / a.share).hi;
+    // its chunks that a row of the group sees (the join looks at no other); without a join there is one, which answers for all rows
+    const bool one = a.chunks == 1;
+    const int cfirst = max(c_first, one ? 0 : kmin >> a.lgc);
+    const int clast = min(c_first + c_end - 1, one ? 0 : kmax < 0 ? -1 : kmax >> a.lgc);
+    if (cfirst > clast) continue;
 
     // the rows' queries as operands, and what they see
     at_bf8 qf[NT][W][QT];
@@ -183,33 +289,28 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
                     const float4 r0 = *(const float4*)((const float*)a.q + d), r1 = *(const float4*)((const float*)a.q + d + 4);
                     v[0] = r0.x; v[1] = r0.y; v[2] = r0.z; v[3] = r0.w; v[4] = r1.x; v[5] = r1.y; v[6] = r1.z; v[7] = r1.w;
                 }
+                bool odd = false;                        // infinities and NaN have rests of NaN: kept out of the sum
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float left = v[j];
+                for (int j = 0; j < 8; ++j) odd |= !(fabsf(v[j]) < __uint_as_float(0x7f800000u));
+                at_bf8 f3[3];
+                split3(v, f3);
+                if (odd) {
 #pragma unroll
-                    for (int t = 0; t < 3; ++t) {
-                        const __bf16 p = (__bf16)left;
-                        qf[n][w][t][j] = p;
-                        left -= (float)p;
-                    }
-                    if (!(fabsf(v[j]) < 0x1.fep127f)) {  // not finite (or rounds to it): the rests would be NaN
-                        qf[n][w][0][j] = (__bf16)v[j];
-                        qf[n][w][1][j] = qf[n][w][2][j] = (__bf16)0.f;
+                    for (int j = 0; j < 8; ++j) {
+                        const bool is = !(fabsf(v[j]) < __uint_as_float(0x7f800000u));
+                        f3[0][j] = is ? (__bf16)v[j] : f3[0][j];
+                        f3[1][j] = is ? (__bf16)0.f : f3[1][j];
+                        f3[2][j] = is ? (__bf16)0.f : f3[2][j];
                     }
                 }
+#pragma unroll
+                for (int x = 0; x < QT; ++x) qf[n][w][x] = f3[x];
             }
         }
     }
 
     mx_v4f o[NT][DT];
     float mx[NT], ls[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        mx[n] = neg_inf();
-        ls[n] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[n][d] = mx_v4f{0.f, 0.f, 0.f, 0.f};
-    }
 
     uint8_t* const own = lds + wave * kOwn;
     const int* const table = a.s.table + (size_t)b * a.s.ld;
@@ -229,39 +330,49 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
             const size_t token = ((size_t)page * a.kv.heads + hk) * a.kv.page + (k0 & (a.kv.page - 1)) + col;
             st.k[t].load(a.kv.kq, a.kv.ke, token, kg);
             st.v[t].load(a.kv.vq, a.kv.ve, token, kg);
-            if (bad) {                                   // scores of NaN for the rows that see these keys
-#pragma unroll
-                for (int i = 0; i < Tile<D>::S; ++i) st.k[t].e[i] = 255;
-            }
+            st.bad[t] = bad;
         }
     };
 
-    const int s0 = max((kmin - c0) & ~(kStep - 1), 0);   // kmin < c0 + chunk
-    int key0 = c0 + s0 + kStep * ((wave - s0 / kStep) & (kWaves - 1));
-    Step<D> cur, next;
-    if (key0 <= c1) load(key0, cur);
-    for (; key0 <= c1; key0 += kStep * kWaves) {
-        const int after = key0 + kStep * kWaves;
-        if (after <= c1) load(after, next);
+    // Steps go round the waves; of a block of 256 keys a wave has two, each with a buffer of its own, which is filled again for the next
+    // block as soon as its codes are converted: two steps are under way.
+    constexpr int kBlock = 2 * kStep * kWaves;
+    const int blocks = a.chunk / kBlock;                 // of a chunk
+    const int b0 = max(cfirst * blocks, kmin / kBlock), b1 = kmax < 0 ? -1 : min((clast + 1) * blocks - 1, kmax / kBlock);
+    auto wanted = [&](int key0) { return key0 <= kmax && key0 + kStep > kmin; };
+    auto step = [&](int key0, Step<D>& st, int after) {
         const bool inside = key0 >= kmin && key0 + kStep - 1 <= kmax;        // every key is seen by a row: none is other memory
+        const bool all = key0 >= lmax && key0 + kStep - 1 <= hmin;           // every row sees every key
         // values whose scale is NaN, and keys that no row sees: out of the products
-        unsigned long long nan[2][Tile<D>::S];
-        bool any = false;
+        unsigned long long nan[2][Tile<D>::S], any = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key = key0 + 16 * t + col;
-            const bool seen = inside || (key >= kmin && key <= kmax);
+            if (!inside) {
+                const int key = key0 + 16 * t + col;
+                if (key < kmin || key > kmax) {
 #pragma unroll
-            for (int i = 0; i < Tile<D>::S; ++i) {
-                const bool is = cur.v[t].e[i] == 255;
-                nan[t][i] = __ballot(is && seen);
-                any |= nan[t][i] != 0;
-                if (is || !seen) {
-                    cur.v[t].e[i] = 127;
-#pragma unroll
-                    for (int w = 0; w < W / Tile<D>::S; ++w) cur.v[t].c[i * (W / Tile<D>::S) + w] = 0;
+                    for (int i = 0; i < Tile<D>::S; ++i) st.v[t].clear(i);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < Tile<D>::S; ++i) {
+                nan[t][i] = __ballot(st.v[t].e[i] == 255);
+                any |= nan[t][i];
+            }
+        }
+        if (any) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < Tile<D>::S; ++i)
+                    if (st.v[t].e[i] == 255) st.v[t].clear(i);
+        }
+        if (st.bad[0] || st.bad[1]) {                    // scores of NaN for the rows that see these keys
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < Tile<D>::S; ++i)
+                    if (st.bad[t]) st.k[t].e[i] = 255;
         }
         // values to LDS
         wave_fence();
@@ -269,7 +380,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                *(uint4*)(own + (16 * t + col) * v_stride(D) + 2 * Tile<D>::dim(w, kg)) = fp4x8(cur.v[t].c[w], cur.v[t].scale(w));
+                *(uint4*)(own + (16 * t + col) * v_stride(D) + 2 * Tile<D>::dim(w, kg)) = fp4x8(st.v[t].word(w), st.v[t].scale(w));
         // scores
         mx_v4f sc[NT][2];
 #pragma unroll
@@ -278,28 +389,36 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const at_bf8 kf = __builtin_bit_cast(at_bf8, fp4x8(cur.k[t].c[w], cur.k[t].scale(w)));
+                const at_bf8 kf = __builtin_bit_cast(at_bf8, fp4x8(st.k[t].word(w), st.k[t].scale(w)));
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int p = 0; p < QT; ++p) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][w][p], sc[n][t], 0, 0, 0);
             }
-        at_bf8 pf[NT][WIDE ? 2 : 1];
+        if (wanted(after)) load(after, st);
+        at_bf8 pf[NT][QT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float top = neg_inf();
+            if (all) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) sc[n][t] *= a.scale;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + 16 * t + 4 * kg + i;
+                        sc[n][t][i] = key < lo[n] || key > hi[n] ? neg_inf() : sc[n][t][i] * a.scale;
+                    }
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 16 * t + 4 * kg + i;
-                    float v = sc[n][t][i] * a.scale;
-                    if (key < lo[n] || key > hi[n]) v = neg_inf();
-                    sc[n][t][i] = v;
-                    top = fmaxf(top, v);
-                }
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[n][t][i]);
             top = max_xor32(max_xor16(top));
-            const float was = mx[n], now = fmaxf(was, top);
+            // a row's sums go on at a new maximum only when it is past the old one by a factor of 2^8 (weights stay below that, as exact)
+            const float was = mx[n], now = top > was + kSlack ? top : was;
             if (__ballot(now != was)) {                  // times 1 where it is the same
                 const float f = weight(was, now);
                 ls[n] *= f;
@@ -308,16 +427,14 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
                 mx[n] = now;
             }
             const float base = now == neg_inf() ? 0.f : now;
+            float p[8];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(sc[n][t][i] - base);
-                    ls[n] += p;
-                    const __bf16 r = (__bf16)p;
-                    pf[n][0][4 * t + i] = r;
-                    if constexpr (WIDE) pf[n][1][4 * t + i] = (__bf16)(p - (float)r);
-                }
+            for (int i = 0; i < 8; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(sc[n][i / 4][i % 4] - base);
+                ls[n] += p[i];
+            }
+            if constexpr (WIDE) split3(p, pf[n]);
+            else pf[n][0] = __builtin_bit_cast(at_bf8, make_uint4(mx_bf16x2(p[0], p[1]), mx_bf16x2(p[2], p[3]), mx_bf16x2(p[4], p[5]), mx_bf16x2(p[6], p[7])));
         }
         wave_fence();                                    // other lanes read what this one wrote
         // values by transposing reads: lane l gets dim 16 d + l % 16 of the keys 16 t + 4 kg .. + 3
@@ -329,7 +446,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int p = 0; p < (WIDE ? 2 : 1); ++p) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][p], o[n][d], 0, 0, 0);
+                for (int p = 0; p < QT; ++p) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][p], o[n][d], 0, 0, 0);
         }
         if (any) {                                       // uniform, and rare: a key's block of NaN reaches the rows that see the key
 #pragma unroll
@@ -340,30 +457,49 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
                         const int l = __builtin_ctzll(left), key = key0 + 16 * t + (l & 15);
                         const int blk = D == 64 ? (l >> 4) / 2 : i * 4 + (l >> 4);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            if (key >= lo[n] && key <= hi[n]) {
+                        for (int n = 0; n < NT; ++n) {
+                            const float f = key >= lo[n] && key <= hi[n] ? __uint_as_float(0x7fc00000u) : 1.f;
 #pragma unroll
-                                for (int d = 0; d < DT; ++d)
-                                    if (d / 2 == blk) o[n][d] = mx_v4f{1.f, 1.f, 1.f, 1.f} * __uint_as_float(0x7fc00000u);
-                            }
+                            for (int d = 0; d < DT; ++d) o[n][d] *= d / 2 == blk ? f : 1.f;
+                        }
                     }
         }
-        cur = next;
+    };
+
+    Step<D> even, odd;
+    const int own0 = kStep * wave, own1 = own0 + kStep * kWaves;             // its steps of a block
+    if (b0 <= b1) {
+        if (wanted(b0 * kBlock + own0)) load(b0 * kBlock + own0, even);
+        if (wanted(b0 * kBlock + own1)) load(b0 * kBlock + own1, odd);
+    }
+    for (int chunk = cfirst, blk = b0; chunk <= clast; ++chunk) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        mx[n] = neg_inf();
+        ls[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] = mx_v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    for (const int end = min((chunk + 1) * blocks - 1, b1); blk <= end; ++blk) {
+        const int k0 = blk * kBlock, next = blk < b1 ? k0 + kBlock : kNone;
+        if (wanted(k0 + own0)) step(k0 + own0, even, next + own0);
+        else if (wanted(next + own0)) load(next + own0, even);
+        if (wanted(k0 + own1)) step(k0 + own1, odd, next + own1);
+        else if (wanted(next + own1)) load(next + own1, odd);
     }
 
     // the four waves' sums in order; lane (col, kg) has dims 16 d + 4 kg .. + 3 of row col
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        __syncthreads();                                 // the values, or the rows before, are read
+        lds_barrier();                                   // the values, or the rows before, are read
         float* const mine = (float*)own;
 #pragma unroll
         for (int d = 0; d < DT; ++d) *(mx_v4f*)(mine + col * (D + 4) + 16 * d + 4 * kg) = o[n][d];
         const float l = sum_xor32(sum_xor16(ls[n]));
         if (kg == 0) { s_m[wave][col] = mx[n]; s_l[wave][col] = l; }
-        __syncthreads();
-        for (int at = threadIdx.x; at < 16 * D; at += 64 * kWaves) {
+        lds_barrier();
+        for (int at = threadIdx.x; at < min(fn - 16 * n, 16) * D; at += 64 * kWaves) {
             const int r = at / D, d = at % D;
-            if (16 * n + r >= fn) continue;
             float top = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][r]);
@@ -385,24 +521,28 @@ __global__ void __launch_bounds__(64 * kWaves) k_attn_kv(AttnArgs a) {
             }
         }
     }
+    lds_barrier();                                       // before the next chunk's values
+    }
+    }
 }
 
-// One workgroup per row and head: its chunks' weights, then D values as groups of threads that take the chunks in turn, joined in order.
+// One workgroup per row, head and 64 dims: the chunks' weights, then the dims' sums by 16 groups of 16 threads that take the chunks in
+// turn, joined in order.
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
-    constexpr int L = D / 4, G = 256 / L;                // lanes of a group, groups
+    constexpr int P = D / 64, L = 16, G = 256 / L;       // parts of a row's head; lanes of a group, groups
     __shared__ float s_w[kChunks], s_red[8];
-    __shared__ __align__(16) float s_o[G][D];
+    __shared__ __align__(16) float s_o[G][64];
     const int tid = threadIdx.x, wave = tid >> 6;
-    const uint32_t row = blockIdx.x / (uint32_t)a.heads, h = blockIdx.x - row * a.heads;
+    const uint32_t rh = blockIdx.x / P, part = blockIdx.x % P, row = rh / (uint32_t)a.heads, h = rh - row * a.heads;
     const int b = seq_of_row(a.s.cu, a.s.n, (int)row);
     if (b < 0) return;
     const SeqSpan q = seq_span(a.s.cu, a.s.lens, b, a.rows);
     const int i = (int)row - q.r0;
     if (i < 0 || i >= min(q.m, a.max_rows)) return;
     const Sight st = sight(a, q.len - q.m + i);
-    const size_t to = (size_t)row * a.ldo + (size_t)h * D, at = ((size_t)row * a.heads + h) * a.chunks;
-    const int first = st.lo / a.chunk, last = st.hi < st.lo ? -1 : st.hi / a.chunk;              // its chunks, below kChunks
+    const size_t to = (size_t)row * a.ldo + (size_t)h * D + part * 64, at = ((size_t)row * a.heads + h) * a.chunks;
+    const int first = st.lo >> a.lgc, last = st.hi < st.lo ? -1 : st.hi >> a.lgc;                // its chunks, below kChunks
     const bool live = tid >= first && tid <= last;
     float m = neg_inf(), l = 0.f;
     if (live) { m = a.ml[2 * (at + tid)]; l = a.ml[2 * (at + tid) + 1]; }
@@ -418,11 +558,15 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     __syncthreads();
     const int g = tid / L, d = (tid % L) * 4;
     mx_v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int c = first - first % G + g; c <= last; c += G)
-        if (c >= first) o += s_w[c] * *(const mx_v4f*)(a.part + (at + c) * D + d);
+    const float* from = a.part + at * D + part * 64 + d;
+#pragma unroll
+    for (int i = 0; i < kChunks / G; ++i) {              // all asked for together
+        const int c = G * i + g;
+        if (c >= first && c <= last) o += s_w[c] * *(const mx_v4f*)(from + (size_t)c * D);
+    }
     *(mx_v4f*)&s_o[g][d] = o;
     __syncthreads();
-    if (tid < D) {
+    if (tid < 64) {
         float v = 0.f;
 #pragma unroll
         for (int k = 0; k < G; ++k) v += s_o[k][tid];
@@ -430,8 +574,10 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     }
 }
 
-// keys of a chunk: 256, or as many as make 128 chunks of max_len
+// keys of a chunk, a power of two: 1024 make one chunk, which needs no join (700 keys of one sequence: CHUNKONE µs, as three
+// chunks of 256 11.3); beyond, 256, or as many as make 128 chunks
 int chunk_of(int max_len) {
+    if (max_len <= 1024) return 1024;
     int c = kChunk;
     while ((int64_t)c * kChunks < max_len) c *= 2;
     return c;
@@ -441,28 +587,29 @@ int chunks_of(int max_len) { return (max_len + chunk_of(max_len) - 1) / chunk_of
 template <int D, int NT, bool WIDE>
 int launch(AttnArgs& a, hipStream_t s) {
     a.groups = (a.max_rows * a.share + 16 * NT - 1) / (16 * NT);
-    const uint64_t grid = (uint64_t)a.s.n * a.kv.heads * a.groups * a.chunks;
-    if (!grid_fits(grid, 64 * kWaves) || !grid_fits((uint64_t)a.rows * a.heads, 256)) return QMM_ERR_SHAPE;
+    const uint64_t most = (uint64_t)a.s.n * a.kv.heads * a.groups * a.chunks, joins = (uint64_t)a.rows * a.heads * (D / 64);
+    if (most > 0x7fffffff) return QMM_ERR_SHAPE;
+    const uint64_t grid = std::min<uint64_t>(most, (uint64_t)device_cu_count() * occupancy(D, NT, WIDE));      // all resident
+    if (!grid_fits(grid, 64 * kWaves) || !grid_fits(joins, 256)) return QMM_ERR_SHAPE;
     hipLaunchKernelGGL((k_attn_kv<D, NT, WIDE>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
     QMM_LAUNCH_CHECK();
     if (a.chunks > 1) {
-        hipLaunchKernelGGL((k_attn_join<D>), dim3((unsigned)(a.rows * a.heads)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_attn_join<D>), dim3((unsigned)joins), dim3(256), 0, s, a);
         QMM_LAUNCH_CHECK();
     }
     return QMM_OK;
 }
 
-// rows of a workgroup: 16, 32 or 64, what covers a sequence's; fewer where operands and sums would not fit 256 registers
+// rows of a group: 16, 32, 48 or 64, what covers a sequence's; fewer where operands and sums would not fit 256 registers
 template <int D>
 int launch_rows(AttnArgs& a, bool wide, hipStream_t s) {
     const int f = a.max_rows * a.share;
-    if (wide) {
-        if (f <= 16 || D == 256) return launch<D, 1, true>(a, s);
-        if constexpr (D < 256) return launch<D, 2, true>(a, s);
+    if (f <= 16 || D == 256 || (wide && D == 128)) return wide ? launch<D, 1, true>(a, s) : launch<D, 1, false>(a, s);
+    if (f <= 32 || wide || D == 128) {
+        if constexpr (D == 128) return launch<D, 2, false>(a, s);
+        if constexpr (D == 64) return wide ? launch<D, 2, true>(a, s) : launch<D, 2, false>(a, s);
     }
-    if (f <= 16) return launch<D, 1, false>(a, s);
-    if (f <= 32 || D == 256) return launch<D, 2, false>(a, s);
-    if constexpr (D < 256) return launch<D, 4, false>(a, s);
+    if constexpr (D == 64) return f <= 48 || (f > 64 && f <= 96) ? launch<D, 3, false>(a, s) : launch<D, 4, false>(a, s);
     return QMM_ERR_SHAPE;                                // not reached
 }
 
@@ -501,6 +648,7 @@ int qmm_attn_kv_mxfp4(const void* q, int q_dtype, size_t ldq, const qmm_kv_mxfp4
     a.window = attn->window; a.rows = rows; a.heads = heads; a.share = heads / kv->heads; a.max_rows = max_rows; a.max_len = max_len;
     a.chunk = chunk_of(max_len);
     a.chunks = chunks_of(max_len);
+    for (a.lgc = 0; 1 << a.lgc != a.chunk;) ++a.lgc;
     a.part = (float*)ws;
     a.ml = a.part + (need ? (size_t)rows * heads * a.chunks * kv->dim : 0);
     a.q_bf = qb; a.out_bf = ob;

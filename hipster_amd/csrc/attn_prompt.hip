@@ -20,6 +20,7 @@ namespace qmm {
 namespace {
 
 constexpr int kTile = 64;                                // keys of a tile
+constexpr float kSlack = 8.f;                            // a maximum may fall behind by a factor of 2^8: weights are then below 2^8, as exact
 constexpr int kMaxLd = 1 << 24;                          // a tile's byte offsets stay in 32 bits
 
 struct PromptArgs {
@@ -29,7 +30,8 @@ struct PromptArgs {
     const float* sinks;
     size_t ldq, ldo;
     uint32_t ldk, ldv;
-    float scale;                                         // times log2(e)
+    float scale;                                         // its magnitude times log2(e), not 0
+    uint32_t flip;                                       // signs of two values of q: its sign
     int n, window, rows, krows, heads, share, tiles;     // tiles: of q rows, at most
 };
 
@@ -71,7 +73,7 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ cu, int n, int
 }
 
 template <int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) k_attn_prompt(PromptArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(PromptArgs a) {
     constexpr int S = D / 16, DT = D / 32, kRow = 2 * D, kBytes = kTile * kRow, kStage = 2 * kBytes, kSize = 32 * WAVES;
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -103,7 +105,11 @@ __global__ void __launch_bounds__(64 * WAVES) k_attn_prompt(PromptArgs a) {
     {
         const uint16_t* p = a.q + (size_t)(q0 + min(i, m - 1)) * a.ldq + (size_t)h * D + 8 * kg;
 #pragma unroll
-        for (int s = 0; s < S; ++s) qf[s] = *(const at_bf8*)(p + 16 * s);
+        for (int s = 0; s < S; ++s) {
+            uint4 w = *(const uint4*)(p + 16 * s);
+            w.x ^= a.flip; w.y ^= a.flip; w.z ^= a.flip; w.w ^= a.flip;
+            qf[s] = __builtin_bit_cast(at_bf8, w);
+        }
     }
     mx_v16f o[DT];
 #pragma unroll
@@ -163,39 +169,34 @@ __global__ void __launch_bounds__(64 * WAVES) k_attn_prompt(PromptArgs a) {
         }
         const bool whole = key0 + kTile - 1 <= wave_first && key0 >= full_lo;
         float top = neg_inf();
-        if (whole) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) { sc[u][e] *= a.scale; top = fmaxf(top, sc[u][e]); }
-        } else {
+        if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int key = key0 + 32 * u + 8 * (e / 4) + 4 * kg + e % 4;
-                    float v = sc[u][e] * a.scale;
-                    if (key < lo || key > hi) v = neg_inf();
-                    sc[u][e] = v;
-                    top = fmaxf(top, v);
+                    if (key < lo || key > hi) sc[u][e] = neg_inf();
                 }
         }
-        top = swap_max(top);
-        const float now = fmaxf(mx, top);
-        if (__ballot(now != mx)) {
-            const float f = __builtin_amdgcn_exp2f(mx - (now == neg_inf() ? 0.f : now));
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[u][e]);
+        top = swap_max(top) * a.scale;
+        if (__ballot(top > mx + kSlack)) {               // the sums go on at the new maximum
+            const float now = fmaxf(mx, top), f = __builtin_amdgcn_exp2f(mx - (now == neg_inf() ? 0.f : now));
             ls *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
             mx = now;
         }
-        const float base = now == neg_inf() ? 0.f : now;
+        const float base = mx == neg_inf() ? 0.f : mx;
         at_bf8 pf[4];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(sc[u][e] - base);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][e], a.scale, -base));
                 ls += p;
                 pf[2 * u + e / 8][e % 8] = (__bf16)p;
             }
@@ -282,8 +283,11 @@ extern "C" int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_
     if (ldq < nq || ldo < nq || ldk < nk || ldv < nk || ldk > kMaxLd || ldv > kMaxLd) return QMM_ERR_SHAPE;
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || ((ldq | ldk | ldv | ldo) & 7)) return QMM_ERR_ARG;
     if (!aligned(cuq, 4) || !aligned(cuk, 4)) return QMM_ERR_ARG;
-    PromptArgs a{q, k, v, out, cuq, cuk, attn->sinks, ldq, ldo, (uint32_t)ldk, (uint32_t)ldv, (float)((double)attn->scale * 1.44269504088896340736),
+    PromptArgs a{q, k, v, out, cuq, cuk, attn->sinks, ldq, ldo, (uint32_t)ldk, (uint32_t)ldv, 0.f, 0u,
                  nseq, attn->window, rows, krows, heads, heads / kv_heads, 0};
+    // a scale of 0 (all keys weigh the same) as 2^-126: times a masked score, -inf, it is still -inf
+    a.scale = fmaxf((float)(fabs((double)attn->scale) * 1.44269504088896340736), 0x1p-126f);
+    a.flip = attn->scale < 0.f ? 0x80008000u : 0u;
     hipStream_t s = (hipStream_t)stream;
     switch (dim) {
         case 64: return launch<64, 4>(a, s);

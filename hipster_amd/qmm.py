@@ -631,42 +631,69 @@ class KVMXBuf:
     [pages][heads][page][dim / 32] uint8 (scale bytes)."""
 
     def __init__(self, pages, page, heads, dim, device="cuda"):
+        self.held = None                                 # what the calls checked, until a tensor or a size is set
         self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
         self.kq, self.vq = (torch.zeros((pages, heads, page, dim // 2), dtype=torch.uint8, device=device) for _ in range(2))
         self.ke, self.ve = (torch.zeros((pages, heads, page, dim // 32), dtype=torch.uint8, device=device) for _ in range(2))
+
+    def __setattr__(self, name, value):
+        if name != "held":
+            object.__setattr__(self, "held", None)
+        object.__setattr__(self, name, value)
 
     def c(self):
         return KVMX(self.kq.data_ptr(), self.ke.data_ptr(), self.vq.data_ptr(), self.ve.data_ptr(), self.pages, self.page, self.heads, self.dim)
 
 
-def _kv(kv):
-    n = kv.pages * kv.heads * kv.page
-    return KVMX(_in(kv.kq, n * (kv.dim // 2), "kv.kq", torch.uint8), _in(kv.ke, n * (kv.dim // 32), "kv.ke", torch.uint8),
-                _in(kv.vq, n * (kv.dim // 2), "kv.vq", torch.uint8), _in(kv.ve, n * (kv.dim // 32), "kv.ve", torch.uint8),
-                kv.pages, kv.page, kv.heads, kv.dim)
+def _at(t, n, dtype, dev, name):
+    """_in for calls that take many tensors: the address of t, contiguous, of this type, on the current device dev, n elements at least."""
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= n:
+        return t.data_ptr()
+    return _in(t, n, name, dtype)
 
 
-def _seqs(cu, lens, table):
-    n = lens.numel()
-    if table.dim() != 2 or table.shape[0] < n:
-        raise QmmError(f"table must have a row of pages for each of {n} sequences, got shape {tuple(table.shape)}")
-    return Seqs(_in(cu, n + 1, "cu", torch.int32), _in(lens, n, "lens", torch.int32), _in(table, 0, "table", torch.int32), n, table.shape[1])
+def _kv(kv, dev):
+    """The cache as the library takes it, checked when a tensor or a size of kv was set, or moved, or the current device is another."""
+    held = kv.held
+    if held is not None:
+        c, at = held[0], held[1]
+        if at == (kv.kq.data_ptr(), kv.ke.data_ptr(), kv.vq.data_ptr(), kv.ve.data_ptr(), dev):
+            return c
+    tokens, u8 = kv.pages * kv.heads * kv.page, torch.uint8
+    q, e = tokens * (kv.dim // 2), tokens * (kv.dim // 32)
+    p = (_at(kv.kq, q, u8, dev, "kv.kq"), _at(kv.ke, e, u8, dev, "kv.ke"), _at(kv.vq, q, u8, dev, "kv.vq"), _at(kv.ve, e, u8, dev, "kv.ve"))
+    c = KVMX(*p, kv.pages, kv.page, kv.heads, kv.dim)
+    kv.held = (c, (*p, dev))
+    return c
 
 
-def _heads(t, rows, heads, dim, name):
+def _seqs(cu, lens, table, dev):
+    n, i32 = lens.numel(), torch.int32
+    shape = table.shape
+    if len(shape) != 2 or shape[0] < n:
+        raise QmmError(f"table must have a row of pages for each of {n} sequences, got shape {tuple(shape)}")
+    return Seqs(_at(cu, n + 1, i32, dev, "cu"), _at(lens, n, i32, dev, "lens"), _at(table, 0, i32, dev, "table"), n, shape[1])
+
+
+def _heads(t, rows, heads, dim, dev, name):
     """The row stride of t, `rows` rows of heads * dim contiguous values: [rows][heads * dim] or [rows][heads][dim], or one such row."""
-    if t is not None and t.is_cuda and t.dim() == 3:
-        if t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
-            raise QmmError(f"{name} must be rows of {heads} heads of {dim} contiguous values, got shape {tuple(t.shape)}, strides {tuple(t.stride())}")
-        if t.get_device() != _device():
-            raise QmmError(f"{name} is on {t.device}, the current device is cuda:{_device()}")
-        if t.shape[0] < rows:
-            raise QmmError(f"{name} has {t.shape[0]} rows, {rows} are needed")
-        ld = t.stride(0) if t.shape[0] > 1 else heads * dim
-        if ld < heads * dim:
-            raise QmmError(f"{name}: rows overlap (stride {ld}, {heads * dim} values)")
-        return ld
-    return _rows(t, rows, heads * dim, name)
+    n = heads * dim
+    if t is not None and t.get_device() == dev:
+        shape = t.shape
+        if len(shape) == 2 and shape[0] >= rows and shape[1] == n and (n == 1 or t.stride(1) == 1):
+            ld = t.stride(0) if shape[0] > 1 else n
+            if ld >= n:
+                return ld
+        elif len(shape) == 3:
+            if shape[1] != heads or shape[2] != dim or (dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim):
+                raise QmmError(f"{name} must be rows of {heads} heads of {dim} contiguous values, got shape {tuple(shape)}, strides {tuple(t.stride())}")
+            if shape[0] < rows:
+                raise QmmError(f"{name} has {shape[0]} rows, {rows} are needed")
+            ld = t.stride(0) if shape[0] > 1 else n
+            if ld < n:
+                raise QmmError(f"{name}: rows overlap (stride {ld}, {n} values)")
+            return ld
+    return _rows(t, rows, n, name)
 
 
 _STYLE = {"halves": 0, "neighbours": 1}
@@ -684,9 +711,10 @@ def rope_axes(x, out, pos, freq, axis, rows, heads, dim, style="halves", scale=1
     axes, ldp = (1, 0) if pos.dim() == 1 else (pos.shape[0], pos.shape[-1])
     if pos.dim() > 2 or (pos.shape[-1] < rows):
         raise QmmError(f"pos must be [axes][rows] or [rows] with {rows} rows, got shape {tuple(pos.shape)}")
-    ldx, ldo = _heads(x, rows, heads, dim, "x"), _heads(out, rows, heads, dim, "out")
-    r = Rope(_in(freq, pairs, "freq", torch.float32), None if axis is None else _in(axis, pairs, "axis", torch.uint8),
-             _in(pos, 0, "pos", torch.int32), ldp, axes, pairs, _STYLE[style], scale)
+    dev = _device()
+    ldx, ldo = _heads(x, rows, heads, dim, dev, "x"), _heads(out, rows, heads, dim, dev, "out")
+    r = Rope(_at(freq, pairs, torch.float32, dev, "freq"), None if axis is None else _at(axis, pairs, torch.uint8, dev, "axis"),
+             _at(pos, 0, torch.int32, dev, "pos"), ldp, axes, pairs, _STYLE[style], scale)
     check(_lib.lib().qmm_rope_axes(x.data_ptr(), _dtype(x, "x"), ldx, out.data_ptr(), _dtype(out, "out"), ldo, r, rows, heads, dim, _handle(stream)),
           "rope_axes")
 
@@ -702,15 +730,17 @@ def kv_write_mxfp4(k, v, kv, cu, lens, table, rows, stream=None):
 
     Rows cu[b] .. cu[b + 1] - 1 are the last ones of sequence b, which has lens[b] tokens with them; table[b] are its pages (int32,
     all on the device).  Rows from the last cu on, and tokens outside the table or the cache, are not written."""
-    ldk, ldv = _heads(k, rows, kv.heads, kv.dim, "k"), _heads(v, rows, kv.heads, kv.dim, "v")
-    check(_lib.lib().qmm_kv_write_mxfp4(k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), _kv(kv), _seqs(cu, lens, table), rows,
+    dev, heads, dim = _device(), kv.heads, kv.dim
+    ldk, ldv = _heads(k, rows, heads, dim, dev, "k"), _heads(v, rows, heads, dim, dev, "v")
+    check(_lib.lib().qmm_kv_write_mxfp4(k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), _kv(kv, dev), _seqs(cu, lens, table, dev), rows,
                                         _handle(stream)), "kv_write_mxfp4")
 
 
 def kv_read_mxfp4(kv, cu, lens, table, k, v, rows, stream=None):
     """The values that kv holds for the tokens of these rows (as kv_write_mxfp4 places them) -> k, v, f32 or bf16 (exact in both)."""
-    ldk, ldv = _heads(k, rows, kv.heads, kv.dim, "k"), _heads(v, rows, kv.heads, kv.dim, "v")
-    check(_lib.lib().qmm_kv_read_mxfp4(_kv(kv), _seqs(cu, lens, table), k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), rows,
+    dev, heads, dim = _device(), kv.heads, kv.dim
+    ldk, ldv = _heads(k, rows, heads, dim, dev, "k"), _heads(v, rows, heads, dim, dev, "v")
+    check(_lib.lib().qmm_kv_read_mxfp4(_kv(kv, dev), _seqs(cu, lens, table, dev), k.data_ptr(), ldk, v.data_ptr(), ldv, _same(k, v, "k and v"), rows,
                                        _handle(stream)), "kv_read_mxfp4")
 
 
@@ -719,8 +749,8 @@ def attn_kv_ws_bytes(rows, heads, dim, max_len):
     return _lib.lib().qmm_attn_kv_ws_bytes(rows, heads, dim, max_len)
 
 
-def _attn(scale, dim, window, sinks, heads):
-    return Attn(None if sinks is None else _in(sinks, heads, "sinks", torch.float32), dim ** -0.5 if scale is None else scale, window)
+def _attn(scale, dim, window, sinks, heads, dev):
+    return Attn(None if sinks is None else _at(sinks, heads, torch.float32, dev, "sinks"), dim ** -0.5 if scale is None else scale, window)
 
 
 def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, ws, scale=None, window=0, sinks=None, stream=None):
@@ -729,10 +759,11 @@ def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, w
     q, out: `rows` rows of heads * kv.dim values, f32 or bf16 each; heads / kv.heads (<= 16) successive heads share one of the cache;
     max_len: at least the longest of lens; ws: a uint8 tensor of attn_kv_ws_bytes(rows, heads, kv.dim, max_len) bytes (None where that
     is 0); scale None: dim ** -0.5; window: keys a row sees with its own (0: all); sinks f32 [heads]: a logit beside the keys'."""
-    ldq, ldo = _heads(q, rows, heads, kv.dim, "q"), _heads(out, rows, heads, kv.dim, "out")
-    check(_lib.lib().qmm_attn_kv_mxfp4(q.data_ptr(), _dtype(q, "q"), ldq, _kv(kv), _seqs(cu, lens, table), _attn(scale, kv.dim, window, sinks, heads),
+    dev, dim = _device(), kv.dim
+    ldq, ldo = _heads(q, rows, heads, dim, dev, "q"), _heads(out, rows, heads, dim, dev, "out")
+    check(_lib.lib().qmm_attn_kv_mxfp4(q.data_ptr(), _dtype(q, "q"), ldq, _kv(kv, dev), _seqs(cu, lens, table, dev), _attn(scale, dim, window, sinks, heads, dev),
                                        out.data_ptr(), _dtype(out, "out"), ldo, rows, heads, max_rows, max_len,
-                                       None if ws is None else _in(ws, 0, "ws", torch.uint8), 0 if ws is None else ws.numel(), _handle(stream)),
+                                       None if ws is None else _at(ws, 0, torch.uint8, dev, "ws"), 0 if ws is None else ws.numel(), _handle(stream)),
           "attn_kv_mxfp4")
 
 
@@ -744,8 +775,9 @@ def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None,
         if t.dtype is not torch.bfloat16:
             raise QmmError(f"{name} must be torch.bfloat16, got {t.dtype}")
     rows, krows, n = q.shape[0], k.shape[0], cu_q.numel() - 1
-    ldq, ldo = _heads(q, rows, heads, dim, "q"), _heads(out, rows, heads, dim, "out")
-    ldk, ldv = _heads(k, krows, kv_heads, dim, "k"), _heads(v, krows, kv_heads, dim, "v")
-    check(_lib.lib().qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _in(cu_q, n + 1, "cu_q", torch.int32),
-                                          None if cu_k is None else _in(cu_k, n + 1, "cu_k", torch.int32), n, _attn(scale, dim, window, sinks, heads),
+    dev = _device()
+    ldq, ldo = _heads(q, rows, heads, dim, dev, "q"), _heads(out, rows, heads, dim, dev, "out")
+    ldk, ldv = _heads(k, krows, kv_heads, dim, dev, "k"), _heads(v, krows, kv_heads, dim, dev, "v")
+    check(_lib.lib().qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _at(cu_q, n + 1, torch.int32, dev, "cu_q"),
+                                          None if cu_k is None else _at(cu_k, n + 1, torch.int32, dev, "cu_k"), n, _attn(scale, dim, window, sinks, heads, dev),
                                           rows, krows, heads, kv_heads, dim, _handle(stream)), "attn_prompt_bf16")
