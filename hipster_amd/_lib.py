@@ -182,7 +182,8 @@ SIGNATURES = {
                                   c_int, c_int, c_int, c_int, c_vp, c_sz, c_vp]),
     "qmm_attn_kv_ws_bytes": (c_sz, [c_int, c_int, c_int, c_int]),
     "qmm_attn_prompt_bf16": (c_int, [c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp, c_sz, c_vp, c_vp, c_int, ctypes.POINTER(Attn), c_int, c_int,
-                                     c_int, c_int, c_int, c_vp]),
+                                     c_int, c_int, c_int, c_vp, c_sz, c_vp]),
+    "qmm_attn_prompt_ws_bytes": (c_sz, [c_int, c_int, c_int, c_int, c_int]),
     "qmm_gemm_wq": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
     "qmm_gemm_bf16_ld": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp]),

@@ -47,6 +47,21 @@ __device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, int n, int
     return b >= 0 && r < cu[b + 1] && r >= cu[b] ? b : -1;
 }
 
+// ---- softmax, in powers of two ----
+// 2^(x - m), 0 for x = -inf whatever m
+__device__ __forceinline__ float weight(float x, float m) { return __builtin_amdgcn_exp2f(x - (m == neg_inf() ? 0.f : m)); }
+
+// o / (l + sink's weight); a row that saw nothing and has no sink: 0
+__device__ __forceinline__ float finish(float o, float l, float m, const float* sinks, int h) {
+    if (sinks) {
+        const float t = sinks[h] * kLog2e, top = fmaxf(m, t);
+        const float w = weight(m, top);
+        o *= w;
+        l = l * w + weight(t, top);
+    }
+    return l == 0.f ? 0.f : o / l;
+}
+
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // what the entry points ask of a cache and of the sequences; *lg: log2 of the page

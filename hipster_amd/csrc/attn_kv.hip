@@ -22,7 +22,6 @@
 #include "attn.hpp"
 
 #include <algorithm>
-#include <cstdlib>
 
 namespace qmm {
 namespace {
@@ -133,20 +132,6 @@ __device__ __forceinline__ Place share(const AttnArgs& a, uint32_t& unit, uint32
         else p = locate<NT>(a, unit);
     }
     return p;
-}
-
-// 2^(x - m), 0 for x = -inf whatever m
-__device__ __forceinline__ float weight(float x, float m) { return __builtin_amdgcn_exp2f(x - (m == neg_inf() ? 0.f : m)); }
-
-// o / (l + sink's weight); a row that saw nothing and has no sink: 0
-__device__ __forceinline__ float finish(float o, float l, float m, const float* sinks, int h) {
-    if (sinks) {
-        const float t = sinks[h] * kLog2e, top = fmaxf(m, t);
-        const float w = weight(m, top);
-        o *= w;
-        l = l * w + weight(t, top);
-    }
-    return l == 0.f ? 0.f : o / l;
 }
 
 __device__ __forceinline__ void put(const AttnArgs& a, size_t at, float v) {

@@ -16,9 +16,14 @@
 // pieces, lie in different banks.
 #include "attn.hpp"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace qmm {
 namespace {
 
+constexpr int kWaves = 4, kRows = 32 * kWaves;           // q rows of a workgroup
+constexpr int kParts = 8;                                // at most
 constexpr int kTile = 64;                                // keys of a tile
 constexpr float kSlack = 8.f;                            // a maximum may fall behind by a factor of 2^8: weights are then below 2^8, as exact
 constexpr int kMaxLd = 1 << 24;                          // a tile's byte offsets stay in 32 bits
@@ -33,6 +38,9 @@ struct PromptArgs {
     float scale;                                         // its magnitude times log2(e), not 0
     uint32_t flip;                                       // signs of two values of q: its sign
     int n, window, rows, krows, heads, share, tiles;     // tiles: of q rows, at most
+    int parts;                                           // that a tile's keys are cut into
+    float* part;                                         // [tiles][heads][parts][D / 4][128 rows][4], with more than one
+    float2* ml;                                          // [tiles][heads][parts][128 rows]: m, l
 };
 
 __device__ __forceinline__ float swap_max(float v) {
@@ -72,18 +80,27 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ cu, int n, int
     return false;
 }
 
-template <int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(PromptArgs a) {
-    constexpr int S = D / 16, DT = D / 32, kRow = 2 * D, kBytes = kTile * kRow, kStage = 2 * kBytes, kSize = 32 * WAVES;
+// the piece that row r's piece p lies at is p ^ turn: 16 rows' pieces of keys in different 16 bytes of 256, and 4 rows' 4 pieces of values
+template <int D>
+__device__ __forceinline__ int key_turn(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+template <int D>
+__device__ __forceinline__ int val_turn(int r) { return D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
+
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(PromptArgs a) {
+    constexpr int S = D / 16, DT = D / 32, kRow = 2 * D, kBytes = kTile * kRow;
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, kg = lane >> 5;
 
     // the last tiles first: they see the most keys
-    const uint32_t id = blockIdx.x;
-    const int h = (int)(id % (uint32_t)a.heads), t = a.tiles - 1 - (int)(id / (uint32_t)a.heads), hk = h / a.share;
+    const uint32_t id = blockIdx.x, turn = id / (uint32_t)a.heads;
+    const int h = (int)(id - turn * a.heads), hk = h / a.share;
+    const int part = (int)(turn % (uint32_t)a.parts), t = a.tiles - 1 - (int)(turn / (uint32_t)a.parts);
     int b, r0;
-    if (!find_tile(a.cuq, a.n, a.rows, kSize, t, b, r0)) return;
+    if (!find_tile(a.cuq, a.n, a.rows, kRows, t, b, r0)) return;
     const int q0 = within(a.cuq[b], a.rows), m = within(a.cuq[b + 1], a.rows) - q0;
     if (r0 < 0 || r0 >= m) return;                       // only where so many spans overlap that their tiles' count wrapped
     const int* const cuk = a.cuk ? a.cuk : a.cuq;
@@ -97,7 +114,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
     const int lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0, hi = pos;
     // the wave's and the workgroup's keys
     const int wave_first = min(r0 + 32 * wave, m - 1) + shift, wave_last = min(r0 + 32 * wave + 31, m - 1) + shift;
-    const int last = min(r0 + kSize - 1, m - 1) + shift, first = a.window > 0 && r0 + shift >= a.window ? r0 + shift - a.window + 1 : 0;
+    const int last = min(r0 + kRows - 1, m - 1) + shift, first = a.window > 0 && r0 + shift >= a.window ? r0 + shift - a.window + 1 : 0;
     const int wave_lo = a.window > 0 && wave_first >= a.window ? wave_first - a.window + 1 : 0;
     const int full_lo = a.window > 0 && wave_last >= a.window ? wave_last - a.window + 1 : 0;       // from here on all rows see
 
@@ -111,64 +128,77 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
             qf[s] = __builtin_bit_cast(at_bf8, w);
         }
     }
-    mx_v16f o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float mx = neg_inf(), ls = 0.f;
-
     // DMA of a tile: 1 KiB an instruction, kTile * kRow / 1024 of each matrix over the waves
-    constexpr int kLines = kBytes / 1024 / WAVES, kPieces = kRow / 16, kRowsPer = 1024 / kRow;      // rows an instruction
+    constexpr int kLines = kBytes / 1024 / kWaves, kPieces = kRow / 16, kPerLine = 1024 / kRow;      // rows an instruction
     static_assert(kLines >= 1, "");
     const uint8_t* const kbase = (const uint8_t*)(a.k + (size_t)k0 * a.ldk + (size_t)hk * D);
     const uint8_t* const vbase = (const uint8_t*)(a.v + (size_t)k0 * a.ldv + (size_t)hk * D);
     const uint32_t lds0 = lds_addr(smem);
-    auto fetch = [&](int key0, int stage) {              // keys key0 .. + 63, those past the last as the last
-        const uint8_t* kp = kbase + (size_t)key0 * a.ldk * 2;
-        const uint8_t* vp = vbase + (size_t)key0 * a.ldv * 2;
+    // keys (or values) key0 .. + 63 into buffer `stage`, those past the last as the last
+    auto fetch_k = [&](int key0, int stage) {
+        const uint8_t* from = kbase + (size_t)key0 * a.ldk * 2;
 #pragma unroll
         for (int j = 0; j < kLines; ++j) {
-            const int line = wave * kLines + j, r = line * kRowsPer + lane / kPieces, p = lane % kPieces;
-            const uint32_t row = (uint32_t)min(r, n - 1 - key0);
-            const uint32_t to = lds0 + stage * kStage + line * 1024;
-            dma16s(kp, row * a.ldk * 2 + (uint32_t)((p ^ (r & 7)) * 16), __builtin_amdgcn_readfirstlane(to));
-            dma16s(vp, row * a.ldv * 2 + (uint32_t)((p ^ (2 * (r & 3))) * 16), __builtin_amdgcn_readfirstlane(to + kBytes));
+            const int line = wave * kLines + j, r = line * kPerLine + lane / kPieces, p = lane % kPieces;
+            dma16s(from, (uint32_t)min(r, n - 1 - key0) * a.ldk * 2 + (uint32_t)((p ^ key_turn<D>(r)) * 16),
+                   __builtin_amdgcn_readfirstlane(lds0 + stage * kBytes + line * 1024));
+        }
+    };
+    auto fetch_v = [&](int key0, int stage) {
+        const uint8_t* from = vbase + (size_t)key0 * a.ldv * 2;
+#pragma unroll
+        for (int j = 0; j < kLines; ++j) {
+            const int line = wave * kLines + j, r = line * kPerLine + lane / kPieces, p = lane % kPieces;
+            dma16s(from, (uint32_t)min(r, n - 1 - key0) * a.ldv * 2 + (uint32_t)((p ^ val_turn<D>(r)) * 16),
+                   __builtin_amdgcn_readfirstlane(lds0 + (2 + stage) * kBytes + line * 1024));
         }
     };
     // addresses of operands within a tile
-    uint32_t ka[4], va[2];
+    constexpr int KA = D == 64 ? 4 : 8, VA = D == 64 ? 2 : 4;
+    uint32_t ka[KA], va[VA];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) ka[s] = col * kRow + (((2 * s) ^ kg ^ (col & 7)) & 7) * 16;
+    for (int s = 0; s < KA; ++s) ka[s] = col * kRow + ((2 * s + kg) ^ key_turn<D>(col)) * 16;
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
-        const int r = (lane & 15) >> 2, piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        va[d] = (4 * kg + r) * kRow + (piece ^ (2 * r)) * 16 + (lane & 1) * 8;
+    for (int d = 0; d < VA; ++d) {
+        const int r = 4 * kg + ((lane & 15) >> 2), piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        va[d] = r * kRow + (piece ^ val_turn<D>(r)) * 16 + (lane & 1) * 8;
     }
 
-    const int t0 = first / kTile, t1 = last < 0 ? -1 : last / kTile;
-    if (t0 <= t1) fetch(t0 * kTile, 0);
-    for (int kt = t0; kt <= t1; ++kt) {
-        const int key0 = kt * kTile, stage = (kt - t0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();                                   // the tile is there, and all are done with the other buffer
-        if (kt < t1) fetch(key0 + kTile, stage ^ 1);
-        if (key0 > wave_last || key0 + kTile <= wave_lo) continue;           // uniform: nothing of it for this wave
-        const uint8_t* const ks = smem + stage * kStage;
-        const uint8_t* const vs = ks + kBytes;
-        mx_v16f sc[2];
+    int t0 = first / kTile, t1 = last < 0 ? -1 : last / kTile;
+    if (a.parts > 1) {                                   // this workgroup's part of them
+        const int each = max((t1 - t0 + a.parts) / a.parts, 1);
+        t0 += part * each;
+        t1 = min(t1, t0 + each - 1);
+    }
+    mx_v16f o[DT], sc[2];
+    float mx, ls, raw;                                   // raw: the largest of sc, unmasked
+    // scores of the tile in key buffer `stage`
+    auto scores = [&](int stage, mx_v16f (&to)[2]) {
+        const uint8_t* const ks = smem + stage * kBytes;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+            for (int e = 0; e < 16; ++e) to[u][e] = 0.f;
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const at_bf8 kf = *(const at_bf8*)(ks + ka[s & 3] + u * 32 * kRow + (s / 4) * 128);
-                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], sc[u], 0, 0, 0);
+                const at_bf8 kf = *(const at_bf8*)(ks + ka[s % KA] + u * 32 * kRow + (s / KA) * 256);
+                to[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], to[u], 0, 0, 0);
             }
         }
+    };
+    // a row's largest score of a tile
+    auto row_max = [&](const mx_v16f (&v)[2]) {
+        float tops[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) tops[e % 4] = fmaxf(tops[e % 4], v[e / 16][e % 16]);
+        return swap_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+    };
+    // One tile: its weights from its scores in sc, the next tile's scores (NEXT) beside them, its values' product.  SAFE: values that are
+    // not finite are kept out of the products where some row does not see them, as 0 times one is not 0.
+    auto tile = [&](int kt, int stage, auto next, auto safe) {
+        constexpr bool NEXT = decltype(next)::value, SAFE = decltype(safe)::value;
+        const int key0 = kt * kTile;
         const bool whole = key0 + kTile - 1 <= wave_first && key0 >= full_lo;
-        float top = neg_inf();
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -178,11 +208,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
                     if (key < lo || key > hi) sc[u][e] = neg_inf();
                 }
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[u][e]);
-        top = swap_max(top) * a.scale;
+        const float top = (whole ? raw : row_max(sc)) * a.scale;
         if (__ballot(top > mx + kSlack)) {               // the sums go on at the new maximum
             const float now = fmaxf(mx, top), f = __builtin_amdgcn_exp2f(mx - (now == neg_inf() ? 0.f : now));
             ls *= f;
@@ -191,29 +217,32 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
             mx = now;
         }
         const float base = mx == neg_inf() ? 0.f : mx;
+        mx_v16f sn[2];
+        if constexpr (NEXT) scores(stage ^ 1, sn);
         at_bf8 pf[4];
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][e], a.scale, -base));
-                ls += p;
-                pf[2 * u + e / 8][e % 8] = (__bf16)p;
-            }
-        bool odd = false;                                // a value that is not finite, where some rows may not see it
+        for (int e = 0; e < 32; ++e) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 16][e % 16], a.scale, -base));
+            sums[e % 4] += p;
+            pf[e / 8][e % 8] = (__bf16)p;
+        }
+        ls += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        const uint8_t* const vs = smem + (2 + stage) * kBytes;
+        bool odd = false;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const uint8_t* from = vs + va[d & 1] + s * 16 * kRow + (d / 2) * 128;
+                const uint8_t* from = vs + va[d % VA] + s * 16 * kRow + (d / VA) * 256;
                 const at_s4 v0 = tr_read(from), v1 = tr_read(from + 8 * kRow);
                 at_bf8 vf = __builtin_bit_cast(at_bf8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                if (!whole) {
+                if constexpr (SAFE) {
                     uint4 w = __builtin_bit_cast(uint4, vf);
                     uint32_t* x = (uint32_t*)&w;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool l = (x[e] & 0x7f80u) == 0x7f80u, g = (x[e] & 0x7f800000u) == 0x7f800000u;
+                        const bool l = !whole && (x[e] & 0x7f80u) == 0x7f80u, g = !whole && (x[e] & 0x7f800000u) == 0x7f800000u;
                         odd |= l | g;
                         x[e] = (l ? 0u : x[e] & 0xffffu) | (g ? 0u : x[e] & 0xffff0000u);
                     }
@@ -221,32 +250,80 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
                 }
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], o[d], 0, 0, 0);
             }
-        if (!whole && __ballot(odd)) {                   // they reach the rows that see their key, and no other
-            for (int key = max(key0, wave_lo); key <= min(key0 + kTile - 1, wave_last); ++key) {
-                const int r = key - key0;
-                const bool sees = key >= lo && key <= hi;
+        if constexpr (SAFE) {
+            if (__ballot(odd))                           // they reach the rows that see their key, and no other
+                for (int key = max(key0, wave_lo); key <= min(key0 + kTile - 1, wave_last); ++key) {
+                    const int r = key - key0;
+                    const bool sees = key >= lo && key <= hi;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+                    for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int dim = 32 * d + 8 * (e / 4) + 4 * kg + e % 4;
-                        const uint32_t x = *(const uint16_t*)(vs + r * kRow + (((dim >> 3) ^ (2 * (r & 3))) * 16) + (dim & 7) * 2);
-                        if ((x & 0x7f80u) == 0x7f80u && sees) o[d][e] += bf2f(x);
-                    }
-            }
+                        for (int e = 0; e < 16; ++e) {
+                            const int dim = 32 * d + 8 * (e / 4) + 4 * kg + e % 4;
+                            const uint32_t x = *(const uint16_t*)(vs + r * kRow + (((dim >> 3) ^ val_turn<D>(r)) * 16) + (dim & 7) * 2);
+                            if ((x & 0x7f80u) == 0x7f80u && sees) o[d][e] += bf2f(x);
+                        }
+                }
         }
-    }
+        if constexpr (NEXT) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sc[u] = sn[u];
+            raw = row_max(sc);
+        }
+    };
+    // All tiles.  Keys are one tile ahead of values: K(t + 2) and V(t + 1) come while tile t is worked on.
+    auto tiles = [&](auto safe) {
+        mx = neg_inf();
+        ls = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        if (t0 > t1) return;
+        fetch_k(t0 * kTile, 0);
+        fetch_v(t0 * kTile, 0);
+        if (t0 < t1) fetch_k((t0 + 1) * kTile, 1);
+        wait_dma();
+        lds_barrier();
+        scores(0, sc);
+        raw = row_max(sc);
+        for (int kt = t0; kt < t1; ++kt) {
+            const int stage = (kt - t0) & 1;
+            wait_dma();
+            lds_barrier();                               // K(kt + 1) and V(kt) are there, and all are done with K(kt) and V(kt - 1)
+            if (kt + 1 < t1) fetch_k((kt + 2) * kTile, stage);
+            fetch_v((kt + 1) * kTile, stage ^ 1);
+            tile(kt, stage, std::true_type{}, safe);
+        }
+        wait_dma();
+        lds_barrier();
+        tile(t1, (t1 - t0) & 1, std::false_type{}, safe);
+    };
+    tiles(std::false_type{});
+    // Where all is finite that is it.  A value that is not, at a key that some row of a tile does not see, made that row's sum NaN:
+    // once more, with such values kept out (all waves, as they fetch together).
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z = __builtin_fmaf(o[d][e], 0.f, z);
+    if (__syncthreads_or(!(z == 0.f))) tiles(std::true_type{});
 
     ls = swap_sum(ls);
     if (!live) return;
-    float f;
-    if (a.sinks) {
-        const float t = a.sinks[h] * kLog2e, top = fmaxf(mx, t), base = top == neg_inf() ? 0.f : top;
-        const float w = __builtin_amdgcn_exp2f(mx - base), l = ls * w + __builtin_amdgcn_exp2f(t - base);
-        f = l == 0.f ? 0.f : w / l;
-    } else {
-        f = ls == 0.f ? 0.f : 1.f / ls;
+    if (a.parts > 1) {
+        const size_t at = ((size_t)t * a.heads + h) * a.parts + part;
+        const int r = 32 * wave + col;
+        if (kg == 0) a.ml[at * kRows + r] = make_float2(mx, ls);
+        if (t0 > t1) return;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *(mx_v4f*)(a.part + ((at * (D / 4) + 8 * d + 2 * e + kg) * kRows + r) * 4) = mx_v4f{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+        return;
     }
+    const float f = finish(1.f, ls, mx, a.sinks, h);
     uint16_t* const to = a.out + (size_t)(q0 + i) * a.ldo + (size_t)h * D + 4 * kg;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -255,14 +332,61 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) k_attn_prompt(Pr
             *(uint2*)(to + 32 * d + 8 * e) = make_uint2(mx_bf16x2(o[d][4 * e] * f, o[d][4 * e + 1] * f), mx_bf16x2(o[d][4 * e + 2] * f, o[d][4 * e + 3] * f));
 }
 
-template <int D, int WAVES>
+// The parts of a tile's rows: 32 rows a workgroup, a thread one row's every eighth four dims.
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_prompt_join(PromptArgs a) {
+    const uint32_t id = blockIdx.x, th = id >> 2;
+    const int h = (int)(th % (uint32_t)a.heads), t = (int)(th / (uint32_t)a.heads);
+    int b, r0;
+    if (!find_tile(a.cuq, a.n, a.rows, kRows, t, b, r0)) return;
+    const int q0 = within(a.cuq[b], a.rows), m = within(a.cuq[b + 1], a.rows) - q0;
+    const int r = (int)(id & 3) * 32 + (threadIdx.x & 31);
+    if (r0 < 0 || r0 + r >= m) return;
+    const size_t at = ((size_t)t * a.heads + h) * a.parts;
+    float w[kParts], top = neg_inf(), l = 0.f;
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+        if (p < a.parts) top = fmaxf(top, a.ml[(at + p) * kRows + r].x);
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+        if (p < a.parts) {
+            const float2 v = a.ml[(at + p) * kRows + r];
+            w[p] = weight(v.x, top);
+            l += w[p] * v.y;
+        }
+    const float f = finish(1.f, l, top, a.sinks, h);
+    uint16_t* const to = a.out + (size_t)(q0 + r0 + r) * a.ldo + (size_t)h * D;
+    for (int d = (int)threadIdx.x >> 5; d < D / 4; d += 8) {
+        mx_v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+            if (p < a.parts && !(w[p] == 0.f)) o += w[p] * *(const mx_v4f*)(a.part + (((at + p) * (D / 4) + d) * kRows + r) * 4);
+        *(uint2*)(to + 4 * d) = make_uint2(mx_bf16x2(o[0] * f, o[1] * f), mx_bf16x2(o[2] * f, o[3] * f));
+    }
+}
+
+// tiles of q rows of a call, at most: a sequence's last may be short
+int64_t tiles_of(int rows, int nseq) { return nseq == 1 ? ((int64_t)rows + kRows - 1) / kRows : (int64_t)rows / kRows + nseq; }
+
+// Parts that a tile's keys are cut into: one, or where that leaves half the CUs' room without work as many as fill it, of 8 tiles of
+// keys at least.
+int parts_of(int rows, int krows, int nseq, int heads, int dim) {
+    const int64_t work = tiles_of(rows, nseq) * heads, room = (int64_t)device_cu_count() * (dim == 256 ? 1 : 2);
+    const int64_t keys = ((int64_t)krows / nseq + kTile - 1) / kTile;
+    return (int)std::max<int64_t>(std::min<int64_t>({room / std::max<int64_t>(work, 1), keys / 8, kParts}), 1);
+}
+
+template <int D>
 int launch(PromptArgs& a, hipStream_t s) {
-    constexpr int kLds = 2 * 2 * kTile * 2 * D, kSize = 32 * WAVES;
-    const int64_t tiles = (int64_t)a.rows / kSize + a.n;                     // a sequence's last tile may be short
-    if (tiles > 0x7fffffff || !grid_fits((uint64_t)tiles * a.heads, 64 * WAVES)) return QMM_ERR_SHAPE;
-    a.tiles = (int)tiles;
-    hipLaunchKernelGGL((k_attn_prompt<D, WAVES>), dim3((unsigned)(tiles * a.heads)), dim3(64 * WAVES), kLds, s, a);
+    constexpr int kLds = 4 * kTile * 2 * D;
+    const uint64_t grid = (uint64_t)a.tiles * a.heads * a.parts;
+    if (!grid_fits(grid, 64 * kWaves)) return QMM_ERR_SHAPE;
+    hipLaunchKernelGGL((k_attn_prompt<D>), dim3((unsigned)grid), dim3(64 * kWaves), kLds, s, a);
     QMM_LAUNCH_CHECK();
+    if (a.parts > 1) {
+        hipLaunchKernelGGL((k_attn_prompt_join<D>), dim3((unsigned)(a.tiles * a.heads * 4)), dim3(256), 0, s, a);
+        QMM_LAUNCH_CHECK();
+    }
     return QMM_OK;
 }
 
@@ -271,9 +395,17 @@ int launch(PromptArgs& a, hipStream_t s) {
 
 using namespace qmm;
 
-extern "C" int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
-                                    const int32_t* cuq, const int32_t* cuk, int nseq, const qmm_attn* attn, int rows, int krows, int heads,
-                                    int kv_heads, int dim, void* stream) {
+extern "C" {
+
+size_t qmm_attn_prompt_ws_bytes(int rows, int krows, int nseq, int heads, int dim) {
+    if (rows <= 0 || krows <= 0 || nseq <= 0 || heads <= 0 || (dim != 64 && dim != 128 && dim != 256)) return 0;
+    const int p = parts_of(rows, krows, nseq, heads, dim);
+    return p == 1 ? 0 : (size_t)tiles_of(rows, nseq) * heads * p * kRows * (dim + 2) * sizeof(float);
+}
+
+int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
+                         const int32_t* cuq, const int32_t* cuk, int nseq, const qmm_attn* attn, int rows, int krows, int heads, int kv_heads, int dim,
+                         void* ws, size_t ws_bytes, void* stream) {
     if (dim != 64 && dim != 128 && dim != 256) return QMM_ERR_SHAPE;
     if (rows < 0 || krows < 0 || nseq < 0 || heads < 1 || kv_heads < 1 || heads > 65536 || heads % kv_heads) return QMM_ERR_SHAPE;
     if (const int st = attn_check(attn)) return st;
@@ -283,15 +415,29 @@ extern "C" int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_
     if (ldq < nq || ldo < nq || ldk < nk || ldv < nk || ldk > kMaxLd || ldv > kMaxLd) return QMM_ERR_SHAPE;
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || ((ldq | ldk | ldv | ldo) & 7)) return QMM_ERR_ARG;
     if (!aligned(cuq, 4) || !aligned(cuk, 4)) return QMM_ERR_ARG;
-    PromptArgs a{q, k, v, out, cuq, cuk, attn->sinks, ldq, ldo, (uint32_t)ldk, (uint32_t)ldv, 0.f, 0u,
-                 nseq, attn->window, rows, krows, heads, heads / kv_heads, 0};
+    const int64_t tiles = tiles_of(rows, nseq);
+    if (tiles * heads > 0x1fffffff) return QMM_ERR_SHAPE;
+    PromptArgs a;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.cuq = cuq; a.cuk = cuk; a.sinks = attn->sinks; a.ldq = ldq; a.ldo = ldo;
+    a.ldk = (uint32_t)ldk; a.ldv = (uint32_t)ldv;
     // a scale of 0 (all keys weigh the same) as 2^-126: times a masked score, -inf, it is still -inf
     a.scale = fmaxf((float)(fabs((double)attn->scale) * 1.44269504088896340736), 0x1p-126f);
     a.flip = attn->scale < 0.f ? 0x80008000u : 0u;
+    a.n = nseq; a.window = attn->window; a.rows = rows; a.krows = krows; a.heads = heads; a.share = heads / kv_heads; a.tiles = (int)tiles;
+    const size_t need = qmm_attn_prompt_ws_bytes(rows, krows, nseq, heads, dim);
+    a.parts = ws ? parts_of(rows, krows, nseq, heads, dim) : 1;
+    if (a.parts > 1) {
+        if (ws_bytes < need) return QMM_ERR_WORKSPACE;
+        if (!aligned(ws, 16)) return QMM_ERR_ARG;
+        a.part = (float*)ws;
+        a.ml = (float2*)(a.part + (size_t)tiles * heads * a.parts * kRows * dim);
+    }
     hipStream_t s = (hipStream_t)stream;
     switch (dim) {
-        case 64: return launch<64, 4>(a, s);
-        case 128: return launch<128, 4>(a, s);
-        default: return launch<256, 4>(a, s);
+        case 64: return launch<64>(a, s);
+        case 128: return launch<128>(a, s);
+        default: return launch<256>(a, s);
     }
 }
+
+}  // extern "C"

@@ -767,17 +767,31 @@ def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, w
           "attn_kv_mxfp4")
 
 
-def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None, window=0, sinks=None, stream=None):
+def attn_prompt_ws_bytes(rows, krows, nseq, heads, dim):
+    """Bytes of attn_prompt_bf16's workspace (0: it needs none)."""
+    return _lib.lib().qmm_attn_prompt_ws_bytes(rows, krows, nseq, heads, dim)
+
+
+def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None, window=0, sinks=None, ws=None, stream=None):
     """Causal attention of packed sequences: rows cu_q[b] .. cu_q[b + 1] - 1 of q, the last ones of the tokens cu_k[b] .. cu_k[b + 1] - 1
     of k and v (cu_k None: cu_q).  q, out rows of heads * dim values, k, v of kv_heads * dim, all bf16 (row strides multiples of 8);
-    scale, window and sinks as in attn_kv_mxfp4."""
+    scale, window and sinks as in attn_kv_mxfp4.  ws: a uint8 tensor of attn_prompt_ws_bytes(...) bytes; None: torch's allocator gives one
+    where few rows see many keys (False: none, the keys stay in one part)."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         if t.dtype is not torch.bfloat16:
             raise QmmError(f"{name} must be torch.bfloat16, got {t.dtype}")
     rows, krows, n = q.shape[0], k.shape[0], cu_q.numel() - 1
-    dev = _device()
+    dev, L = _device(), _lib.lib()
     ldq, ldo = _heads(q, rows, heads, dim, dev, "q"), _heads(out, rows, heads, dim, dev, "out")
     ldk, ldv = _heads(k, krows, kv_heads, dim, dev, "k"), _heads(v, krows, kv_heads, dim, dev, "v")
-    check(_lib.lib().qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _at(cu_q, n + 1, torch.int32, dev, "cu_q"),
-                                          None if cu_k is None else _at(cu_k, n + 1, torch.int32, dev, "cu_k"), n, _attn(scale, dim, window, sinks, heads, dev),
-                                          rows, krows, heads, kv_heads, dim, _handle(stream)), "attn_prompt_bf16")
+    handle = _handle(stream)
+    if ws is None:
+        size = L.qmm_attn_prompt_ws_bytes(rows, krows, n, heads, dim)
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+            if stream is not None:
+                ws.record_stream(stream)
+    pw, size = (_at(ws, 0, torch.uint8, dev, "ws"), ws.numel()) if isinstance(ws, torch.Tensor) else (None, 0)
+    check(L.qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _at(cu_q, n + 1, torch.int32, dev, "cu_q"),
+                                 None if cu_k is None else _at(cu_k, n + 1, torch.int32, dev, "cu_k"), n, _attn(scale, dim, window, sinks, heads, dev),
+                                 rows, krows, heads, kv_heads, dim, pw, size, handle), "attn_prompt_bf16")

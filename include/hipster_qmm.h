@@ -521,10 +521,14 @@ size_t qmm_attn_kv_ws_bytes(int rows, int heads, int dim, int max_len);
 /* causal attention of packed sequences, bf16: q and out [rows][heads][dim], k and v [krows][kv_heads][dim] with row strides in values
  * (multiples of 8, 16-byte aligned).  Sequence b has the q rows cuq[b] .. cuq[b + 1] - 1 and the keys cuk[b] .. cuk[b + 1] - 1
  * (cuk NULL: cuq); of m rows and n keys, row i is at position n - m + i.  The formula of qmm_attn_kv_mxfp4; dim 64, 128 or 256; heads
- * a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were. */
+ * a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were.
+ * ws: qmm_attn_prompt_ws_bytes(...) bytes, 16-byte aligned, for calls with few rows and many keys, whose keys are then cut into parts
+ * that are joined (the bits are others); NULL: no parts.  Calls that overlap need one each. */
 int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
                          const int32_t* cuq, const int32_t* cuk, int nseq, const qmm_attn* attn, int rows, int krows, int heads, int kv_heads, int dim,
-                         void* stream);
+                         void* ws, size_t ws_bytes, void* stream);
+/* bytes of its workspace (0: it would use none) */
+size_t qmm_attn_prompt_ws_bytes(int rows, int krows, int nseq, int heads, int dim);
 
 #ifdef __cplusplus
 }
