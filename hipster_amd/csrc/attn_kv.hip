@@ -13,8 +13,7 @@
 //     scale) of key l % 16, one conversion instruction makes two bf16 of them, scale included, exactly.  Which dims a lane's eight
 //     of a step are does not matter as long as Q's operand has the same.
 //   - Values have to be turned (the second product sums over keys): a wave writes 32 keys' values as bf16 into LDS of its own and reads
-//     them back with the transposing read, four keys of 16 dims at a time.  Rows are 32 bytes longer than their values, so that four
-//     rows' 32 bytes lie in different banks.
+//     them back with the transposing read, four keys of 16 dims at a time.
 // The four waves of a workgroup take the chunk's steps of 32 keys in turn and join their (m, l, O) through LDS in order.
 //
 // A chunk's length goes by max_len alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
@@ -26,7 +25,7 @@
 namespace qmm {
 namespace {
 
-constexpr int kWaves = 4, kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kChunk = 256, kMaxLen = 1 << 30, kNone = 0x7fff0000;
+constexpr int kWaves = 4, kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kMaxLen = 1 << 30, kNone = 0x7fff0000;
 constexpr float kSlack = 8.f;
 
 struct AttnArgs {
@@ -41,10 +40,13 @@ struct AttnArgs {
     float scale;                                         // times log2(e)
     int lg, window, rows, heads, share, max_rows, max_len, chunk, chunks, groups;   // groups: of 16 NT rows
     int lgc;                                             // log2 of chunk
-    int q_bf, out_bf;
+    int q_bf, out_bf, out_vec;                           // out_vec: four values of a row of out are aligned
 };
 
-__host__ __device__ constexpr int v_stride(int D) { return 2 * D + 32; }       // bytes of a key's values in LDS
+// A key's values in LDS: 2 D bytes, its 16-byte piece p at p ^ v_turn(key).  What is written together (a piece of eight keys) and read
+// together (two pieces of eight keys) then lies in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t v_turn(int key) { return (uint32_t)(D == 64 ? key & 7 : (key & 7) ^ ((key & 1) << 3)); }
 
 // the positions that a token at `pos` sees, [lo, hi]
 struct Sight { int lo, hi; };
@@ -134,9 +136,10 @@ __device__ __forceinline__ Place share(const AttnArgs& a, uint32_t& unit, uint32
     return p;
 }
 
-__device__ __forceinline__ void put(const AttnArgs& a, size_t at, float v) {
-    if (a.out_bf) ((uint16_t*)a.out)[at] = (uint16_t)mx_bf16x2(v, 0.f);
-    else ((float*)a.out)[at] = v;
+// four values of a row
+__device__ __forceinline__ void put4(const AttnArgs& a, size_t at, const mx_v4f& v) {
+    if (a.out_bf) mx_store4<true>(a.out, at, v, 4, a.out_vec);
+    else mx_store4<false>(a.out, at, v, 4, a.out_vec);
 }
 
 // v, an f32, as three bf16 that add up to it: its leading 8 significant bits, the next 8 and the last 8 (dropping bits, not rounding,
@@ -217,9 +220,11 @@ struct Step { Tile<D> k[2], v[2]; bool bad[2]; };      // bad: on a page outside
 template <int D, int NT, bool WIDE>
 __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv(AttnArgs a) {
     constexpr int W = Tile<D>::W, QT = WIDE ? 3 : 1, DT = D / 16;
-    constexpr int kVBytes = kStep * v_stride(D), kOBytes = 16 * (D + 4) * 4, kOwn = kVBytes > kOBytes ? kVBytes : kOBytes;
-    __shared__ __align__(16) uint8_t lds[kWaves * kOwn];
+    constexpr int kOwn = (16 * (D + 4) * 4 + 511) / 512 * 512;               // of a wave: 32 keys' values, or 16 rows' sums
+    static_assert(kOwn >= kStep * 2 * D, "");
+    __shared__ __align__(512) uint8_t lds[kWaves * kOwn];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    __shared__ int s_row[16 * NT], s_head[16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
 
@@ -246,6 +251,11 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
     const int clast = min(c_first + c_end - 1, one ? 0 : kmax < 0 ? -1 : kmax >> a.lgc);
     if (cfirst > clast) continue;
 
+    if (threadIdx.x < 16 * NT) {                         // read behind the chunks' barriers
+        const int f = f0 + (int)threadIdx.x, i = f / a.share;
+        s_row[threadIdx.x] = q.r0 + i;
+        s_head[threadIdx.x] = hk * a.share + f - i * a.share;
+    }
     // the rows' queries as operands, and what they see
     at_bf8 qf[NT][W][QT];
     int lo[NT], hi[NT];
@@ -298,6 +308,10 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
     float mx[NT], ls[NT];
 
     uint8_t* const own = lds + wave * kOwn;
+    // where this lane writes the first piece of its key's values, and where it reads those of its row (offsets below 2 D come by xor)
+    const uint32_t v_to = (uint32_t)col * (2 * D) + ((uint32_t)(Tile<D>::dim(0, kg) / 8) ^ v_turn<D>(col)) * 16;
+    const int v_row = 4 * kg + (col >> 2);
+    const uint32_t v_from = (uint32_t)v_row * (2 * D) + ((uint32_t)((col >> 1) & 1) ^ v_turn<D>(v_row)) * 16 + 8 * (col & 1);
     const int* const table = a.s.table + (size_t)b * a.s.ld;
     int block = -1, entry = 0;                           // lane l: the page of the 16 keys from 1024 block + 16 l on
     auto load = [&](int key0, Step<D>& st) {             // the step of the 32 keys from key0 on
@@ -361,11 +375,12 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
         }
         // values to LDS
         wave_fence();
+        const uint32_t to = opaque(v_to);                // the pieces' addresses are made anew each time, not kept
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                *(uint4*)(own + (16 * t + col) * v_stride(D) + 2 * Tile<D>::dim(w, kg)) = fp4x8(st.v[t].word(w), st.v[t].scale(w));
+                *(uint4*)(own + 16 * t * (2 * D) + (to ^ (Tile<D>::dim(w, 0) * 2))) = fp4x8(st.v[t].word(w), st.v[t].scale(w));
         // scores
         mx_v4f sc[NT][2];
 #pragma unroll
@@ -423,10 +438,11 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
         }
         wave_fence();                                    // other lanes read what this one wrote
         // values by transposing reads: lane l gets dim 16 d + l % 16 of the keys 16 t + 4 kg .. + 3
+        const uint32_t at_row = opaque(v_from);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            const uint8_t* from = own + (4 * kg + (col >> 2)) * v_stride(D) + 32 * d + 8 * (col & 3);
-            const at_s4 v0 = tr_read(from), v1 = tr_read(from + 16 * v_stride(D));
+            const uint8_t* from = own + (at_row ^ (32 * d));
+            const at_s4 v0 = tr_read(from), v1 = tr_read(from + 16 * 2 * D);
             const at_bf8 vf = __builtin_bit_cast(at_bf8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -483,26 +499,31 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
         const float l = sum_xor32(sum_xor16(ls[n]));
         if (kg == 0) { s_m[wave][col] = mx[n]; s_l[wave][col] = l; }
         lds_barrier();
-        for (int at = threadIdx.x; at < min(fn - 16 * n, 16) * D; at += 64 * kWaves) {
-            const int r = at / D, d = at % D;
+        const int tid = (int)opaque(threadIdx.x);        // addresses made here, not kept through the steps
+#pragma unroll 1
+        for (int k = 0; k < D / 64; ++k) {               // four dims a thread
+            const int at = tid + 64 * kWaves * k, r = at / (D / 4), d = at % (D / 4) * 4;
+            if (16 * n + r >= fn) break;
             float top = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][r]);
-            float v = 0.f, sum = 0.f;
+            mx_v4f v = {0.f, 0.f, 0.f, 0.f};
+            float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 const float f = weight(s_m[w][r], top);
-                v += f * ((const float*)(lds + w * kOwn))[r * (D + 4) + d];
+                v += f * *(const mx_v4f*)((const float*)(lds + w * kOwn) + r * (D + 4) + d);
                 sum += f * s_l[w][r];
             }
-            const int f = f0 + 16 * n + r, i = f / a.share, h = hk * a.share + f - i * a.share;
-            const size_t row = (size_t)(q.r0 + i);
+            const int h = s_head[16 * n + r];
+            const size_t row = (size_t)s_row[16 * n + r];
             if (a.chunks == 1) {
-                put(a, row * a.ldo + (size_t)h * D + d, finish(v, sum, top, a.sinks, h));
+                const float f = finish(1.f, sum, top, a.sinks, h);
+                put4(a, row * a.ldo + (size_t)h * D + d, v * f);
             } else {
                 const size_t to = (row * a.heads + h) * a.chunks + chunk;
-                a.part[to * D + d] = v;
-                if (d == 0) { a.ml[2 * to] = top; a.ml[2 * to + 1] = sum; }
+                *(mx_v4f*)(a.part + to * D + d) = v;
+                if (d == 0) *(float2*)(a.ml + 2 * to) = make_float2(top, sum);
             }
         }
     }
@@ -511,14 +532,13 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
     }
 }
 
-// One workgroup per row, head and 64 dims: the chunks' weights, then the dims' sums by 16 groups of 16 threads that take the chunks in
-// turn, joined in order.
+// One wave per row, head and 64 dims: the chunks' weights, then the dims' sums by four groups of 16 lanes that take the chunks in turn.
+// A chunk's place in every sum goes by its number alone.
 template <int D>
-__global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
-    constexpr int P = D / 64, L = 16, G = 256 / L;       // parts of a row's head; lanes of a group, groups
-    __shared__ float s_w[kChunks], s_red[8];
-    __shared__ __align__(16) float s_o[G][64];
-    const int tid = threadIdx.x, wave = tid >> 6;
+__global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
+    constexpr int P = D / 64, G = 4;                     // parts of a row's head; groups
+    __shared__ float s_w[kChunks];
+    const int lane = threadIdx.x;
     const uint32_t rh = blockIdx.x / P, part = blockIdx.x % P, row = rh / (uint32_t)a.heads, h = rh - row * a.heads;
     const int b = seq_of_row(a.s.cu, a.s.n, (int)row);
     if (b < 0) return;
@@ -526,44 +546,54 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     const int i = (int)row - q.r0;
     if (i < 0 || i >= min(q.m, a.max_rows)) return;
     const Sight st = sight(a, q.len - q.m + i);
-    const size_t to = (size_t)row * a.ldo + (size_t)h * D + part * 64, at = ((size_t)row * a.heads + h) * a.chunks;
+    const size_t at = ((size_t)row * a.heads + h) * a.chunks;
     const int first = st.lo >> a.lgc, last = st.hi < st.lo ? -1 : st.hi >> a.lgc;                // its chunks, below kChunks
-    const bool live = tid >= first && tid <= last;
-    float m = neg_inf(), l = 0.f;
-    if (live) { m = a.ml[2 * (at + tid)]; l = a.ml[2 * (at + tid) + 1]; }
-    float top = m;
+    float m[kChunks / 64], l[kChunks / 64], top = neg_inf(), sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kChunks / 64; ++k) {
+        const int c = 64 * k + lane;
+        const bool live = c >= first && c <= last;
+        const float2 v = live ? *(const float2*)(a.ml + 2 * (at + c)) : make_float2(neg_inf(), 0.f);
+        m[k] = v.x;
+        l[k] = v.y;
+        top = fmaxf(top, m[k]);
+    }
     for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-    if ((tid & 63) == 0) s_red[wave] = top;
-    __syncthreads();
-    top = fmaxf(s_red[0], s_red[1]);                     // two waves have all the chunks
-    const float w = live ? weight(m, top) : 0.f;
-    if (tid < kChunks) s_w[tid] = w;
-    const float sum = wave_sum(w * l);                   // a chunk's place in the sums goes by its number alone
-    if ((tid & 63) == 0) s_red[4 + wave] = sum;
-    __syncthreads();
-    const int g = tid / L, d = (tid % L) * 4;
-    mx_v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kChunks / 64; ++k) {
+        const float w = weight(m[k], top);
+        s_w[64 * k + lane] = w;
+        sum += w * l[k];
+    }
+    sum = wave_sum(sum);
+    wave_fence();
+    const int g = lane >> 4, d = (lane & 15) * 4;
     const float* from = a.part + at * D + part * 64 + d;
+    mx_v4f o = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = first & ~(8 * G - 1); c0 <= last; c0 += 8 * G) {           // eight chunks a lane asked for together
+        mx_v4f v[8];
 #pragma unroll
-    for (int i = 0; i < kChunks / G; ++i) {              // all asked for together
-        const int c = G * i + g;
-        if (c >= first && c <= last) o += s_w[c] * *(const mx_v4f*)(from + (size_t)c * D);
-    }
-    *(mx_v4f*)&s_o[g][d] = o;
-    __syncthreads();
-    if (tid < 64) {
-        float v = 0.f;
+        for (int i8 = 0; i8 < 8; ++i8) {
+            const int c = c0 + G * i8 + g;
+            v[i8] = c >= first && c <= last ? *(const mx_v4f*)(from + (size_t)c * D) : mx_v4f{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
-        for (int k = 0; k < G; ++k) v += s_o[k][tid];
-        put(a, to + tid, finish(v, s_red[4] + s_red[5], top, a.sinks, (int)h));
+        for (int i8 = 0; i8 < 8; ++i8) {
+            const int c = c0 + G * i8 + g;
+            o += (c >= first && c <= last ? s_w[c] : 0.f) * v[i8];
+        }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = sum_xor32(sum_xor16(o[e]));
+    const float f = finish(1.f, sum, top, a.sinks, (int)h);
+    if (g == 0) put4(a, (size_t)row * a.ldo + (size_t)h * D + part * 64 + d, o * f);
 }
 
 // keys of a chunk, a power of two: 1024 make one chunk, which needs no join (700 keys of one sequence: CHUNKONE µs, as three
 // chunks of 256 11.3); beyond, 256, or as many as make 128 chunks
 int chunk_of(int max_len) {
     if (max_len <= 1024) return 1024;
-    int c = kChunk;
+    int c = max_len <= 2048 ? 256 : 512;
     while ((int64_t)c * kChunks < max_len) c *= 2;
     return c;
 }
@@ -575,11 +605,11 @@ int launch(AttnArgs& a, hipStream_t s) {
     const uint64_t most = (uint64_t)a.s.n * a.kv.heads * a.groups * a.chunks, joins = (uint64_t)a.rows * a.heads * (D / 64);
     if (most > 0x7fffffff) return QMM_ERR_SHAPE;
     const uint64_t grid = std::min<uint64_t>(most, (uint64_t)device_cu_count() * occupancy(D, NT, WIDE));      // all resident
-    if (!grid_fits(grid, 64 * kWaves) || !grid_fits(joins, 256)) return QMM_ERR_SHAPE;
+    if (!grid_fits(grid, 64 * kWaves) || !grid_fits(joins, 64)) return QMM_ERR_SHAPE;
     hipLaunchKernelGGL((k_attn_kv<D, NT, WIDE>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
     QMM_LAUNCH_CHECK();
     if (a.chunks > 1) {
-        hipLaunchKernelGGL((k_attn_join<D>), dim3((unsigned)joins), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_attn_join<D>), dim3((unsigned)joins), dim3(64), 0, s, a);
         QMM_LAUNCH_CHECK();
     }
     return QMM_OK;
@@ -637,6 +667,7 @@ int qmm_attn_kv_mxfp4(const void* q, int q_dtype, size_t ldq, const qmm_kv_mxfp4
     a.part = (float*)ws;
     a.ml = a.part + (need ? (size_t)rows * heads * a.chunks * kv->dim : 0);
     a.q_bf = qb; a.out_bf = ob;
+    a.out_vec = aligned(out, ob ? 8 : 16) && ldo % 4 == 0;
     hipStream_t s = (hipStream_t)stream;
     const bool wide = !qb || !ob;
     switch (kv->dim) {
