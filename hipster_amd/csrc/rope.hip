@@ -14,7 +14,7 @@
 namespace qmm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kBatch = 4;
 
 struct RopeArgs {
     const void* x;
@@ -112,33 +112,41 @@ __global__ void __launch_bounds__(kThreads) k_rope_axes(RopeArgs a) {
     }
     const int h0 = (int)g * a.per, h1 = min(h0 + a.per, a.heads);
     const bool both = second < a.dim;
-    for (int h = h0; h < h1; ++h) {
-        const size_t from = (size_t)t * a.ldx + (size_t)h * a.dim, to = (size_t)t * a.ldo + (size_t)h * a.dim;
-        float p[V], q[V];
-        load<BI, V>(a.x, from + first, p);
-        load<BI, V>(a.x, from + (both ? second : first), q);
-        if (turn) {
-            if constexpr (NEXT && V == 4) {              // pairs (p0, p1), (p2, p3), (q0, q1), (q2, q3)
-                const float v[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
-                float w[8];
+    for (int h = h0; h < h1; h += kBatch) {              // a batch of heads is asked for before the first of them is written
+        float p[kBatch][V], q[kBatch][V];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[2 * i] = v[2 * i] * c[i] - v[2 * i + 1] * s[i];
-                    w[2 * i + 1] = v[2 * i + 1] * c[i] + v[2 * i] * s[i];
-                }
+        for (int j = 0; j < kBatch; ++j) {
+            const size_t from = (size_t)t * a.ldx + (size_t)min(h + j, h1 - 1) * a.dim;
+            load<BI, V>(a.x, from + first, p[j]);
+            load<BI, V>(a.x, from + (both ? second : first), q[j]);
+        }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { p[i] = w[i]; q[i] = w[4 + i]; }
-            } else {
+        for (int j = 0; j < kBatch; ++j) {
+            if (h + j >= h1) break;
+            if (turn) {
+                if constexpr (NEXT && V == 4) {          // pairs (p0, p1), (p2, p3), (q0, q1), (q2, q3)
+                    const float v[8] = {p[j][0], p[j][1], p[j][2], p[j][3], q[j][0], q[j][1], q[j][2], q[j][3]};
+                    float w[8];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float e = p[i] * c[i] - q[i] * s[i], f = q[i] * c[i] + p[i] * s[i];
-                    p[i] = e;
-                    q[i] = f;
+                    for (int i = 0; i < 4; ++i) {
+                        w[2 * i] = v[2 * i] * c[i] - v[2 * i + 1] * s[i];
+                        w[2 * i + 1] = v[2 * i + 1] * c[i] + v[2 * i] * s[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { p[j][i] = w[i]; q[j][i] = w[4 + i]; }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float e = p[j][i] * c[i] - q[j][i] * s[i], f = q[j][i] * c[i] + p[j][i] * s[i];
+                        p[j][i] = e;
+                        q[j][i] = f;
+                    }
                 }
             }
+            const size_t to = (size_t)t * a.ldo + (size_t)(h + j) * a.dim;
+            store<BO, V>(a.out, to + first, p[j]);
+            if (both) store<BO, V>(a.out, to + second, q[j]);
         }
-        store<BO, V>(a.out, to + first, p);
-        if (both) store<BO, V>(a.out, to + second, q);
     }
 }
 
