@@ -791,7 +791,7 @@ def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None,
             ws = torch.empty(size, dtype=torch.uint8, device=q.device)
             if stream is not None:
                 ws.record_stream(stream)
-    pw, size = (_at(ws, 0, torch.uint8, dev, "ws"), ws.numel()) if isinstance(ws, torch.Tensor) else (None, 0)
+    pw, size = (_at(ws, 0, torch.uint8, dev, "ws"), ws.numel()) if ws is not None and ws is not False else (None, 0)
     check(L.qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _at(cu_q, n + 1, torch.int32, dev, "cu_q"),
                                  None if cu_k is None else _at(cu_k, n + 1, torch.int32, dev, "cu_k"), n, _attn(scale, dim, window, sinks, heads, dev),
                                  rows, krows, heads, kv_heads, dim, pw, size, handle), "attn_prompt_bf16")

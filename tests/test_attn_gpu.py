@@ -519,6 +519,53 @@ def test_prompt_long(gpu):
         assert (np.abs(got[pick, h] - want) <= bound + 2.0 ** -8 * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, False), (1500, True)])
+def test_prompt_keys_in_parts(gpu, D, window, sinks):
+    """Few rows behind many keys: the keys are cut into parts.  A workspace of the caller's gives the bits of the one that is made; without one
+    the formula holds too; one too small is refused."""
+    lens, ms, Hq, Hk = [2300, 900], [70, 20], 4, 2
+    out, q, k, v, s = run_prompt(lens, ms, Hq, Hk, D, window, sinks)
+    size = qmm.attn_prompt_ws_bytes(91, 3201, 2, Hq, D)
+    assert size > 0
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    args = (q, k, v, ints(offsets(ms)), ints(offsets(lens)))
+    for w in (ws, ws, False):
+        got = torch.full_like(out, 3.0)
+        qmm.attn_prompt_bf16(*args, got, Hq, Hk, D, window=window, sinks=s, ws=w)
+        if w is False:
+            check_prompt(got, q, k, v, s, lens, ms, Hq, Hk, D, window)
+        else:
+            assert torch.equal(got, out)
+    with pytest.raises(QmmError, match="WORKSPACE"):
+        qmm.attn_prompt_bf16(*args, out, Hq, Hk, D, ws=ws[:-16])
+    st = torch.cuda.Stream()                             # a workspace made for another stream
+    st.wait_stream(torch.cuda.current_stream())
+    got = torch.full_like(out, 3.0)
+    st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        qmm.attn_prompt_bf16(*args, got, Hq, Hk, D, window=window, sinks=s, stream=st)
+    torch.cuda.synchronize()
+    assert torch.equal(got, out)
+
+
+def test_prompt_parts_not_finite(gpu):
+    """A value that is not finite in one part: it reaches the rows that see it, in that dim."""
+    lens, ms, D = [2300], [40], 128
+    out, q, k, v, _ = run_prompt(lens, ms, 2, 1, D)
+    v2 = v.clone()
+    v2[100, 0, 5], v2[2280, 0, 9] = float("inf"), float("nan")
+    got = torch.full_like(out, 3.0)
+    qmm.attn_prompt_bf16(q, k, v2, ints([0, 40]), ints([0, 2300]), got, 2, 1, D)
+    want = out.float()
+    want[:40, :, 5] = float("inf")
+    want[20:40, :, 9] = float("nan")
+    w, o = want[:40], got.float()[:40]
+    assert torch.equal(o.isnan(), w.isnan()) and torch.equal(o.isinf(), w.isinf())
+    fin = w.isfinite()
+    assert torch.equal(o[fin], w[fin])
+
+
 # ---------------------------------------------------------------- together
 def block(s):
     """Positions, cache, attention of one step, as a decoder block runs them."""
@@ -658,6 +705,6 @@ def test_foreign_tensors_are_refused(gpu):
         with pytest.raises(QmmError):
             qmm.kv_write_mxfp4(a["k"], x, kv, a["cu"], ln, a["table"], 2)
     with pytest.raises(QmmError):
-        qmm.attn_kv_mxfp4(x, kv, cu, ln, table, x.clone(), 2, 1, 2, 1000, torch.empty(8, dtype=torch.uint8, device="cuda"))
+        qmm.attn_kv_mxfp4(x, kv, cu, ln, table, x.clone(), 2, 1, 2, 5000, torch.empty(8, dtype=torch.uint8, device="cuda"))
     with pytest.raises(QmmError):
         qmm.attn_prompt_bf16(x.float(), x, x, cu, None, x.clone(), 1, 1, 64)
