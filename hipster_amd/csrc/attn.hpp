@@ -31,6 +31,17 @@ __device__ __forceinline__ SeqSpan seq_span(const int* __restrict__ cu, const in
     return {r0, max(r1 - r0, 0), max(lens[b], 0)};
 }
 
+// the sum of the lanes up to this one: within rows of 16 lanes by shifts, then the rows' last sums to the rows behind them
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);       // from 1, 2, 4, 8 lanes below
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);       // lane 15 of the row below, rows 1 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);       // lane 31, rows 2 and 3
+    return v;
+}
+
 // The sequence that row r (the same in all lanes) belongs to, -1: none.  The wave compares 64 offsets at a time, so that up to 64
 // sequences cost one load's latency.
 __device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, int n, int r) {

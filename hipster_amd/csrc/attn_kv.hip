@@ -25,7 +25,7 @@
 namespace qmm {
 namespace {
 
-constexpr int kWaves = 4, kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kMaxLen = 1 << 30, kNone = 0x7fff0000;
+constexpr int kStep = 32, kMaxRows = 16, kMaxShare = 16, kChunks = 128, kMaxLen = 1 << 30, kNone = 0x7fff0000;
 constexpr float kSlack = 8.f;
 
 struct AttnArgs {
@@ -75,15 +75,15 @@ __device__ __forceinline__ float sum_xor32(float v) {
 // The units of work, in order: sequence, kv head, group of 16 NT rows, chunk.  What a call has of them is known on the device alone;
 // each workgroup counts them and takes its share.  A unit's place: its sequence, that one's chunks (from `first` on) and groups, and
 // the unit's number in it (`units`); past the last unit: `units` is how many there are.  The wave adds up 64 sequences at a time.
-struct Place { int b, first, chunks, groups; uint32_t units; };
-struct Counts { int first, chunks, groups; uint32_t mine, upto; };           // a lane's sequence; upto: of the sequences to it
+struct Place { int b, first, chunks, groups; uint32_t units; SeqSpan q; };
+struct Counts { int first, chunks, groups; uint32_t mine, upto; SeqSpan q; };           // a lane's sequence; upto: of the sequences to it
 
 template <int NT>
 __device__ __forceinline__ Counts count(const AttnArgs& a, int base) {
     const int lane = threadIdx.x & 63;
-    Counts c = {0, 0, 0, 0, 0};
+    Counts c = {0, 0, 0, 0, 0, {0, 0, 0}};
     if (base + lane < a.s.n) {
-        const SeqSpan q = seq_span(a.s.cu, a.s.lens, base + lane, a.rows);
+        const SeqSpan q = c.q = seq_span(a.s.cu, a.s.lens, base + lane, a.rows);
         const int m = min(q.m, a.max_rows);
         if (m > 0) {
             const int lo = sight(a, q.len - q.m).lo, hi = sight(a, q.len - q.m + m - 1).hi;
@@ -92,12 +92,8 @@ __device__ __forceinline__ Counts count(const AttnArgs& a, int base) {
             c.groups = (m * a.share + 16 * NT - 1) / (16 * NT);
         }
     }
-    c.mine = c.upto = (uint32_t)(c.chunks * c.groups * a.kv.heads);
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const uint32_t v = (uint32_t)__shfl_up((int)c.upto, k, 64);
-        if (lane >= k) c.upto += v;
-    }
+    c.mine = (uint32_t)(c.chunks * c.groups * a.kv.heads);
+    c.upto = wave_upto(c.mine);
     return c;
 }
 // the place of a unit that lies in the 64 sequences counted in c, `before` units lying in front of them
@@ -106,12 +102,13 @@ __device__ __forceinline__ bool pick(const Counts& c, int base, uint32_t before,
     if (!behind) return false;
     const int l = __builtin_ctzll(behind);
     p = {base + l, __builtin_amdgcn_readlane(c.first, l), __builtin_amdgcn_readlane(c.chunks, l), __builtin_amdgcn_readlane(c.groups, l),
-         unit - before - (uint32_t)__builtin_amdgcn_readlane((int)(c.upto - c.mine), l)};
+         unit - before - (uint32_t)__builtin_amdgcn_readlane((int)(c.upto - c.mine), l),
+         {__builtin_amdgcn_readlane(c.q.r0, l), __builtin_amdgcn_readlane(c.q.m, l), __builtin_amdgcn_readlane(c.q.len, l)}};
     return true;
 }
 template <int NT>
 __device__ __forceinline__ Place locate(const AttnArgs& a, uint32_t unit) {
-    Place p = {-1, 0, 1, 1, 0};
+    Place p = {-1, 0, 1, 1, 0, {0, 0, 0}};
     for (int base = 0; base < a.s.n; base += 64) {
         const Counts c = count<NT>(a, base);
         if (pick(c, base, p.units, unit, p)) return p;
@@ -122,7 +119,7 @@ __device__ __forceinline__ Place locate(const AttnArgs& a, uint32_t unit) {
 // the workgroup's first unit and the one after its last, and the first one's place: as many as any other's, one more at most
 template <int NT>
 __device__ __forceinline__ Place share(const AttnArgs& a, uint32_t& unit, uint32_t& end) {
-    Place p = {-1, 0, 1, 1, 0};
+    Place p = {-1, 0, 1, 1, 0, {0, 0, 0}};
     const bool once = a.s.n <= 64;
     Counts c;
     if (once) c = count<NT>(a, 0);
@@ -217,13 +214,13 @@ struct Step { Tile<D> k[2], v[2]; bool bad[2]; };      // bad: on a page outside
 
 // WIDE: q in f32 as three bf16 that add up to it, P as three too.
 // Else q is bf16 and P rounded to it (2^-9 of a weight at most), as the output is.
-template <int D, int NT, bool WIDE>
-__global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv(AttnArgs a) {
+template <int D, int NT, bool WIDE, int NW>
+__global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW / 4)) k_attn_kv(AttnArgs a) {
     constexpr int W = Tile<D>::W, QT = WIDE ? 3 : 1, DT = D / 16;
     constexpr int kOwn = (16 * (D + 4) * 4 + 511) / 512 * 512;               // of a wave: 32 keys' values, or 16 rows' sums
     static_assert(kOwn >= kStep * 2 * D, "");
-    __shared__ __align__(512) uint8_t lds[kWaves * kOwn];
-    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    __shared__ __align__(512) uint8_t lds[NW * kOwn];
+    __shared__ float s_m[NW][16], s_l[NW][16];
     __shared__ int s_row[16 * NT], s_head[16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
@@ -239,7 +236,7 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
     const int c_first = at_unit.first + c_off;
     if (unit < end) at_unit = locate<NT>(a, unit);       // the next group's
 
-    const SeqSpan q = seq_span(a.s.cu, a.s.lens, b, a.rows);
+    const SeqSpan q = at_unit.q;
     const int m = min(q.m, a.max_rows);                  // rows of this call
     const int f0 = group * 16 * NT, fn = min(m * a.share - f0, 16 * NT);     // the group's first (token, head), and how many
     const int first_pos = q.len - q.m;
@@ -335,7 +332,7 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
 
     // Steps go round the waves; of a block of 256 keys a wave has two, each with a buffer of its own, which is filled again for the next
     // block as soon as its codes are converted: two steps are under way.
-    constexpr int kBlock = 2 * kStep * kWaves;
+    constexpr int kBlock = 2 * kStep * NW;
     const int blocks = a.chunk / kBlock;                 // of a chunk
     const int b0 = max(cfirst * blocks, kmin / kBlock), b1 = kmax < 0 ? -1 : min((clast + 1) * blocks - 1, kmax / kBlock);
     auto wanted = [&](int key0) { return key0 <= kmax && key0 + kStep > kmin; };
@@ -468,7 +465,7 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
     };
 
     Step<D> even, odd;
-    const int own0 = kStep * wave, own1 = own0 + kStep * kWaves;             // its steps of a block
+    const int own0 = kStep * wave, own1 = own0 + kStep * NW;             // its steps of a block
     if (b0 <= b1) {
         if (wanted(b0 * kBlock + own0)) load(b0 * kBlock + own0, even);
         if (wanted(b0 * kBlock + own1)) load(b0 * kBlock + own1, odd);
@@ -501,16 +498,16 @@ __global__ void __launch_bounds__(64 * kWaves, occupancy(D, NT, WIDE)) k_attn_kv
         lds_barrier();
         const int tid = (int)opaque(threadIdx.x);        // addresses made here, not kept through the steps
 #pragma unroll 1
-        for (int k = 0; k < D / 64; ++k) {               // four dims a thread
-            const int at = tid + 64 * kWaves * k, r = at / (D / 4), d = at % (D / 4) * 4;
-            if (16 * n + r >= fn) break;
+        for (int k = 0; k < (4 * D + 64 * NW - 1) / (64 * NW); ++k) {         // four dims a thread
+            const int at = tid + 64 * NW * k, r = at / (D / 4), d = at % (D / 4) * 4;
+            if (r >= 16 || 16 * n + r >= fn) break;
             float top = s_m[0][r];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][r]);
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, s_m[w][r]);
             mx_v4f v = {0.f, 0.f, 0.f, 0.f};
             float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float f = weight(s_m[w][r], top);
                 v += f * *(const mx_v4f*)((const float*)(lds + w * kOwn) + r * (D + 4) + d);
                 sum += f * s_l[w][r];
@@ -599,14 +596,14 @@ int chunk_of(int max_len) {
 }
 int chunks_of(int max_len) { return (max_len + chunk_of(max_len) - 1) / chunk_of(max_len); }
 
-template <int D, int NT, bool WIDE>
+template <int D, int NT, bool WIDE, int NW>
 int launch(AttnArgs& a, hipStream_t s) {
     a.groups = (a.max_rows * a.share + 16 * NT - 1) / (16 * NT);
     const uint64_t most = (uint64_t)a.s.n * a.kv.heads * a.groups * a.chunks, joins = (uint64_t)a.rows * a.heads * (D / 64);
     if (most > 0x7fffffff) return QMM_ERR_SHAPE;
-    const uint64_t grid = std::min<uint64_t>(most, (uint64_t)device_cu_count() * occupancy(D, NT, WIDE));      // all resident
-    if (!grid_fits(grid, 64 * kWaves) || !grid_fits(joins, 64)) return QMM_ERR_SHAPE;
-    hipLaunchKernelGGL((k_attn_kv<D, NT, WIDE>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+    const uint64_t grid = std::min<uint64_t>(most, (uint64_t)device_cu_count() * (occupancy(D, NT, WIDE) * 4 / NW));     // all resident
+    if (!grid_fits(grid, 64 * NW) || !grid_fits(joins, 64)) return QMM_ERR_SHAPE;
+    hipLaunchKernelGGL((k_attn_kv<D, NT, WIDE, NW>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
     QMM_LAUNCH_CHECK();
     if (a.chunks > 1) {
         hipLaunchKernelGGL((k_attn_join<D>), dim3((unsigned)joins), dim3(64), 0, s, a);
@@ -615,11 +612,22 @@ int launch(AttnArgs& a, hipStream_t s) {
     return QMM_OK;
 }
 
+// Waves of a workgroup: four; eight where the keys are one chunk (few workgroups, whose own time counts) and two waves of the kernel
+// share a SIMD.
+template <int D, int NT, bool WIDE>
+int launch(AttnArgs& a, hipStream_t s) {
+    if constexpr (occupancy(D, NT, WIDE) >= 2)
+        if (a.chunks == 1) return launch<D, NT, WIDE, 8>(a, s);
+    return launch<D, NT, WIDE, 4>(a, s);
+}
+
 // rows of a group: 16, 32, 48 or 64, what covers a sequence's; fewer where operands and sums would not fit 256 registers
 template <int D>
 int launch_rows(AttnArgs& a, bool wide, hipStream_t s) {
     const int f = a.max_rows * a.share;
     if (f <= 16 || D == 256 || (wide && D == 128)) return wide ? launch<D, 1, true>(a, s) : launch<D, 1, false>(a, s);
+    if constexpr (D == 64)
+        if (wide && (f > 32 && f <= 48)) return launch<D, 3, true>(a, s);
     if (f <= 32 || wide || D == 128) {
         if constexpr (D == 128) return launch<D, 2, false>(a, s);
         if constexpr (D == 64) return wide ? launch<D, 2, true>(a, s) : launch<D, 2, false>(a, s);

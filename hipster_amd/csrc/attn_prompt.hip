@@ -61,16 +61,12 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ cu, int n, int
         const int at = base + lane;
         int tiles = 0;
         if (at < n) tiles = (max(within(cu[at + 1], rows) - within(cu[at], rows), 0) + size - 1) / size;
-        int upto = tiles;
-        for (int k = 1; k < 64; k <<= 1) {
-            const int v = __shfl_up(upto, k, 64);
-            if (lane >= k) upto += v;
-        }
+        const int upto = (int)wave_upto((uint32_t)tiles);
         const unsigned long long behind = __ballot(before + upto > t);
         if (behind) {
             const int l = __builtin_ctzll(behind);
             b = base + l;
-            row = (t - before - (__shfl(upto, l, 64) - __shfl(tiles, l, 64))) * size;
+            row = (t - before - __builtin_amdgcn_readlane(upto - tiles, l)) * size;
             b = __builtin_amdgcn_readfirstlane(b);
             row = __builtin_amdgcn_readfirstlane(row);
             return true;
