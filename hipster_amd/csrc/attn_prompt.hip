@@ -52,24 +52,29 @@ __device__ __forceinline__ float swap_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The sequence and the first row in it of the t-th tile of `size` q rows (all lanes alike); false: there are fewer tiles.  The wave
-// adds up 64 sequences' tiles at a time.
-__device__ __forceinline__ bool find_tile(const int* __restrict__ cu, int n, int rows, int size, int t, int& b, int& row) {
+// The t-th tile of 128 q rows (all lanes alike): its sequence's rows q0 .. q0 + m - 1 and keys k0 .. k0 + n - 1, its first row r0 of
+// them.  false: there are fewer tiles.  The wave adds up 64 sequences' tiles at a time.
+struct Tiled { int q0, m, k0, n, r0; };
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, int t, Tiled& w) {
     const int lane = threadIdx.x & 63;
+    const int* const cuk = a.cuk ? a.cuk : a.cuq;
     int before = 0;
-    for (int base = 0; base < n; base += 64) {
+    for (int base = 0; base < a.n; base += 64) {
         const int at = base + lane;
-        int tiles = 0;
-        if (at < n) tiles = (max(within(cu[at + 1], rows) - within(cu[at], rows), 0) + size - 1) / size;
-        const int upto = (int)wave_upto((uint32_t)tiles);
+        int q0 = 0, m = 0, k0 = 0, n = 0;
+        if (at < a.n) {
+            q0 = within(a.cuq[at], a.rows);
+            m = max(within(a.cuq[at + 1], a.rows) - q0, 0);
+            k0 = within(cuk[at], a.krows);
+            n = max(within(cuk[at + 1], a.krows) - k0, 0);
+        }
+        const int tiles = (m + kRows - 1) / kRows, upto = (int)wave_upto((uint32_t)tiles);
         const unsigned long long behind = __ballot(before + upto > t);
         if (behind) {
             const int l = __builtin_ctzll(behind);
-            b = base + l;
-            row = (t - before - __builtin_amdgcn_readlane(upto - tiles, l)) * size;
-            b = __builtin_amdgcn_readfirstlane(b);
-            row = __builtin_amdgcn_readfirstlane(row);
-            return true;
+            w = {__builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(m, l), __builtin_amdgcn_readlane(k0, l), __builtin_amdgcn_readlane(n, l),
+                 __builtin_amdgcn_readfirstlane((t - before - __builtin_amdgcn_readlane(upto - tiles, l)) * kRows)};
+            return w.r0 >= 0 && w.r0 < w.m;              // false only where so many spans overlap that their tiles' count wrapped
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
@@ -95,12 +100,9 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     const uint32_t id = blockIdx.x, turn = id / (uint32_t)a.heads;
     const int h = (int)(id - turn * a.heads), hk = h / a.share;
     const int part = (int)(turn % (uint32_t)a.parts), t = a.tiles - 1 - (int)(turn / (uint32_t)a.parts);
-    int b, r0;
-    if (!find_tile(a.cuq, a.n, a.rows, kRows, t, b, r0)) return;
-    const int q0 = within(a.cuq[b], a.rows), m = within(a.cuq[b + 1], a.rows) - q0;
-    if (r0 < 0 || r0 >= m) return;                       // only where so many spans overlap that their tiles' count wrapped
-    const int* const cuk = a.cuk ? a.cuk : a.cuq;
-    const int k0 = within(cuk[b], a.krows), n = max(within(cuk[b + 1], a.krows) - k0, 0);
+    Tiled w;
+    if (!find_tile(a, t, w)) return;
+    const int q0 = w.q0, m = w.m, k0 = w.k0, n = w.n, r0 = w.r0;
     const int shift = n - m;                             // position of row 0
 
     // this lane's row
@@ -333,11 +335,11 @@ template <int D>
 __global__ void __launch_bounds__(256) k_attn_prompt_join(PromptArgs a) {
     const uint32_t id = blockIdx.x, th = id >> 2;
     const int h = (int)(th % (uint32_t)a.heads), t = (int)(th / (uint32_t)a.heads);
-    int b, r0;
-    if (!find_tile(a.cuq, a.n, a.rows, kRows, t, b, r0)) return;
-    const int q0 = within(a.cuq[b], a.rows), m = within(a.cuq[b + 1], a.rows) - q0;
+    Tiled w0;
+    if (!find_tile(a, t, w0)) return;
+    const int q0 = w0.q0, r0 = w0.r0;
     const int r = (int)(id & 3) * 32 + (threadIdx.x & 31);
-    if (r0 < 0 || r0 + r >= m) return;
+    if (r0 + r >= w0.m) return;
     const size_t at = ((size_t)t * a.heads + h) * a.parts;
     float w[kParts], top = neg_inf(), l = 0.f;
 #pragma unroll
