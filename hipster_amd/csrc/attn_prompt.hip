@@ -330,15 +330,16 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
             *(uint2*)(to + 32 * d + 8 * e) = make_uint2(mx_bf16x2(o[d][4 * e] * f, o[d][4 * e + 1] * f), mx_bf16x2(o[d][4 * e + 2] * f, o[d][4 * e + 3] * f));
 }
 
-// The parts of a tile's rows: 32 rows a workgroup, a thread one row's every eighth four dims.
+// The parts of a tile's rows: 32 rows and 32 dims a workgroup, four dims of a row a thread.
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_prompt_join(PromptArgs a) {
-    const uint32_t id = blockIdx.x, th = id >> 2;
+    constexpr int kCuts = 4 * (D / 32);                  // workgroups of a tile
+    const uint32_t th = blockIdx.x / kCuts, cut = blockIdx.x % kCuts;
     const int h = (int)(th % (uint32_t)a.heads), t = (int)(th / (uint32_t)a.heads);
     Tiled w0;
     if (!find_tile(a, t, w0)) return;
     const int q0 = w0.q0, r0 = w0.r0;
-    const int r = (int)(id & 3) * 32 + (threadIdx.x & 31);
+    const int r = (int)(cut & 3) * 32 + (threadIdx.x & 31), d = (int)(cut >> 2) * 8 + ((int)threadIdx.x >> 5);
     if (r0 + r >= w0.m) return;
     const size_t at = ((size_t)t * a.heads + h) * a.parts;
     float w[kParts], top = neg_inf(), l = 0.f;
@@ -354,24 +355,23 @@ __global__ void __launch_bounds__(256) k_attn_prompt_join(PromptArgs a) {
         }
     const float f = finish(1.f, l, top, a.sinks, h);
     uint16_t* const to = a.out + (size_t)(q0 + r0 + r) * a.ldo + (size_t)h * D;
-    for (int d = (int)threadIdx.x >> 5; d < D / 4; d += 8) {
-        mx_v4f o = {0.f, 0.f, 0.f, 0.f};
+    mx_v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 0; p < kParts; ++p)
-            if (p < a.parts && !(w[p] == 0.f)) o += w[p] * *(const mx_v4f*)(a.part + (((at + p) * (D / 4) + d) * kRows + r) * 4);
-        *(uint2*)(to + 4 * d) = make_uint2(mx_bf16x2(o[0] * f, o[1] * f), mx_bf16x2(o[2] * f, o[3] * f));
-    }
+    for (int p = 0; p < kParts; ++p)                     // a part without keys has left nothing
+        if (p < a.parts && !(w[p] == 0.f)) o += w[p] * *(const mx_v4f*)(a.part + (((at + p) * (D / 4) + d) * kRows + r) * 4);
+    *(uint2*)(to + 4 * d) = make_uint2(mx_bf16x2(o[0] * f, o[1] * f), mx_bf16x2(o[2] * f, o[3] * f));
 }
 
 // tiles of q rows of a call, at most: a sequence's last may be short
 int64_t tiles_of(int rows, int nseq) { return nseq == 1 ? ((int64_t)rows + kRows - 1) / kRows : (int64_t)rows / kRows + nseq; }
 
-// Parts that a tile's keys are cut into: one, or where that leaves half the CUs' room without work as many as fill it, of 8 tiles of
-// keys at least.
+// Parts that a tile's keys are cut into: one, or where that leaves half the CUs' room without work as many as fill it, of 16 tiles of
+// keys at least (an average row's; each part writes and reads its sums, 64 KB for 128 dims).  512 rows behind 7488 keys, 16 heads of
+// 256: one part 309 us, four 106; 1024 rows alone, 32 heads of 128, whose parts would be of 8 tiles: one 27, two 31.
 int parts_of(int rows, int krows, int nseq, int heads, int dim) {
     const int64_t work = tiles_of(rows, nseq) * heads, room = (int64_t)device_cu_count() * (dim == 256 ? 1 : 2);
-    const int64_t keys = ((int64_t)krows / nseq + kTile - 1) / kTile;
-    return (int)std::max<int64_t>(std::min<int64_t>({room / std::max<int64_t>(work, 1), keys / 8, kParts}), 1);
+    const int64_t keys = std::max<int64_t>((int64_t)krows - rows / 2, 0) / nseq / kTile;
+    return (int)std::max<int64_t>(std::min<int64_t>({room / std::max<int64_t>(work, 1), keys / 16, kParts}), 1);
 }
 
 template <int D>
@@ -382,7 +382,7 @@ int launch(PromptArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_attn_prompt<D>), dim3((unsigned)grid), dim3(64 * kWaves), kLds, s, a);
     QMM_LAUNCH_CHECK();
     if (a.parts > 1) {
-        hipLaunchKernelGGL((k_attn_prompt_join<D>), dim3((unsigned)(a.tiles * a.heads * 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_attn_prompt_join<D>), dim3((unsigned)(a.tiles * a.heads * 4 * (D / 32))), dim3(256), 0, s, a);
         QMM_LAUNCH_CHECK();
     }
     return QMM_OK;

@@ -524,9 +524,9 @@ def test_prompt_long(gpu):
 def test_prompt_keys_in_parts(gpu, D, window, sinks):
     """Few rows behind many keys: the keys are cut into parts.  A workspace of the caller's gives the bits of the one that is made; without one
     the formula holds too; one too small is refused."""
-    lens, ms, Hq, Hk = [2300, 900], [70, 20], 4, 2
+    lens, ms, Hq, Hk = [4600, 2500], [70, 20], 4, 2
     out, q, k, v, s = run_prompt(lens, ms, Hq, Hk, D, window, sinks)
-    size = qmm.attn_prompt_ws_bytes(91, 3201, 2, Hq, D)
+    size = qmm.attn_prompt_ws_bytes(91, 7101, 2, Hq, D)
     assert size > 0
     ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
     args = (q, k, v, ints(offsets(ms)), ints(offsets(lens)))
