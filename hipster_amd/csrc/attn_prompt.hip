@@ -87,7 +87,13 @@ __device__ __forceinline__ int key_turn(int r) { return D == 64 ? (r >> 1) & 7 :
 template <int D>
 __device__ __forceinline__ int val_turn(int r) { return D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
 
-__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// dma16s without a claim on memory: the compiler may move its own LDS reads past it (they are of other buffers; barriers order the rest)
+__device__ __forceinline__ void dma16q(const void* base, uint32_t voff, uint32_t lds) {
+    asm volatile(QMM_VMEM_ASM_GUARD "global_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "{m0}"(lds));
+}
+// s_waitcnt vmcnt(n): at most n of the wave's DMAs are under way
+template <int N>
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 
 template <int D>
 __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(PromptArgs a) {
@@ -132,24 +138,25 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     const uint8_t* const kbase = (const uint8_t*)(a.k + (size_t)k0 * a.ldk + (size_t)hk * D);
     const uint8_t* const vbase = (const uint8_t*)(a.v + (size_t)k0 * a.ldv + (size_t)hk * D);
     const uint32_t lds0 = lds_addr(smem);
-    // keys (or values) key0 .. + 63 into buffer `stage`, those past the last as the last
+    // Line j of the wave's of keys (VAL: of values) key0 .. + 63 into buffer `stage`, those past the last as the last.  Its rows are the
+    // wave's first ones and j * kPerLine further; where a piece lies goes by the row.
+    const int fr = wave * kLines * kPerLine + lane / kPieces, fp = lane % kPieces;
+    const uint32_t frk = (uint32_t)fr * a.ldk * 2, frv = (uint32_t)fr * a.ldv * 2;
+    auto fetch = [&](auto val, int j, int key0, int stage) {
+        constexpr bool VAL = decltype(val)::value;
+        const uint32_t ld2 = (VAL ? a.ldv : a.ldk) * 2, last_row = (uint32_t)(n - 1 - key0) * ld2;
+        const uint32_t row = min((VAL ? frv : frk) + (uint32_t)(j * kPerLine) * ld2, last_row);
+        const int turn = VAL ? val_turn<D>(fr + j * kPerLine) : key_turn<D>(fr + j * kPerLine);
+        dma16q((VAL ? vbase : kbase) + (size_t)key0 * ld2, row + (uint32_t)((fp ^ turn) * 16),
+               lds0 + ((VAL ? 2 : 0) + stage) * kBytes + (wave * kLines + j) * 1024);
+    };
     auto fetch_k = [&](int key0, int stage) {
-        const uint8_t* from = kbase + (size_t)key0 * a.ldk * 2;
 #pragma unroll
-        for (int j = 0; j < kLines; ++j) {
-            const int line = wave * kLines + j, r = line * kPerLine + lane / kPieces, p = lane % kPieces;
-            dma16s(from, (uint32_t)min(r, n - 1 - key0) * a.ldk * 2 + (uint32_t)((p ^ key_turn<D>(r)) * 16),
-                   __builtin_amdgcn_readfirstlane(lds0 + stage * kBytes + line * 1024));
-        }
+        for (int j = 0; j < kLines; ++j) fetch(std::false_type{}, j, key0, stage);
     };
     auto fetch_v = [&](int key0, int stage) {
-        const uint8_t* from = vbase + (size_t)key0 * a.ldv * 2;
 #pragma unroll
-        for (int j = 0; j < kLines; ++j) {
-            const int line = wave * kLines + j, r = line * kPerLine + lane / kPieces, p = lane % kPieces;
-            dma16s(from, (uint32_t)min(r, n - 1 - key0) * a.ldv * 2 + (uint32_t)((p ^ val_turn<D>(r)) * 16),
-                   __builtin_amdgcn_readfirstlane(lds0 + (2 + stage) * kBytes + line * 1024));
-        }
+        for (int j = 0; j < kLines; ++j) fetch(std::true_type{}, j, key0, stage);
     };
     // addresses of operands within a tile
     constexpr int KA = D == 64 ? 4 : 8, VA = D == 64 ? 2 : 4;
@@ -171,7 +178,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     mx_v16f o[DT], sc[2];
     float mx, ls, raw;                                   // raw: the largest of sc, unmasked
     // scores of the tile in key buffer `stage`
-    auto scores = [&](int stage, mx_v16f (&to)[2]) {
+    auto scores = [&](int stage, mx_v16f (&to)[2], auto between) {
         const uint8_t* const ks = smem + stage * kBytes;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -181,6 +188,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
             for (int s = 0; s < S; ++s) {
                 const at_bf8 kf = *(const at_bf8*)(ks + ka[s % KA] + u * 32 * kRow + (s / KA) * 256);
                 to[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], to[u], 0, 0, 0);
+                between(u * S + s);
             }
         }
     };
@@ -216,7 +224,12 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
         }
         const float base = mx == neg_inf() ? 0.f : mx;
         mx_v16f sn[2];
-        if constexpr (NEXT) scores(stage ^ 1, sn);
+        // between the products the DMAs of K(kt + 2), into this tile's keys' buffer, and below of V(kt + 1): the CU takes in 64 bytes a
+        // cycle, and what is issued faster holds the wave up
+        if constexpr (NEXT)
+            scores(stage ^ 1, sn, [&](int i) {
+                if (i % (2 * S / kLines) == 0) fetch(std::false_type{}, i / (2 * S / kLines), min(kt + 2, t1) * kTile, stage);
+            });
         at_bf8 pf[4];
         float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -226,6 +239,10 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
             pf[e / 8][e % 8] = (__bf16)p;
         }
         ls += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if constexpr (NEXT) {
+            wait_dma<kLines>();
+            lds_barrier();                               // V(kt) is there (K(kt + 2) need not be)
+        }
         const uint8_t* const vs = smem + (2 + stage) * kBytes;
         bool odd = false;
 #pragma unroll
@@ -247,6 +264,9 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
                     vf = __builtin_bit_cast(at_bf8, w);
                 }
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], o[d], 0, 0, 0);
+                const int i = s * DT + d;
+                if constexpr (NEXT)
+                    if (i % (4 * DT / kLines) == 0) fetch(std::true_type{}, i / (4 * DT / kLines), (kt + 1) * kTile, stage ^ 1);
             }
         if constexpr (SAFE) {
             if (__ballot(odd))                           // they reach the rows that see their key, and no other
@@ -279,21 +299,18 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
         if (t0 > t1) return;
         fetch_k(t0 * kTile, 0);
+        fetch_k(min(t0 + 1, t1) * kTile, 1);             // past the last tile it is asked for again: as many are under way at every wait
         fetch_v(t0 * kTile, 0);
-        if (t0 < t1) fetch_k((t0 + 1) * kTile, 1);
-        wait_dma();
-        lds_barrier();
-        scores(0, sc);
+        wait_dma<2 * kLines>();
+        lds_barrier();                                   // K(t0) is there
+        scores(0, sc, [](int) {});
         raw = row_max(sc);
         for (int kt = t0; kt < t1; ++kt) {
-            const int stage = (kt - t0) & 1;
-            wait_dma();
-            lds_barrier();                               // K(kt + 1) and V(kt) are there, and all are done with K(kt) and V(kt - 1)
-            if (kt + 1 < t1) fetch_k((kt + 2) * kTile, stage);
-            fetch_v((kt + 1) * kTile, stage ^ 1);
-            tile(kt, stage, std::true_type{}, safe);
+            wait_dma<kLines>();
+            lds_barrier();                               // K(kt + 1) is there, and all are done with K(kt) and V(kt - 1)
+            tile(kt, (kt - t0) & 1, std::true_type{}, safe);
         }
-        wait_dma();
+        wait_dma<0>();
         lds_barrier();
         tile(t1, (t1 - t0) & 1, std::false_type{}, safe);
     };
