@@ -104,7 +104,9 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
 
     // the last tiles first: they see the most keys
     const uint32_t id = blockIdx.x, turn = id / (uint32_t)a.heads;
-    const int h = (int)(id - turn * a.heads), hk = h / a.share;
+    // Successive workgroups run on successive dies of eight, each with a cache of its own: a die gets successive heads, which share keys
+    // and values.
+    const int i8 = (int)(id - turn * a.heads), h = a.heads % 8 ? i8 : (i8 % 8) * (a.heads / 8) + i8 / 8, hk = h / a.share;
     const int part = (int)(turn % (uint32_t)a.parts), t = a.tiles - 1 - (int)(turn / (uint32_t)a.parts);
     Tiled w;
     if (!find_tile(a, t, w)) return;
@@ -232,17 +234,21 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
             });
         at_bf8 pf[4];
         float sums[4] = {0.f, 0.f, 0.f, 0.f};
+        auto weights = [&](int u) {                      // of 32 of the tile's keys
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 16][e % 16], a.scale, -base));
-            sums[e % 4] += p;
-            pf[e / 8][e % 8] = (__bf16)p;
-        }
-        ls += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][e], a.scale, -base));
+                sums[e % 4] += p;
+                pf[2 * u + e / 8][e % 8] = (__bf16)p;
+            }
+        };
+        // half of the weights beside the next tile's scores, half beside the first half of the values' product
+        weights(0);
         if constexpr (NEXT) {
             wait_dma<kLines>();
             lds_barrier();                               // V(kt) is there (K(kt + 2) need not be)
         }
+        weights(1);
         const uint8_t* const vs = smem + (2 + stage) * kBytes;
         bool odd = false;
 #pragma unroll
@@ -268,6 +274,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
                 if constexpr (NEXT)
                     if (i % (4 * DT / kLines) == 0) fetch(std::true_type{}, i / (4 * DT / kLines), (kt + 1) * kTile, stage ^ 1);
             }
+        ls += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         if constexpr (SAFE) {
             if (__ballot(odd))                           // they reach the rows that see their key, and no other
                 for (int key = max(key0, wave_lo); key <= min(key0 + kTile - 1, wave_last); ++key) {
