@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     const uint32_t frk = (uint32_t)fr * a.ldk * 2, frv = (uint32_t)fr * a.ldv * 2;
     auto fetch = [&](auto val, int j, int key0, int stage) {
         constexpr bool VAL = decltype(val)::value;
-        const uint32_t ld2 = (VAL ? a.ldv : a.ldk) * 2, last_row = (uint32_t)(n - 1 - key0) * ld2;
+        const uint32_t ld2 = (VAL ? a.ldv : a.ldk) * 2, last_row = (uint32_t)min(n - 1 - key0, kTile - 1) * ld2;
         const uint32_t row = min((VAL ? frv : frk) + (uint32_t)(j * kPerLine) * ld2, last_row);
         const int turn = VAL ? val_turn<D>(fr + j * kPerLine) : key_turn<D>(fr + j * kPerLine);
         dma16q((VAL ? vbase : kbase) + (size_t)key0 * ld2, row + (uint32_t)((fp ^ turn) * 16),

@@ -303,11 +303,13 @@ def test_attend_rows_that_see_nothing(gpu):
 
 
 @pytest.mark.parametrize("D,Hq,Hk", [(64, 8, 2), (128, 4, 1), (256, 8, 1), (128, 12, 1)])
-@pytest.mark.parametrize("qt", ["bf16", "f32"])
-def test_attend_rows_do_not_depend_on_each_other(gpu, D, Hq, Hk, qt):
+@pytest.mark.parametrize("qt,ml", [("bf16", 600), ("f32", 600), ("bf16", 3000), ("f32", 3000)])
+def test_attend_rows_do_not_depend_on_each_other(gpu, D, Hq, Hk, qt, ml):
     """Drafted rows checked together are the bits that one after the other gives, and other sequences change nothing."""
     g = torch.Generator().manual_seed(7)
-    lens, ms, ml = [530, 40, 270], [6, 1, 3], 600
+    lens, ms = [530, 40, 270], [6, 1, 3]
+    if ml > 600:                                         # several chunks, some rows' last key the first of one
+        lens = [1540, 40, 513]
     out, kv, table, q, _ = attend(g, lens, ms, Hq, Hk, D, 32, qt, qt, max_len=ml)
     at = offsets(ms)
     for b, (n, m) in enumerate(zip(lens, ms)):
@@ -506,6 +508,23 @@ def test_prompt_offsets_that_lead_out(gpu):
         got = torch.full_like(out, 3.0)
         qmm.attn_prompt_bf16(q[:50], k[:50], v[:50], ints(cu), None, got[:50], 2, 1, 64)
         assert torch.equal(got[:50], out[:50]) if cu in ([0, 1000], [-5, 51]) else (got == 3).all()
+
+
+def test_prompt_rows_far_apart(gpu):
+    """Keys and values whose rows lie beyond 2^32 bytes of the first one."""
+    n, ld, D = 61000, 40000, 64
+    far = torch.empty((n, ld), dtype=torch.bfloat16, device="cuda")
+    k, v = far[:, :D], far[:, ld - D:]
+    g = torch.Generator().manual_seed(30)
+    k.copy_(torch.randn(n, D, generator=g))
+    v.copy_(torch.randn(n, D, generator=g))
+    q = torch.randn(3, D, generator=g).bfloat16().cuda()
+    for ws in (None, False):
+        out = torch.empty_like(q)
+        qmm.attn_prompt_bf16(q, k, v, ints([0, 3]), ints([0, n]), out, 1, 1, D, ws=ws)
+        qh, kh, vh = (host(t).astype(np.float64) for t in (q, k, v))
+        want, bound = attn_ref.attention(qh, kh, vh, [n - 3, n - 2, n - 1], D ** -0.5, 0, None, D // 16 + 1, 2.0 ** -8, n / 16 + 4)
+        assert (np.abs(host(out) - want) <= bound + 2.0 ** -8 * np.abs(want)).all()
 
 
 def test_prompt_long(gpu):
