@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
     const int c_end = min(at_unit.chunks - c_off, (int)(end - unit));        // units of this group here
     unit += (uint32_t)c_end;
     const int c_first = at_unit.first + c_off;
+    const SeqSpan q = at_unit.q;
     if (unit < end) at_unit = locate<NT>(a, unit);       // the next group's
 
-    const SeqSpan q = at_unit.q;
     const int m = min(q.m, a.max_rows);                  // rows of this call
     const int f0 = group * 16 * NT, fn = min(m * a.share - f0, 16 * NT);     // the group's first (token, head), and how many
     const int first_pos = q.len - q.m;

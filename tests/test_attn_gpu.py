@@ -225,24 +225,27 @@ def attend(g, lens, ms, Hq, Hk, D, page, qt="bf16", ot="bf16", window=0, sinks=F
     return out, kv, table, q, s
 
 
-def gather(kv, table, b, n, h):
-    """float64 keys and values of head h of sequence b."""
-    out = []
-    for x in "kv":
-        p = np.arange(n)
-        pg, at = table[b].cpu().numpy()[p // kv.page], p % kv.page
-        out.append(attn_ref.values(getattr(kv, x + "q").cpu().numpy()[pg, h, at], getattr(kv, x + "e").cpu().numpy()[pg, h, at]))
-    return out
+def fetched(kv, table):
+    """The cache and the table on the host."""
+    return {x: getattr(kv, x).cpu().numpy() for x in ("kq", "ke", "vq", "ve")} | {"table": table.cpu().numpy(), "page": kv.page}
+
+
+def gather(c, b, n, h):
+    """float64 keys and values of head h of sequence b, of a fetched cache."""
+    p = np.arange(n)
+    pg, at = c["table"][b][p // c["page"]], p % c["page"]
+    return [attn_ref.values(c[x + "q"][pg, h, at], c[x + "e"][pg, h, at]) for x in "kv"]
 
 
 def check_attend(out, kv, table, q, s, lens, ms, Hq, Hk, D, qt, ot, window, scale=None, max_rows=16):
     got, qh = host(out).reshape(-1, Hq, D), host(q).astype(np.float64).reshape(-1, Hq, D)
-    wide = "f32" in (qt, ot)
+    wide, c = "f32" in (qt, ot), fetched(kv, table)
     r = 0
     for b, (n, m) in enumerate(zip(lens, ms)):
-        for h in range(Hq):
-            k, v = gather(kv, table, b, n, h // (Hq // Hk))
-            mm = min(m, max_rows)
+        mm = min(m, max_rows)
+        for h in range(Hq if mm else 0):
+            if h % (Hq // Hk) == 0:
+                k, v = gather(c, b, n, h // (Hq // Hk))
             want, bound = attn_ref.attention(qh[r:r + mm, h], k, v, n - m + np.arange(mm), D ** -0.5 if scale is None else scale, window,
                                              None if s is None else float(s[h]), D // 32 * (3 if wide else 1) + 1, 2.0 ** -16 if wide else 2.0 ** -8, 24)
             err = np.abs(got[r:r + mm, h] - want)
@@ -287,6 +290,16 @@ def test_attend_many_chunks(gpu):
         check_attend(far, kv, table, q, s, lens, ms, 2, 1, 64, "bf16", "bf16", 0)
 
 
+@pytest.mark.parametrize("D,B,m,Hq,Hk,window", [(64, 70, 1, 8, 8, 0), (128, 45, 1, 16, 8, 0), (256, 40, 2, 8, 8, 0), (128, 100, 3, 24, 4, 700), (64, 90, 2, 40, 4, 0)])
+def test_attend_more_units_than_workgroups(gpu, D, B, m, Hq, Hk, window):
+    """Workgroups that go from one sequence and head to the next, more sequences than a wave has lanes among them."""
+    g = torch.Generator().manual_seed(B)
+    lens = [1030 + (i * 211) % 1018 for i in range(B)]
+    ms = [m if i % 7 else 0 for i in range(B)]
+    out, kv, table, q, s = attend(g, lens, ms, Hq, Hk, D, 64, window=window, max_len=2048)
+    check_attend(out, kv, table, q, s, lens, ms, Hq, Hk, D, "bf16", "bf16", window)
+
+
 def test_attend_rows_that_see_nothing(gpu):
     """Positions below 0: zeros, with and without a sink; keys beyond max_len are not seen."""
     g = torch.Generator().manual_seed(6)
@@ -297,7 +310,7 @@ def test_attend_rows_that_see_nothing(gpu):
         check_attend(out, kv, table, q, s, lens, ms, 4, 2, 64, "bf16", "bf16", 0)
     for window in (0, 4):                                                       # max_len 8: 8 keys of 20, or none of the window's
         cut, *_ = attend(g, [20], [1], 4, 2, 64, 16, kv=kv, table=table[1:], q=q, max_len=8, window=window, extra=0)
-        k, v = gather(kv, table, 1, 8, 0)
+        k, v = gather(fetched(kv, table), 1, 8, 0)
         want, bound = attn_ref.attention(host(q).astype(np.float64)[:1, 0], k, v, [19], 0.125, window, None, 3, 2.0 ** -8, 24)
         assert (np.abs(host(cut)[0, :64] - want) <= bound + 2.0 ** -8 * np.abs(want)).all()
 
@@ -621,7 +634,7 @@ def check_block(s):
     r = 0
     for b, (n, m) in enumerate(zip(s["l"], s["m"])):
         for h in range(s["Hq"]):
-            k, v = gather(s["kv"], s["table"], b, n, h // 4)
+            k, v = gather(fetched(s["kv"], s["table"]), b, n, h // 4)
             want, bo = attn_ref.attention(q[r:r + m, h], k, v, n - m + np.arange(m), s["D"] ** -0.5, 0, None, 9, 2.0 ** -8, n / 16 + 24)
             err = np.abs(host(s["out"])[r:r + m].reshape(m, s["Hq"], s["D"])[:, h] - want)
             assert (err <= bo + 2.0 ** -8 * np.abs(want)).all(), (b, h)
