@@ -42,20 +42,30 @@ __device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
     return v;
 }
 
-// The sequence that row r (the same in all lanes) belongs to, -1: none.  The wave compares 64 offsets at a time, so that up to 64
-// sequences cost one load's latency.
-__device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, int n, int r) {
+// The sequence that row r (the same in all lanes) belongs to and its span, -1: none.  The wave looks at 64 sequences at a time, so that
+// up to 64 cost one load's latency.
+__device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, const int* __restrict__ lens, int n, int rows, int r, SeqSpan& q) {
     const int lane = threadIdx.x & 63;
-    int b = -1;
+    int b = -1, from = 0, to = 0, len = 0;               // of the last sequence that begins at r or before it
     for (int base = 0; base < n; base += 64) {
         const int at = base + lane;
-        const int c = at < n ? cu[at] : 0x7fffffff;
-        const int below = __popcll(__ballot(c <= r));
-        if (below) b = base + below - 1;
+        int c0 = 0x7fffffff, c1 = 0, c2 = 0;
+        if (at < n) { c0 = cu[at]; c1 = cu[at + 1]; c2 = lens[at]; }
+        const int below = __popcll(__ballot(at < n && c0 <= r));
+        if (below) {
+            const int l = below - 1;
+            b = base + l;
+            from = __builtin_amdgcn_readlane(c0, l);
+            to = __builtin_amdgcn_readlane(c1, l);
+            len = __builtin_amdgcn_readlane(c2, l);
+        }
         if (below < 64) break;
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    return b >= 0 && r < cu[b + 1] && r >= cu[b] ? b : -1;
+    if (b < 0 || r >= to || r < from) return -1;
+    const int r0 = within(from, rows);
+    q = {r0, max(within(to, rows) - r0, 0), max(len, 0)};
+    return b;
 }
 
 // ---- softmax, in powers of two ----

@@ -537,9 +537,8 @@ __global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
     __shared__ float s_w[kChunks];
     const int lane = threadIdx.x;
     const uint32_t rh = blockIdx.x / P, part = blockIdx.x % P, row = rh / (uint32_t)a.heads, h = rh - row * a.heads;
-    const int b = seq_of_row(a.s.cu, a.s.n, (int)row);
-    if (b < 0) return;
-    const SeqSpan q = seq_span(a.s.cu, a.s.lens, b, a.rows);
+    SeqSpan q;
+    if (seq_of_row(a.s.cu, a.s.lens, a.s.n, a.rows, (int)row, q) < 0) return;
     const int i = (int)row - q.r0;
     if (i < 0 || i >= min(q.m, a.max_rows)) return;
     const Sight st = sight(a, q.len - q.m + i);

@@ -24,9 +24,9 @@ struct KvArgs {
 
 // Row, page (-1: outside the cache) and place in it of a wave's row; false: the row has no place
 __device__ __forceinline__ bool place(const KvArgs& a, int row, int& page, int& at) {
-    const int b = seq_of_row(a.s.cu, a.s.n, row);
+    SeqSpan q;
+    const int b = seq_of_row(a.s.cu, a.s.lens, a.s.n, a.rows, row, q);
     if (b < 0) return false;
-    const SeqSpan q = seq_span(a.s.cu, a.s.lens, b, a.rows);
     const int pos = q.len - q.m + (row - q.r0);
     if (pos < 0 || (pos >> a.lg) >= a.s.ld) return false;
     page = a.s.table[(size_t)b * a.s.ld + (pos >> a.lg)];
