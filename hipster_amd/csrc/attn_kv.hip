@@ -585,8 +585,11 @@ __global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
     if (g == 0) put4(a, (size_t)row * a.ldo + (size_t)h * D + part * 64 + d, o * f);
 }
 
-// keys of a chunk, a power of two: 1024 make one chunk, which needs no join (700 keys of one sequence: CHUNKONE µs, as three
-// chunks of 256 11.3); beyond, 256, or as many as make 128 chunks
+// Keys of a chunk, a power of two.  Up to 1024 keys are one chunk, which needs no join (700 keys of one sequence: 9.2 µs, as three chunks of
+// 256 9.9).  Beyond, short chunks spread few sequences over the device and long ones have less to join; in µs with chunks of 256, 512, 1024:
+//   1 sequence of 2000 keys     9.9  12.1  16.5        1 of 30000 keys     19.7  16.8  18.8
+//   16 of 2000                 14.1  15.7  18.3        32 of 8000 to 500   49.9  47.0  44.5
+//   1 of 8000                  10.4  12.2  16.4        16 of 32000          120   111   107
 int chunk_of(int max_len) {
     if (max_len <= 1024) return 1024;
     int c = max_len <= 2048 ? 256 : 512;
@@ -595,12 +598,16 @@ int chunk_of(int max_len) {
 }
 int chunks_of(int max_len) { return (max_len + chunk_of(max_len) - 1) / chunk_of(max_len); }
 
+// units of work at most, and the workgroups that are resident at once
+uint64_t units_of(const AttnArgs& a, int nt) { return (uint64_t)a.s.n * a.kv.heads * ((a.max_rows * a.share + 16 * nt - 1) / (16 * nt)) * a.chunks; }
+uint64_t resident(int D, int NT, bool wide, int nw) { return (uint64_t)device_cu_count() * (occupancy(D, NT, wide) * 4 / nw); }
+
 template <int D, int NT, bool WIDE, int NW>
 int launch(AttnArgs& a, hipStream_t s) {
     a.groups = (a.max_rows * a.share + 16 * NT - 1) / (16 * NT);
-    const uint64_t most = (uint64_t)a.s.n * a.kv.heads * a.groups * a.chunks, joins = (uint64_t)a.rows * a.heads * (D / 64);
+    const uint64_t most = units_of(a, NT), joins = (uint64_t)a.rows * a.heads * (D / 64);
     if (most > 0x7fffffff) return QMM_ERR_SHAPE;
-    const uint64_t grid = std::min<uint64_t>(most, (uint64_t)device_cu_count() * (occupancy(D, NT, WIDE) * 4 / NW));     // all resident
+    const uint64_t grid = std::min(most, resident(D, NT, WIDE, NW));
     if (!grid_fits(grid, 64 * NW) || !grid_fits(joins, 64)) return QMM_ERR_SHAPE;
     hipLaunchKernelGGL((k_attn_kv<D, NT, WIDE, NW>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
     QMM_LAUNCH_CHECK();
@@ -611,19 +618,28 @@ int launch(AttnArgs& a, hipStream_t s) {
     return QMM_OK;
 }
 
-// Waves of a workgroup: four; eight where the keys are one chunk (few workgroups, whose own time counts) and two waves of the kernel
-// share a SIMD.
+// Waves of a workgroup: four; eight where the keys are one chunk (few workgroups, whose own time counts) and registers leave room for two
+// waves a SIMD.  A row's bits follow from it, so this must not go by NT, which goes by the rows of a call.
+constexpr bool eight(int D, bool wide) { return D < 256 || !wide; }
 template <int D, int NT, bool WIDE>
 int launch(AttnArgs& a, hipStream_t s) {
-    if constexpr (occupancy(D, NT, WIDE) >= 2)
+    if constexpr (eight(D, WIDE)) {
+        static_assert(occupancy(D, NT, WIDE) >= 2, "");
         if (a.chunks == 1) return launch<D, NT, WIDE, 8>(a, s);
+    }
     return launch<D, NT, WIDE, 4>(a, s);
 }
 
-// rows of a group: 16, 32, 48 or 64, what covers a sequence's; fewer where operands and sums would not fit 256 registers
+// Rows of a group: 16, 32, 48 or 64, what covers a sequence's, so that the cache is read and converted once; fewer where operands and sums
+// would not fit 256 registers, and 16 where the units that this makes are all resident at once (then a workgroup's own time counts).  In
+// µs, groups of 16 rows and of more:
+//   dim 64, 40 rows a kv head, 8 kv heads: 1 sequence of 700 keys  8.2  12.7,  16 of 700  10.4  13.0,  1 of 8000  12.6  14.1,
+//                                          4 of 8000  25.4  19.3,  1 of 30000  25.0  20.1,  16 of 8000 to 500  47.8  40.4
+//   dim 128, 32 rows, 4 kv heads:          1 of 8000  12.9  15.3,  4 of 8000  17.1  17.4,  32 of 32000 to 2000  185  146
 template <int D>
 int launch_rows(AttnArgs& a, bool wide, hipStream_t s) {
-    const int f = a.max_rows * a.share;
+    int f = a.max_rows * a.share;
+    if (units_of(a, 1) <= resident(D, 1, wide, a.chunks == 1 && eight(D, wide) ? 8 : 4)) f = 16;
     if (f <= 16 || D == 256 || (wide && D == 128)) return wide ? launch<D, 1, true>(a, s) : launch<D, 1, false>(a, s);
     if constexpr (D == 64)
         if (wide && (f > 32 && f <= 48)) return launch<D, 3, true>(a, s);

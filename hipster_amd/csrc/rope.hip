@@ -182,9 +182,10 @@ extern "C" int qmm_rope_axes(const void* x, int dtype, size_t ldx, void* out, in
     const int V = vec ? 4 : 1;
     a.turned = (uint32_t)(rope->pairs / V);
     a.units = a.turned + (uint32_t)((dim - 2 * rope->pairs + 2 * V - 1) / (2 * V));
-    // 8 heads a thread where that still leaves four waves a SIMD (2^18 threads), else fewer, down to one
+    // 8 heads a thread where that still leaves two waves a SIMD (2^17 threads), else fewer, down to one.  40 heads of 128 in µs, one head a
+    // thread and eight: 64 tokens 3.5 and 4.5, 2048 tokens 24 and 9.5
     a.per = 8;
-    while (a.per > 1 && (uint64_t)rows * ((heads + a.per - 1) / a.per) * a.units < (1u << 18)) a.per >>= 1;
+    while (a.per > 1 && (uint64_t)rows * ((heads + a.per - 1) / a.per) * a.units < (1u << 17)) a.per >>= 1;
     a.groups = (uint32_t)((heads + a.per - 1) / a.per);
     const uint64_t items = (uint64_t)rows * a.groups * a.units;
     if (items > 0xffffffffu - kThreads) return QMM_ERR_SHAPE;

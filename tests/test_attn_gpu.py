@@ -300,6 +300,27 @@ def test_attend_more_units_than_workgroups(gpu, D, B, m, Hq, Hk, window):
     check_attend(out, kv, table, q, s, lens, ms, Hq, Hk, D, "bf16", "bf16", window)
 
 
+@pytest.mark.parametrize("D,Hk,share,m", [(64, 2, 8, 3), (64, 2, 8, 5), (64, 2, 7, 9), (64, 2, 10, 8), (64, 2, 8, 16), (128, 2, 8, 3), (128, 2, 5, 13), (256, 2, 8, 4)])
+@pytest.mark.parametrize("qt", ["bf16", "f32"])
+@pytest.mark.parametrize("chunks", [1, 118])
+def test_attend_groups_of_many_rows(gpu, D, Hk, share, m, qt, chunks):
+    """More units than are resident at once: groups of more than 16 rows, with the bits that a sequence by itself gives in groups of 16."""
+    g = torch.Generator().manual_seed(m + D)
+    if chunks == 1:
+        lens, max_len = [1 + (i * 37) % 61 for i in range(140)], 1000
+    else:
+        lens, max_len = [530, 40, 1270], 512 * chunks
+    ms = [m if i % 3 == 0 else 1 + i % m for i in range(len(lens))]
+    Hq = Hk * share
+    out, kv, table, q, s = attend(g, lens, ms, Hq, Hk, D, 32, qt, qt, 0, True, max_len=max_len)
+    at = offsets(ms)
+    for b in range(0, len(lens), 1 if chunks > 1 else 9):
+        lone, *_ = attend(g, [lens[b]], [ms[b]], Hq, Hk, D, 32, qt, qt, 0, s, max_len=max_len, max_rows=m, kv=kv, table=table[b:b + 1],
+                          q=q[at[b]:at[b + 1]], extra=0)
+        assert torch.equal(lone, out[at[b]:at[b + 1]]), b
+        check_attend(lone, kv, table[b:b + 1], q[at[b]:at[b + 1]], s, [lens[b]], [ms[b]], Hq, Hk, D, qt, qt, 0)
+
+
 def test_attend_rows_that_see_nothing(gpu):
     """Positions below 0: zeros, with and without a sink; keys beyond max_len are not seen."""
     g = torch.Generator().manual_seed(6)
