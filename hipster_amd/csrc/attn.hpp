@@ -8,6 +8,7 @@ typedef __bf16 at_bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 at_bf8 __attribute__((ext_vector_type(8)));
 typedef short at_s4 __attribute__((ext_vector_type(4)));
 
+constexpr uint32_t kMxNan = 253;                         // scale bytes from here on: 255 is NaN, 253 and 254 hold values that bf16 does not
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xff800000u); }
 
@@ -99,6 +100,7 @@ inline int kv_check(const qmm_kv_mxfp4* kv, const qmm_seqs* s, int* lg) {
 inline int attn_check(const qmm_attn* a) {
     if (!a) return QMM_ERR_NULL;
     if (a->window < 0) return QMM_ERR_SHAPE;
+    if (!(a->scale >= -0x1p100f && a->scale <= 0x1p100f)) return QMM_ERR_ARG;          // times log2(e) it is finite; NaN
     return aligned(a->sinks, 4) ? QMM_OK : QMM_ERR_ARG;
 }
 

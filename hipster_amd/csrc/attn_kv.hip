@@ -186,6 +186,10 @@ struct Tile {
     uint32_t e[S];
     __device__ __forceinline__ uint32_t word(int w) const { return c[w / V][w % V]; }
     __device__ __forceinline__ float scale(int w) const { return __uint_as_float(e[w / V] << 23); }
+    __device__ __forceinline__ void nan_out() {          // what counts as NaN to NaN
+#pragma unroll
+        for (int i = 0; i < S; ++i) e[i] = e[i] >= kMxNan ? 255 : e[i];
+    }
     __device__ __forceinline__ void clear(int i) {       // to values of 0
         c[i] = Codes(0);
         e[i] = 127;
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
             }
 #pragma unroll
             for (int i = 0; i < Tile<D>::S; ++i) {
-                nan[t][i] = __ballot(st.v[t].e[i] == 255);
+                nan[t][i] = __ballot(st.v[t].e[i] >= kMxNan);
                 any |= nan[t][i];
             }
         }
@@ -361,8 +365,10 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < Tile<D>::S; ++i)
-                    if (st.v[t].e[i] == 255) st.v[t].clear(i);
+                    if (st.v[t].e[i] >= kMxNan) st.v[t].clear(i);
         }
+        st.k[0].nan_out();
+        st.k[1].nan_out();
         if (st.bad[0] || st.bad[1]) {                    // scores of NaN for the rows that see these keys
 #pragma unroll
             for (int t = 0; t < 2; ++t)

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     if (a.parts > 1) {
         const size_t at = ((size_t)t * a.heads + h) * a.parts + part;
         const int r = 32 * wave + col;
-        if (kg == 0) a.ml[at * kRows + r] = make_float2(mx, ls);
+        if (kg == 0) a.ml[at * kRows + r] = make_float2(mx, t0 > t1 ? -1.f : ls);            // -1: no keys, and nothing behind it
         if (t0 > t1) return;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -374,15 +374,15 @@ __global__ void __launch_bounds__(256) k_attn_prompt_join(PromptArgs a) {
     for (int p = 0; p < kParts; ++p)
         if (p < a.parts) {
             const float2 v = a.ml[(at + p) * kRows + r];
-            w[p] = weight(v.x, top);
-            l += w[p] * v.y;
+            w[p] = v.y < 0.f ? -1.f : weight(v.x, top);
+            l += v.y < 0.f ? 0.f : w[p] * v.y;
         }
     const float f = finish(1.f, l, top, a.sinks, h);
     uint16_t* const to = a.out + (size_t)(q0 + r0 + r) * a.ldo + (size_t)h * D;
     mx_v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int p = 0; p < kParts; ++p)                     // a part without keys has left nothing
-        if (p < a.parts && !(w[p] == 0.f)) o += w[p] * *(const mx_v4f*)(a.part + (((at + p) * (D / 4) + d) * kRows + r) * 4);
+    for (int p = 0; p < kParts; ++p)                     // a part without keys has left nothing; one without weight may have left NaN
+        if (p < a.parts && !(w[p] < 0.f)) o += w[p] * *(const mx_v4f*)(a.part + (((at + p) * (D / 4) + d) * kRows + r) * 4);
     *(uint2*)(to + 4 * d) = make_uint2(mx_bf16x2(o[0] * f, o[1] * f), mx_bf16x2(o[2] * f, o[3] * f));
 }
 

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_read(void* __restrict__ k, v
         const bool val = cc >= C;
         const int c = val ? cc - C : cc;
         // the conversion reads the scale's exponent field: 2^(byte - 127), 255 NaN
-        const float s = __uint_as_float((page < 0 ? 255u : byte[i]) << 23);
+        const float s = __uint_as_float((page < 0 || byte[i] >= kMxNan ? 255u : byte[i]) << 23);
         uint32_t w[4];                                   // two significant bits: exact in bf16
         w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], s, 0));
         w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[i], s, 1));

@@ -641,6 +641,9 @@ class KVMXBuf:
             object.__setattr__(self, "held", None)
         object.__setattr__(self, name, value)
 
+    def __getstate__(self):                              # copies check anew
+        return {**self.__dict__, "held": None}
+
     def c(self):
         return KVMX(self.kq.data_ptr(), self.ke.data_ptr(), self.vq.data_ptr(), self.ve.data_ptr(), self.pages, self.page, self.heads, self.dim)
 
@@ -788,9 +791,8 @@ def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None,
     if ws is None:
         size = L.qmm_attn_prompt_ws_bytes(rows, krows, n, heads, dim)
         if size:
-            ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-            if stream is not None:
-                ws.record_stream(stream)
+            with torch.cuda.stream(stream):              # of that stream's memory: what this one still uses is not given away
+                ws = torch.empty(size, dtype=torch.uint8, device=q.device)
     pw, size = (_at(ws, 0, torch.uint8, dev, "ws"), ws.numel()) if ws is not None and ws is not False else (None, 0)
     check(L.qmm_attn_prompt_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _at(cu_q, n + 1, torch.int32, dev, "cu_q"),
                                  None if cu_k is None else _at(cu_k, n + 1, torch.int32, dev, "cu_k"), n, _attn(scale, dim, window, sinks, heads, dev),

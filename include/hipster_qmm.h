@@ -101,13 +101,14 @@ typedef struct { const void* g; size_t ld; int32_t dtype, act, per_value; } qmm_
 
 /* a cache of keys and values in MXFP4, in pages of `page` tokens (a power of two, 16 .. 4096): codes kq, vq [pages][heads][page][dim / 2]
  * (value 2i in the low half of byte i), scale bytes ke, ve [pages][heads][page][dim / 32]; dim 64, 128 or 256.  kq and vq are
- * 16-byte aligned, ke and ve 8-byte. */
+ * 16-byte aligned, ke and ve 8-byte.  The scale bytes 253 and 254, whose values bf16 does not hold and which no call here writes, stand for
+ * NaN as 255 does. */
 typedef struct { uint8_t* kq; uint8_t* ke; uint8_t* vq; uint8_t* ve; int32_t pages, page, heads, dim; } qmm_kv_mxfp4;
 /* the n sequences of a call, all on the device: rows cu[b] .. cu[b + 1] - 1 of the call's row tensors are the last ones of sequence b,
  * which has lens[b] tokens with them: of m rows, row i is the token at position lens[b] - m + i.  Token p is in the cache at
  * page table[b * ld + p / page], place p % page. */
 typedef struct { const int32_t* cu; const int32_t* lens; const int32_t* table; int32_t n, ld; } qmm_seqs;
-/* how far and how a row of attention sees: score = scale * q . k; keys of the positions (p - window, p] (window 0: all up to p); sinks
+/* how far and how a row of attention sees: score = scale * q . k (|scale| at most 2^100); keys of the positions (p - window, p] (window 0: all up to p); sinks
  * [heads of q] f32 or NULL: a logit per head that takes part in the softmax and has no value */
 typedef struct { const float* sinks; float scale; int32_t window; } qmm_attn;
 /* rotary positions: pair i < pairs of a head turns by pos[axis[i] * ldp + t] * freq[i] (pos int32 [axes][ldp], axis NULL: axis 0 for all);
@@ -496,7 +497,7 @@ int qmm_postnorm_add_rmsnorm_mxfp4(const float* x, const void* y, int y_dtype, s
  * A call for no rows does nothing and needs no buffers. */
 /* x [rows][heads][dim] (row stride ldx values, a row's heads one after the other) -> out, f32 or bf16 each, out = x allowed where types
  * and strides are the same.  dim <= 1024, 2 * pairs <= dim, axes <= 255, values from 2 * pairs on are copied.  The angle is exact
- * before its reduction, whatever the position; its sine and cosine are within 2^-22. */
+ * before its reduction, and its sine and cosine are within 2^-22, for |pos * freq| up to 2^50. */
 int qmm_rope_axes(const void* x, int dtype, size_t ldx, void* out, int out_dtype, size_t ldo, const qmm_rope* rope, int rows, int heads, int dim,
                   void* stream);
 /* k and v [rows][heads][dim] (f32 or bf16, row strides ldk, ldv) -> their sequences' places in the cache, the codes that
@@ -504,10 +505,11 @@ int qmm_rope_axes(const void* x, int dtype, size_t ldx, void* out, int out_dtype
 int qmm_kv_write_mxfp4(const void* k, size_t ldk, const void* v, size_t ldv, int dtype, const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, int rows,
                        void* stream);
 /* the values that the cache holds for these rows' tokens -> k and v (f32 or bf16, exact in both; row strides ldk, ldv): what
- * qmm_kv_write_mxfp4 was given, quantised.  cu of the whole sequences reads them whole. */
+ * qmm_kv_write_mxfp4 was given, quantised.  cu of the whole sequences reads them whole.  Rows whose token has no place in the table are left as they were. */
 int qmm_kv_read_mxfp4(const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, void* k, size_t ldk, void* v, size_t ldv, int dtype, int rows, void* stream);
 /* attention of up to 16 new rows a sequence over the cache (which holds their own keys and values): out[r][h] = sum_j w_j v_j / (sum_j w_j +
  * exp(sink)), w_j = exp(scale q[r][h] . k_j), over the keys that row r sees; no key (or scores of -inf alone): 0.
+ * Sums are f32 of weights up to 2^8: the largest value times the number of keys has to stay below 2^119.
  * q (16-byte aligned, ldq a multiple of 16 bytes) and out [rows][heads][dim], f32 or bf16 each, row
  * strides ldq, ldo; heads a multiple of the cache's, at most 16 times as many, successive heads sharing one.  max_rows (<= 16): the
  * most rows of a sequence, later ones are left as they were; max_len (<= 2^30): at least the longest lens[b] (later keys are not seen).  ws:

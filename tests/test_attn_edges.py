@@ -1,5 +1,6 @@
 """What attention's operators refuse before a device is asked: status codes of the library, and the checks of the Python mirror on stand-ins
 for device tensors.  No call below reaches a device."""
+import copy
 import ctypes
 
 import numpy as np
@@ -105,6 +106,13 @@ def test_prompt_refusals():
     assert need > 0 and f(rows=40, krows=9000, n=1, ws=D, wb=need - 1) == WORKSPACE and f(rows=40, krows=9000, n=1, ws=72, wb=need) == ARG
     for none in ((4000, 4000, 1, 32, 128), (40, 300, 1, 4, 64), (0, 9000, 1, 4, 64), (40, 9000, 0, 4, 64), (40, 9000, 1, 4, 80)):
         assert L.qmm_attn_prompt_ws_bytes(*none) == 0
+
+
+@pytest.mark.parametrize("scale,want", [(float("nan"), ARG), (float("inf"), ARG), (-float("inf"), ARG), (2.0 ** 101, ARG), (-2.0 ** 101, ARG)])
+def test_scales_that_are_refused(scale, want):
+    L = _lib.lib()
+    assert L.qmm_attn_kv_mxfp4(D, 1, 256, kvmx(), seqs(), Attn(None, scale, 0), D, 1, 256, 3, 4, 2, 64, D, BIG, None) == want
+    assert L.qmm_attn_prompt_bf16(D, 256, D, 128, D, 128, D, 256, D, D, 2, Attn(None, scale, 0), 3, 3, 4, 2, 64, None, 0, None) == want
 
 
 def test_rope_refusals():
@@ -223,6 +231,13 @@ def test_a_cache_is_checked_again_when_it_changed(launched):  # noqa: F811
     kv.kq.data_ptr = lambda: 4096
     with pytest.raises(QmmError, match="kv.kq"):
         f()
+
+
+def test_a_cache_can_be_copied_after_a_call():
+    kv = qmm.KVMXBuf(2, 16, 1, 64, device="cpu")
+    kv.held = (kv.c(), ())
+    kv2 = copy.deepcopy(kv)
+    assert kv2.held is None and kv2.pages == 2 and torch.equal(kv2.kq, kv.kq) and kv2.kq.data_ptr() != kv.kq.data_ptr()
 
 
 def test_python_checks_of_prompt_and_rope(launched):  # noqa: F811

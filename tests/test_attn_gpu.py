@@ -390,6 +390,29 @@ def test_attend_nan_reaches_those_that_see_it(gpu, D, qt):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
+@pytest.mark.parametrize("byte", [253, 254, 255])
+@pytest.mark.parametrize("qt", ["bf16", "f32"])
+def test_scale_bytes_past_bf16(gpu, byte, qt):
+    """They are NaN whatever the codes: in reads, and for the rows that see them; other rows keep their bits."""
+    g = torch.Generator().manual_seed(14)
+    lens, ms, D = [50], [4], 128
+    out, kv, table, q, _ = attend(g, lens, ms, 2, 2, D, 16, qt, qt, extra=0)
+    pg, at, want = int(table[0, 3]), 0, out.view(4, 2, D).clone()               # the key at 48: rows 2 and 3 see it
+    kv.ve[pg, 1, at, 2] = byte
+    want[2:, 1, 64:96] = float("nan")
+    got = attend(g, lens, ms, 2, 2, D, 16, qt, qt, kv=kv, table=table, q=q, extra=0)[0].view(4, 2, D)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    kv.ke[pg, 1, at, 0] = byte
+    want[2:, 1] = float("nan")
+    got = attend(g, lens, ms, 2, 2, D, 16, qt, qt, kv=kv, table=table, q=q, extra=0)[0].view(4, 2, D)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    ko, vo = torch.zeros(2, 4, 2, D, dtype=T[qt], device="cuda")
+    qmm.kv_read_mxfp4(kv, ints([0, 4]), ints(lens), table, ko, vo, 4)
+    nan = torch.zeros(2, 4, 2, D, dtype=torch.bool)
+    nan[0, 2, 1, :32] = nan[1, 2, 1, 64:96] = True
+    assert torch.equal(torch.stack([ko, vo]).isnan().cpu(), nan)
+
+
 def test_attend_page_outside_the_cache(gpu):
     """Its rows become NaN if they see the page, other sequences keep their bits."""
     g = torch.Generator().manual_seed(10)
@@ -617,6 +640,40 @@ def test_prompt_parts_not_finite(gpu):
     assert torch.equal(o.isnan(), w.isnan()) and torch.equal(o.isinf(), w.isinf())
     fin = w.isfinite()
     assert torch.equal(o[fin], w[fin])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_parts_without_weight(gpu, D):
+    """A NaN value at a key whose weight is 0 in 32 bits, which an earlier part alone has seen, is NaN as without parts."""
+    lens, n = [4000], 40
+    q = torch.ones(n, 2, D, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(4000, 1, D, dtype=torch.bfloat16, device="cuda")
+    k[3900:] = 8.0                                       # scores 32 sqrt(D) above the others': their weights are below 2^-369
+    v = torch.randn(4000, 1, D, generator=torch.Generator().manual_seed(15)).bfloat16().cuda()
+    v[70, 0, 3] = float("nan")
+    assert qmm.attn_prompt_ws_bytes(n, 4000, 1, 2, D) > 0
+    for w in (None, False):
+        out = torch.zeros(n, 2, D, dtype=torch.bfloat16, device="cuda")
+        qmm.attn_prompt_bf16(q, k, v, ints([0, n]), ints([0, 4000]), out, 2, 1, D, scale=4 * D ** -0.5, ws=w)
+        assert out[:, :, 3].isnan().all() and not torch.cat([out[:, :, :3], out[:, :, 4:]], 2).isnan().any(), w
+
+
+def test_prompt_workspace_of_another_stream(gpu):
+    """The workspace that is made for a call on another stream is not memory that the current stream's work still reads."""
+    lens, ms, D = [4600], [70], 64
+    out, q, k, v, _ = run_prompt(lens, ms, 4, 2, D)
+    size = qmm.attn_prompt_ws_bytes(q.shape[0], k.shape[0], 1, 4, D)
+    assert size > 0
+    cu, cuk, got = ints([0, 70]), ints([0, 4600]), torch.full_like(out, 3.0)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    t = torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+    torch.cuda._sleep(20_000_000)                        # some 10 ms
+    kept = t.clone()
+    del t
+    qmm.attn_prompt_bf16(q, k, v, cu, cuk, got, 4, 2, D, stream=st)
+    torch.cuda.synchronize()
+    assert (kept == 7).all() and torch.equal(got[:70], out[:70])
 
 
 # ---------------------------------------------------------------- together
