@@ -14,7 +14,9 @@
 //     of a step are does not matter as long as Q's operand has the same.
 //   - Values have to be turned (the second product sums over keys): a wave writes 32 keys' values as bf16 into LDS of its own and reads
 //     them back with the transposing read, four keys of 16 dims at a time.
-// The four waves of a workgroup take the chunk's steps of 32 keys in turn and join their (m, l, O) through LDS in order.
+// The waves of a workgroup take the chunk's steps of 32 keys in turn and join their (m, l, O) through LDS in order.
+//
+// 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 41.6 us and 4.8 for the join (loads alone 34); 700 keys of one 9.2 us.
 //
 // A chunk's length goes by max_len alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
@@ -217,7 +219,7 @@ template <int D>
 struct Step { Tile<D> k[2], v[2]; bool bad[2]; };      // bad: on a page outside the cache
 
 // WIDE: q in f32 as three bf16 that add up to it, P as three too.
-// Else q is bf16 and P rounded to it (2^-9 of a weight at most), as the output is.
+// Else q is bf16 and P rounded to it (2^-8 of a weight at most), as the output is.
 template <int D, int NT, bool WIDE, int NW>
 __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW / 4)) k_attn_kv(AttnArgs a) {
     constexpr int W = Tile<D>::W, QT = WIDE ? 3 : 1, DT = D / 16;
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
         else if (wanted(next + own1)) load(next + own1, odd);
     }
 
-    // the four waves' sums in order; lane (col, kg) has dims 16 d + 4 kg .. + 3 of row col
+    // the waves' sums in order; lane (col, kg) has dims 16 d + 4 kg .. + 3 of row col
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         lds_barrier();                                   // the values, or the rows before, are read

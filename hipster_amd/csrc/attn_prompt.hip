@@ -3,7 +3,7 @@
 //   k_attn_prompt   32 query rows a wave, keys and values in tiles of 64 through LDS
 //
 // Per row: t_j = scale log2(e) q . k_j, o = sum_j 2^(t_j - m) v_j / (sum_j 2^(t_j - m) + 2^(sink log2(e) - m)), in one pass over the keys
-// with the running maximum m.  Scores, weights, sums and outputs are f32; a weight is rounded to bf16 (2^-9 of it at most, as the output
+// with the running maximum m.  Scores, weights, sums and outputs are f32; a weight is rounded to bf16 (2^-8 of it at most, as the output
 // is) as a factor of the second product.
 //
 // Bound by the matrix units: 4 dim operations a visible pair.  Products run on the 32 x 32 x 16 bf16 instruction with keys as
@@ -11,9 +11,12 @@
 // one exchange with lane l ^ 32, and what the second product takes of P^T from a lane is just what it has, so P never leaves its
 // registers.  V^T is read from LDS by the transposing read, four keys of 16 dims at a time.
 //
-// Tiles come by DMA into one of two buffers while the other is worked on: one barrier a tile.  Lines of a tile's rows are permuted
-// (16-byte piece p of row r lies at p ^ (r % 8) for keys, p ^ 2 (r % 4) for values), so that eight rows' pieces, or four rows' pairs of
-// pieces, lie in different banks.
+// Tiles come by DMA into one of two buffers while the other is worked on: two barriers a tile.  Lines of a tile's rows are permuted
+// (key_turn, val_turn), so that what one instruction reads lies in different banks (counted: no conflicts).
+//
+// 8192 rows, 32 heads on 8 of 128 dims: 519 to 542 us (1010 to 1060 TFLOP/s; a library product of bf16 that is bound by the card's power
+// reaches 1250), LDS reads and DMAs 94 % of the LDS's cycles, matrix units busy 59 % of theirs at some 1.36 GHz.  2048 rows 51 us:
+// the last rows' chain of 32 tiles.
 #include "attn.hpp"
 
 #include <algorithm>
@@ -391,7 +394,7 @@ int64_t tiles_of(int rows, int nseq) { return nseq == 1 ? ((int64_t)rows + kRows
 
 // Parts that a tile's keys are cut into: one, or where that leaves half the CUs' room without work as many as fill it, of 16 tiles of
 // keys at least (an average row's; each part writes and reads its sums, 64 KB for 128 dims).  512 rows behind 7488 keys, 16 heads of
-// 256: one part 309 us, four 106; 1024 rows alone, 32 heads of 128, whose parts would be of 8 tiles: one 27, two 31.
+// 256: one part 309 us, four 91; 1024 rows alone, 32 heads of 128, whose parts would be of 8 tiles: one 27, two 31.
 int parts_of(int rows, int krows, int nseq, int heads, int dim) {
     const int64_t work = tiles_of(rows, nseq) * heads, room = (int64_t)device_cu_count() * (dim == 256 ? 1 : 2);
     const int64_t keys = std::max<int64_t>((int64_t)krows - rows / 2, 0) / nseq / kTile;
