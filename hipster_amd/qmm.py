@@ -656,17 +656,16 @@ def _at(t, n, dtype, dev, name):
 
 
 def _kv(kv, dev):
-    """The cache as the library takes it, checked when a tensor or a size of kv was set, or moved, or the current device is another."""
-    held = kv.held
-    if held is not None:
-        c, at = held[0], held[1]
-        if at == (kv.kq.data_ptr(), kv.ke.data_ptr(), kv.vq.data_ptr(), kv.ve.data_ptr(), dev):
-            return c
+    """The cache as the library takes it, made anew when one of its tensors or sizes was set, has moved or has another number of elements, or
+    the current device is another."""
+    kq, ke, vq, ve, held = kv.kq, kv.ke, kv.vq, kv.ve, kv.held
+    if held is not None and held[1] == (kq.data_ptr(), ke.data_ptr(), vq.data_ptr(), ve.data_ptr(), kq.numel(), ke.numel(), vq.numel(), ve.numel(), dev):
+        return held[0]
     tokens, u8 = kv.pages * kv.heads * kv.page, torch.uint8
     q, e = tokens * (kv.dim // 2), tokens * (kv.dim // 32)
-    p = (_at(kv.kq, q, u8, dev, "kv.kq"), _at(kv.ke, e, u8, dev, "kv.ke"), _at(kv.vq, q, u8, dev, "kv.vq"), _at(kv.ve, e, u8, dev, "kv.ve"))
+    p = (_at(kq, q, u8, dev, "kv.kq"), _at(ke, e, u8, dev, "kv.ke"), _at(vq, q, u8, dev, "kv.vq"), _at(ve, e, u8, dev, "kv.ve"))
     c = KVMX(*p, kv.pages, kv.page, kv.heads, kv.dim)
-    kv.held = (c, (*p, dev))
+    kv.held = (c, (*p, kq.numel(), ke.numel(), vq.numel(), ve.numel(), dev))
     return c
 
 

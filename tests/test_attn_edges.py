@@ -227,8 +227,7 @@ def test_a_cache_is_checked_again_when_it_changed(launched):  # noqa: F811
     kv.kq.data_ptr = lambda: 8192                                        # set in place
     f()
     assert launched[-1][1][5].kq == 8192
-    kv.kq.n = 1                                                          # and cut: seen when its address moves
-    kv.kq.data_ptr = lambda: 4096
+    kv.kq.n = 1                                                          # and cut where it lies
     with pytest.raises(QmmError, match="kv.kq"):
         f()
 
