@@ -18,7 +18,7 @@
 //
 // 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 41.6 us and 4.8 for the join (loads alone 34); 700 keys of one 9.2 us.
 //
-// A chunk's length goes by max_len alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
+// A chunk's length goes by max_len and the dims alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
 #include "attn.hpp"
 
@@ -598,13 +598,18 @@ __global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
 //   1 sequence of 2000 keys     9.9  12.1  16.5        1 of 30000 keys     19.7  16.8  18.8
 //   16 of 2000                 14.1  15.7  18.3        32 of 8000 to 500   49.9  47.0  44.5
 //   1 of 8000                  10.4  12.2  16.4        16 of 32000          120   111   107
-int chunk_of(int max_len) {
-    if (max_len <= 1024) return 1024;
-    int c = max_len <= 2048 ? 256 : 512;
+// With 256 dims a workgroup's own time counts for more (1 and 32 sequences, one chunk and chunks of 256: 300 keys 10.7, 11.0 and 12.7, 14.1;
+// 500 keys 13.3, 13.3 and 13.0, 14.3; 1000 keys 18.5, 18.7 and 13.0, 17.8): one chunk up to 512 keys, chunks of
+// 256 up to 4096 (1, 4, 16, 48 sequences of 3000 keys and fewer 13.2, 13.4, 24.9, 36.1, with chunks of 512 16.7, 16.9, 22.7, 38.0; with 128
+// dims 10.0, 11.7, 20.4, 33.9 and 12.2, 12.5, 17.7, 36.1, and drafted rows, which have more to join, lose more).
+int chunk_of(int max_len, int dim) {
+    const int one = dim == 256 ? 512 : 1024;
+    if (max_len <= one) return one;
+    int c = max_len <= (dim == 256 ? 4096 : 2048) ? 256 : 512;
     while ((int64_t)c * kChunks < max_len) c *= 2;
     return c;
 }
-int chunks_of(int max_len) { return (max_len + chunk_of(max_len) - 1) / chunk_of(max_len); }
+int chunks_of(int max_len, int dim) { return (max_len + chunk_of(max_len, dim) - 1) / chunk_of(max_len, dim); }
 
 // units of work at most, and the workgroups that are resident at once
 uint64_t units_of(const AttnArgs& a, int nt) { return (uint64_t)a.s.n * a.kv.heads * ((a.max_rows * a.share + 16 * nt - 1) / (16 * nt)) * a.chunks; }
@@ -668,7 +673,7 @@ extern "C" {
 
 size_t qmm_attn_kv_ws_bytes(int rows, int heads, int dim, int max_len) {
     if (rows <= 0 || heads <= 0 || max_len <= 0 || max_len > kMaxLen || (dim != 64 && dim != 128 && dim != 256)) return 0;
-    const int n = chunks_of(max_len);
+    const int n = chunks_of(max_len, dim);
     return n == 1 ? 0 : (size_t)rows * heads * n * (dim + 2) * sizeof(float);
 }
 
@@ -692,8 +697,8 @@ int qmm_attn_kv_mxfp4(const void* q, int q_dtype, size_t ldq, const qmm_kv_mxfp4
     a.q = q; a.out = out; a.kv = *kv; a.s = *seqs; a.sinks = attn->sinks; a.ldq = ldq; a.ldo = ldo;
     a.scale = (float)((double)attn->scale * 1.44269504088896340736);
     a.window = attn->window; a.rows = rows; a.heads = heads; a.share = heads / kv->heads; a.max_rows = max_rows; a.max_len = max_len;
-    a.chunk = chunk_of(max_len);
-    a.chunks = chunks_of(max_len);
+    a.chunk = chunk_of(max_len, kv->dim);
+    a.chunks = chunks_of(max_len, kv->dim);
     for (a.lgc = 0; 1 << a.lgc != a.chunk;) ++a.lgc;
     a.part = (float*)ws;
     a.ml = a.part + (need ? (size_t)rows * heads * a.chunks * kv->dim : 0);

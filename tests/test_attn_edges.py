@@ -87,6 +87,11 @@ def test_attend_workspace(max_len, chunks):
         assert qmm.attn_kv_ws_bytes(*bad) == 0
 
 
+@pytest.mark.parametrize("max_len,chunks", [(1, 1), (512, 1), (513, 3), (1024, 4), (4096, 16), (4097, 9), (1 << 30, 128)])
+def test_attend_workspace_of_256_dims(max_len, chunks):
+    assert qmm.attn_kv_ws_bytes(3, 4, 256, max_len) == (0 if chunks == 1 else 3 * 4 * chunks * 258 * 4)
+
+
 def test_prompt_refusals():
     L = _lib.lib()
 
