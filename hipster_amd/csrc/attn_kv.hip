@@ -632,7 +632,7 @@ int launch(AttnArgs& a, hipStream_t s) {
 }
 
 // Waves of a workgroup: four; eight where the keys are one chunk (few workgroups, whose own time counts) and registers leave room for two
-// waves a SIMD.  A row's bits follow from it, so this must not go by NT, which goes by the rows of a call.
+// waves a SIMD (700 keys of one sequence, 128 dims: 9.2 µs, with four 11.1).  A row's bits follow from it, so this must not go by NT, which goes by the rows of a call.
 constexpr bool eight(int D, bool wide) { return D < 256 || !wide; }
 template <int D, int NT, bool WIDE>
 int launch(AttnArgs& a, hipStream_t s) {

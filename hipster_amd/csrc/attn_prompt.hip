@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) k_attn_prompt(P
     // the last tiles first: they see the most keys
     const uint32_t id = blockIdx.x, turn = id / (uint32_t)a.heads;
     // Successive workgroups run on successive dies of eight, each with a cache of its own: a die gets successive heads, which share keys
-    // and values.
+    // and values (16 prompts of 1024 and fewer, 32 heads on 8 of 128: 121 us, heads in turn 124; 2048 rows 53.5 and 54.5; 256 dims 1 % slower).
     const int i8 = (int)(id - turn * a.heads), h = a.heads % 8 ? i8 : (i8 % 8) * (a.heads / 8) + i8 / 8, hk = h / a.share;
     const int part = (int)(turn % (uint32_t)a.parts), t = a.tiles - 1 - (int)(turn / (uint32_t)a.parts);
     Tiled w;
