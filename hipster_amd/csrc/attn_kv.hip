@@ -201,13 +201,19 @@ struct Tile {
 
     __device__ __forceinline__ void load(const uint8_t* __restrict__ q, const uint8_t* __restrict__ se, size_t token, int kg) {
         const uint8_t* p = q + token * (D / 2);
-        const uint8_t* s = se + token * (D / 32);
+        const uint8_t* s = se + (D == 64 ? token & ~(size_t)1 : token) * (D / 32);        // D = 64: a word is two keys' bytes
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             c[i] = *(const Codes*)(p + i * 64 + kg * (4 * V));
-            e[i] = s[D == 64 ? kg / 2 : i * 4 + kg];
+            e[i] = *(const uint32_t*)(s + 4 * i);
         }
     }
+    // to the lane's scale bytes from the words that hold them
+    __device__ __forceinline__ void open(int shift) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) e[i] = __builtin_amdgcn_ubfe(e[i], (uint32_t)shift, 8);
+    }
+    static __device__ __forceinline__ int shift(int col, int kg) { return D == 64 ? 16 * (col & 1) + 8 * (kg / 2) : 8 * kg; }
 };
 
 // workgroups of a CU (waves of a SIMD) that the registers are cut for
@@ -317,38 +323,50 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
     const uint32_t v_from = (uint32_t)v_row * (2 * D) + ((uint32_t)((col >> 1) & 1) ^ v_turn<D>(v_row)) * 16 + 8 * (col & 1);
     const int* const table = a.s.table + (size_t)b * a.s.ld;
     int block = -1, entry = 0;                           // lane l: the page of the 16 keys from 1024 block + 16 l on
+    auto wanted = [&](int key0) { return key0 <= kmax && key0 + kStep > kmin; };
     auto load = [&](int key0, Step<D>& st) {             // the step of the 32 keys from key0 on
         if ((key0 >> 10) != block) {
             block = key0 >> 10;
             const int pg = ((block << 10) + lane * 16) >> a.lg;
-            entry = pg < a.s.ld ? table[pg] : -1;
+            entry = -1;
+            if (pg < a.s.ld) entry = table[pg];
+            entry = (int)opaque((uint32_t)entry);        // waited for here, not at each of its uses
         }
+        size_t token[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int k0 = key0 + 16 * t;
             int page = __builtin_amdgcn_readlane(entry, (k0 >> 4) & 63);
             const bool bad = (unsigned)page >= (unsigned)a.kv.pages;
             page = bad ? 0 : page;
-            const size_t token = ((size_t)page * a.kv.heads + hk) * a.kv.page + (k0 & (a.kv.page - 1)) + col;
-            st.k[t].load(a.kv.kq, a.kv.ke, token, kg);
-            st.v[t].load(a.kv.vq, a.kv.ve, token, kg);
+            token[t] = ((size_t)page * a.kv.heads + hk) * a.kv.page + (k0 & (a.kv.page - 1)) + col;
             st.bad[t] = bad;
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) st.v[t].load(a.kv.vq, a.kv.ve, token[t], kg);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) st.k[t].load(a.kv.kq, a.kv.ke, token[t], kg);
     };
 
     // Steps go round the waves; of a block of 256 keys a wave has two, each with a buffer of its own, which is filled again for the next
-    // block as soon as its codes are converted: two steps are under way.
+    // block as soon as its codes are converted: two steps are under way.  A buffer is filled in one place, with words (a byte's extension is
+    // work on it), and the pages' load is waited for where it is made, so that no wait of the compiler's is for the other buffer too (16
+    // sequences of up to 32000 keys 111 -> 107 us).
     constexpr int kBlock = 2 * kStep * NW;
     const int blocks = a.chunk / kBlock;                 // of a chunk
     const int b0 = max(cfirst * blocks, kmin / kBlock), b1 = kmax < 0 ? -1 : min((clast + 1) * blocks - 1, kmax / kBlock);
-    auto wanted = [&](int key0) { return key0 <= kmax && key0 + kStep > kmin; };
     auto step = [&](int key0, Step<D>& st, int after) {
         const bool inside = key0 >= kmin && key0 + kStep - 1 <= kmax;        // every key is seen by a row: none is other memory
         const bool all = key0 >= lmax && key0 + kStep - 1 <= hmin;           // every row sees every key
         // values whose scale is NaN, and keys that no row sees: out of the products
         unsigned long long nan[2][Tile<D>::S], any = 0;
+        const bool want = wanted(key0);
+        mx_v4f sc[NT][2];
+        if (want) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            st.v[t].open(Tile<D>::shift(col, kg));
+            st.k[t].open(Tile<D>::shift(col, kg));
             if (!inside) {
                 const int key = key0 + 16 * t + col;
                 if (key < kmin || key > kmax) {
@@ -387,7 +405,6 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
             for (int w = 0; w < W; ++w)
                 *(uint4*)(own + 16 * t * (2 * D) + (to ^ (Tile<D>::dim(w, 0) * 2))) = fp4x8(st.v[t].word(w), st.v[t].scale(w));
         // scores
-        mx_v4f sc[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = mx_v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -400,7 +417,9 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
 #pragma unroll
                     for (int p = 0; p < QT; ++p) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][w][p], sc[n][t], 0, 0, 0);
             }
+        }
         if (wanted(after)) load(after, st);
+        if (!want) return;
         at_bf8 pf[NT][QT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -474,10 +493,8 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
 
     Step<D> even, odd;
     const int own0 = kStep * wave, own1 = own0 + kStep * NW;             // its steps of a block
-    if (b0 <= b1) {
-        if (wanted(b0 * kBlock + own0)) load(b0 * kBlock + own0, even);
-        if (wanted(b0 * kBlock + own1)) load(b0 * kBlock + own1, odd);
-    }
+    if (wanted(b0 * kBlock + own0)) load(b0 * kBlock + own0, even);
+    if (wanted(b0 * kBlock + own1)) load(b0 * kBlock + own1, odd);
     for (int chunk = cfirst, blk = b0; chunk <= clast; ++chunk) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -488,10 +505,8 @@ __global__ void __launch_bounds__(64 * NW, occupancy(D, NT, WIDE) * 4 / NW * (NW
     }
     for (const int end = min((chunk + 1) * blocks - 1, b1); blk <= end; ++blk) {
         const int k0 = blk * kBlock, next = blk < b1 ? k0 + kBlock : kNone;
-        if (wanted(k0 + own0)) step(k0 + own0, even, next + own0);
-        else if (wanted(next + own0)) load(next + own0, even);
-        if (wanted(k0 + own1)) step(k0 + own1, odd, next + own1);
-        else if (wanted(next + own1)) load(next + own1, odd);
+        step(k0 + own0, even, next + own0);
+        step(k0 + own1, odd, next + own1);
     }
 
     // the waves' sums in order; lane (col, kg) has dims 16 d + 4 kg .. + 3 of row col
