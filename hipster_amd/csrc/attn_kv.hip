@@ -16,7 +16,7 @@
 //     them back with the transposing read, four keys of 16 dims at a time.
 // The waves of a workgroup take the chunk's steps of 32 keys in turn and join their (m, l, O) through LDS in order.
 //
-// 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 41.6 us and 4.8 for the join (loads alone 34); 700 keys of one 9.2 us.
+// 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 45 us with the join's 4.8 (loads alone 34 and the join); 700 keys of one 9.2 us.
 //
 // A chunk's length goes by max_len and the dims alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
