@@ -656,10 +656,11 @@ def _at(t, n, dtype, dev, name):
 
 
 def _kv(kv, dev):
-    """The cache as the library takes it, made anew when one of its tensors or sizes was set, has moved or has another number of elements, or
-    the current device is another."""
+    """The cache as the library takes it, made anew when one of its tensors or sizes was set, has moved, was turned in place or has another
+    number of elements, or the current device is another."""
     kq, ke, vq, ve, held = kv.kq, kv.ke, kv.vq, kv.ve, kv.held
-    if held is not None and held[1] == (kq.data_ptr(), ke.data_ptr(), vq.data_ptr(), ve.data_ptr(), kq.numel(), ke.numel(), vq.numel(), ve.numel(), dev):
+    if (held is not None and held[1] == (kq.data_ptr(), ke.data_ptr(), vq.data_ptr(), ve.data_ptr(), kq.numel(), ke.numel(), vq.numel(), ve.numel(), dev)
+            and kq.is_contiguous() and ke.is_contiguous() and vq.is_contiguous() and ve.is_contiguous()):
         return held[0]
     tokens, u8 = kv.pages * kv.heads * kv.page, torch.uint8
     q, e = tokens * (kv.dim // 2), tokens * (kv.dim // 32)
