@@ -395,11 +395,26 @@ int64_t tiles_of(int rows, int nseq) { return nseq == 1 ? ((int64_t)rows + kRows
 // Parts that a tile's keys are cut into: one, or where that leaves half the CUs' room without work as many as fill it, of 16 tiles of
 // keys at least (an average row's; each part writes and reads its sums, 64 KB for 128 dims).  512 rows behind 7488 keys, 16 heads of
 // 256: one part 309 us, four 91; 1024 rows alone, 32 heads of 128, whose parts would be of 8 tiles: one 27, two 31.
-int parts_of(int rows, int krows, int nseq, int heads, int dim) {
+// A window leaves a tile of rows window + 127 keys, however many there are.  Below 8 tiles of window (4 of 256 dims, whose tile takes
+// twice the time) they stay one part, above parts are of two tiles at least.  In us with one part and with the parts that the keys' number
+// would make, at windows of
+//                                                            128          256          512         1024         2048
+//   128 rows, 8000 keys, 32 heads of 128, 7 parts        12.6  17.3   15.1  20.0   19.3  20.0   27.5  22.8   44.5  27.2
+//   512 rows of them, 4 parts                            13.1  30.9   15.6  30.5   19.6  31.3   28.0  34.9   45.2  40.5
+//   64 rows, 16000 keys, 8 heads of 64, 8 parts           7.3  11.6    8.9  12.5   12.0  13.3   18.5  14.6   31.0  16.5
+//   512 rows, 8000 keys, 16 heads of 256, 4 parts        21.7  31.8   26.4  31.3   34.5  35.0   51.1  38.0   84.2  46.4
+int parts_of(int rows, int krows, int nseq, int heads, int dim, int window) {
     const int64_t work = tiles_of(rows, nseq) * heads, room = (int64_t)device_cu_count() * (dim == 256 ? 1 : 2);
     const int64_t keys = std::max<int64_t>((int64_t)krows - rows / 2, 0) / nseq / kTile;
-    return (int)std::max<int64_t>(std::min<int64_t>({room / std::max<int64_t>(work, 1), keys / 16, kParts}), 1);
+    int64_t parts = std::min<int64_t>({room / std::max<int64_t>(work, 1), keys / 16, kParts});
+    if (window > 0) {
+        const int64_t seen = ((int64_t)window + kRows - 1 + kTile - 1) / kTile;          // tiles of keys
+        parts = window < (dim == 256 ? 4 : 8) * kTile ? 1 : std::min(parts, seen / 2);
+    }
+    return (int)std::max<int64_t>(parts, 1);
 }
+
+size_t ws_of(int64_t tiles, int heads, int parts, int dim) { return parts == 1 ? 0 : (size_t)tiles * heads * parts * kRows * (dim + 2) * sizeof(float); }
 
 template <int D>
 int launch(PromptArgs& a, hipStream_t s) {
@@ -424,8 +439,7 @@ extern "C" {
 
 size_t qmm_attn_prompt_ws_bytes(int rows, int krows, int nseq, int heads, int dim) {
     if (rows <= 0 || krows <= 0 || nseq <= 0 || heads <= 0 || (dim != 64 && dim != 128 && dim != 256)) return 0;
-    const int p = parts_of(rows, krows, nseq, heads, dim);
-    return p == 1 ? 0 : (size_t)tiles_of(rows, nseq) * heads * p * kRows * (dim + 2) * sizeof(float);
+    return ws_of(tiles_of(rows, nseq), heads, parts_of(rows, krows, nseq, heads, dim, 0), dim);      // of all windows the most
 }
 
 int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
@@ -449,10 +463,9 @@ int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_
     a.scale = fmaxf((float)(fabs((double)attn->scale) * 1.44269504088896340736), 0x1p-126f);
     a.flip = attn->scale < 0.f ? 0x80008000u : 0u;
     a.n = nseq; a.window = attn->window; a.rows = rows; a.krows = krows; a.heads = heads; a.share = heads / kv_heads; a.tiles = (int)tiles;
-    const size_t need = qmm_attn_prompt_ws_bytes(rows, krows, nseq, heads, dim);
-    a.parts = ws ? parts_of(rows, krows, nseq, heads, dim) : 1;
+    a.parts = ws ? parts_of(rows, krows, nseq, heads, dim, attn->window) : 1;
     if (a.parts > 1) {
-        if (ws_bytes < need) return QMM_ERR_WORKSPACE;
+        if (ws_bytes < ws_of(tiles, heads, a.parts, dim)) return QMM_ERR_WORKSPACE;
         if (!aligned(ws, 16)) return QMM_ERR_ARG;
         a.part = (float*)ws;
         a.ml = (float2*)(a.part + (size_t)tiles * heads * a.parts * kRows * dim);

@@ -525,11 +525,11 @@ size_t qmm_attn_kv_ws_bytes(int rows, int heads, int dim, int max_len);
  * (cuk NULL: cuq); of m rows and n keys, row i is at position n - m + i.  The formula of qmm_attn_kv_mxfp4; dim 64, 128 or 256; heads
  * a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were.
  * ws: qmm_attn_prompt_ws_bytes(...) bytes, 16-byte aligned, for calls with few rows and many keys, whose keys are then cut into parts
- * that are joined (the bits are others); NULL: no parts.  Calls that overlap need one each. */
+ * that are joined (the bits are others; a small window is never cut); NULL: no parts.  Calls that overlap need one each. */
 int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
                          const int32_t* cuq, const int32_t* cuk, int nseq, const qmm_attn* attn, int rows, int krows, int heads, int kv_heads, int dim,
                          void* ws, size_t ws_bytes, void* stream);
-/* bytes of its workspace (0: it would use none) */
+/* bytes of its workspace, enough for any window (0: it would use none) */
 size_t qmm_attn_prompt_ws_bytes(int rows, int krows, int nseq, int heads, int dim);
 
 #ifdef __cplusplus
