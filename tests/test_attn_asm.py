@@ -85,3 +85,11 @@ def test_no_scratch(asm):
     name, lines = asm
     sizes = [int(l.split(":")[1]) for l in lines if l.startswith(".private_segment_fixed_size:")]
     assert sizes and max(sizes) <= 64, sizes
+
+
+def test_all_state_is_in_registers(asm):
+    """No kernel has a private segment, nor a spilled register."""
+    name, lines = asm
+    sizes, spills = ([int(l.split(":")[1]) for l in lines if l.startswith(x)] for x in (".private_segment_fixed_size:", ".vgpr_spill_count:"))
+    assert len(sizes) == len(spills) == {"attn_prompt.hip": 6, "attn_kv.hip": 26}[name]
+    assert max(sizes) == 0 and max(spills) == 0, (sizes, spills)
