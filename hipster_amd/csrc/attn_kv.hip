@@ -16,7 +16,11 @@
 //     them back with the transposing read, four keys of 16 dims at a time.
 // The waves of a workgroup take the chunk's steps of 32 keys in turn and join their (m, l, O) through LDS in order.
 //
-// 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 45 us with the join's 4.8 (loads alone 34 and the join); 700 keys of one 9.2 us.
+// 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 50 us with the join's 4.8 on caches in turn, 45 on one again and again, which
+// the last-level cache holds (as in all the times below; loads alone then 34 and the join).  700 keys of one sequence 9.2 us.
+// The join of a workgroup's waves after each chunk, with the sums it writes, takes 5.5 of these us (44.4 traced, without it 38.9), and 8.3 of 44.0 where 16
+// such sequences check 8 drafted rows each, 64 heads on 8 of 64 dims.  That one is bound by vector instructions: 387 of a wave for 32 keys
+// and 64 rows (codes 40, the rest the softmax of four groups of rows) and 88 of the waves' join, 59 % of a SIMD's cycles with two waves on it.
 //
 // A chunk's length goes by max_len and the dims alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
@@ -617,6 +621,10 @@ __global__ void __launch_bounds__(64) k_attn_join(AttnArgs a) {
 // 500 keys 13.3, 13.3 and 13.0, 14.3; 1000 keys 18.5, 18.7 and 13.0, 17.8): one chunk up to 512 keys, chunks of
 // 256 up to 4096 (1, 4, 16, 48 sequences of 3000 keys and fewer 13.2, 13.4, 24.9, 36.1, with chunks of 512 16.7, 16.9, 22.7, 38.0; with 128
 // dims 10.0, 11.7, 20.4, 33.9 and 12.2, 12.5, 17.7, 36.1, and drafted rows, which have more to join, lose more).
+// It goes by max_len, not by the lengths, which the host does not know, nor by the window.  So a capacity far above the lengths costs: one
+// sequence of 128 dims with max_len 131072 and its own length, 700 keys 14.4 and 9.3, 2000 keys 16.8 and 9.9, 8192 keys 17.7 and 12.2.  And a
+// window has the chunks of max_len and their join: of 8192 keys a window of 128, with max_len 8192 and 131072, 8.6 and 8.9 (128 keys in one chunk 5.6),
+// of 1024 12.0 and 16.6; 32 such sequences 9.8 and 9.8 (5.8), 15.8 and 18.5.
 int chunk_of(int max_len, int dim) {
     const int one = dim == 256 ? 512 : 1024;
     if (max_len <= one) return one;

@@ -4,9 +4,11 @@
 //
 // Per row: t_j = scale log2(e) q . k_j, o = sum_j 2^(t_j - m) v_j / (sum_j 2^(t_j - m) + 2^(sink log2(e) - m)), in one pass over the keys
 // with the running maximum m.  Scores, weights, sums and outputs are f32; a weight is rounded to bf16 (2^-8 of it at most, as the output
-// is) as a factor of the second product.
+// is) as a factor of the second product, the sum of weights takes them unrounded.  Against 64 bits an output is off by 0.0019 to 0.0023 of its
+// size, where weights in f32 give 0.0016 to 0.0017 (its own rounding to bf16 among both); weights of more bits would take two or
+// three products for one.
 //
-// Bound by the matrix units: 4 dim operations a visible pair.  Products run on the 32 x 32 x 16 bf16 instruction with keys as
+// The floor is the matrix units': 4 dim operations a visible pair.  Products run on the 32 x 32 x 16 bf16 instruction with keys as
 // rows: S^T = K Q^T, O^T = V^T P^T.  A lane of S^T holds 16 of 32 keys of one query row: the row's maximum and sum are its own registers and
 // one exchange with lane l ^ 32, and what the second product takes of P^T from a lane is just what it has, so P never leaves its
 // registers.  V^T is read from LDS by the transposing read, four keys of 16 dims at a time.
@@ -14,9 +16,12 @@
 // Tiles come by DMA into one of two buffers while the other is worked on: two barriers a tile.  Lines of a tile's rows are permuted
 // (key_turn, val_turn), so that what one instruction reads lies in different banks (counted: no conflicts).
 //
-// 8192 rows, 32 heads on 8 of 128 dims: 519 to 542 us (1010 to 1060 TFLOP/s; a library product of bf16 that is bound by the card's power
-// reaches 1250), LDS reads and DMAs 94 % of the LDS's cycles, matrix units busy 59 % of theirs at some 1.36 GHz.  2048 rows 51 us:
-// the last rows' chain of 32 tiles.
+// 8192 rows, 32 heads on 8 of 128 dims: 519 to 547 us (1005 to 1060 TFLOP/s; a library product of bf16 that is bound by the card's power
+// reaches 1250).  Counted: a CU is busy for 906 000 cycles whatever the time (launches of 547 to 616 us: the clock falls from 1.8 to 1.55 GHz
+// under load), 3480 for a tile of both its workgroups.  Of a SIMD's the matrix unit takes 2048 (59 %) and vector instructions 2120
+// (61 %): neither is full, as two waves a SIMD with two barriers a tile leave both waiting.  64 dims, 64 heads 631 us: vector instructions 88 %,
+// matrix unit 49 %, so bound by the softmax, as much a pair for half the products.  256 dims, 16 heads 622 to 637 us: 41 and 39 %, one
+// wave a SIMD does one mostly after the other.  2048 rows of 128 dims 50 to 55 us: the last rows' chain of 32 tiles.
 #include "attn.hpp"
 
 #include <algorithm>

@@ -748,7 +748,7 @@ def kv_read_mxfp4(kv, cu, lens, table, k, v, rows, stream=None):
 
 
 def attn_kv_ws_bytes(rows, heads, dim, max_len):
-    """Bytes of attn_kv_mxfp4's workspace (0: it needs none)."""
+    """Bytes of attn_kv_mxfp4's workspace (0: it needs none): every row and head has room for up to 128 chunks of the keys up to max_len."""
     return _lib.lib().qmm_attn_kv_ws_bytes(rows, heads, dim, max_len)
 
 
@@ -761,7 +761,8 @@ def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, w
 
     q, out: `rows` rows of heads * kv.dim values, f32 or bf16 each; heads / kv.heads (<= 16) successive heads share one of the cache;
     max_len: at least the longest of lens; ws: a uint8 tensor of attn_kv_ws_bytes(rows, heads, kv.dim, max_len) bytes (None where that
-    is 0); scale None: dim ** -0.5; window: keys a row sees with its own (0: all); sinks f32 [heads]: a logit beside the keys'."""
+    is 0); scale None: dim ** -0.5; window: keys a row sees with its own (0: all); sinks f32 [heads]: a logit beside the keys'.  Where q and
+    out are bf16, weights are rounded to bf16 as factors of their products with the values."""
     dev, dim = _device(), kv.dim
     ldq, ldo = _heads(q, rows, heads, dim, dev, "q"), _heads(out, rows, heads, dim, dev, "out")
     check(_lib.lib().qmm_attn_kv_mxfp4(q.data_ptr(), _dtype(q, "q"), ldq, _kv(kv, dev), _seqs(cu, lens, table, dev), _attn(scale, dim, window, sinks, heads, dev),
@@ -771,7 +772,7 @@ def attn_kv_mxfp4(q, kv, cu, lens, table, out, rows, heads, max_rows, max_len, w
 
 
 def attn_prompt_ws_bytes(rows, krows, nseq, heads, dim):
-    """Bytes of attn_prompt_bf16's workspace (0: it needs none)."""
+    """Bytes of attn_prompt_bf16's workspace, enough for any window (0: it needs none)."""
     return _lib.lib().qmm_attn_prompt_ws_bytes(rows, krows, nseq, heads, dim)
 
 
@@ -779,7 +780,7 @@ def attn_prompt_bf16(q, k, v, cu_q, cu_k, out, heads, kv_heads, dim, scale=None,
     """Causal attention of packed sequences: rows cu_q[b] .. cu_q[b + 1] - 1 of q, the last ones of the tokens cu_k[b] .. cu_k[b + 1] - 1
     of k and v (cu_k None: cu_q).  q, out rows of heads * dim values, k, v of kv_heads * dim, all bf16 (row strides multiples of 8);
     scale, window and sinks as in attn_kv_mxfp4.  ws: a uint8 tensor of attn_prompt_ws_bytes(...) bytes; None: torch's allocator gives one
-    where few rows see many keys (False: none, the keys stay in one part)."""
+    where few rows see many keys (False: none, the keys stay in one part).  Weights are rounded to bf16 as factors of their products with v."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         if t.dtype is not torch.bfloat16:
             raise QmmError(f"{name} must be torch.bfloat16, got {t.dtype}")

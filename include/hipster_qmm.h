@@ -514,16 +514,18 @@ int qmm_kv_read_mxfp4(const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, void* k, siz
  * strides ldq, ldo; heads a multiple of the cache's, at most 16 times as many, successive heads sharing one.  max_rows (<= 16): the
  * most rows of a sequence, later ones are left as they were; max_len (<= 2^30): at least the longest lens[b] (later keys are not seen).  ws:
  * qmm_attn_kv_ws_bytes(...) bytes, 16-byte aligned; calls that overlap need one each, calls one after another may share it.
+ * Where q and out are bf16 a weight is rounded to bf16 (by 2^-8 of it at most) as a factor of its product with v_j; the sum of weights takes it unrounded.
  * A row's bits depend on q, its sequence, max_len and whether q or out is f32 (then the matrix products carry more bits): not
  * on the other sequences or rows of the call. */
 int qmm_attn_kv_mxfp4(const void* q, int q_dtype, size_t ldq, const qmm_kv_mxfp4* kv, const qmm_seqs* seqs, const qmm_attn* attn, void* out,
                       int out_dtype, size_t ldo, int rows, int heads, int max_rows, int max_len, void* ws, size_t ws_bytes, void* stream);
-/* bytes of its workspace (0: nothing needed, or a size out of range) */
+/* bytes of its workspace (0: nothing needed, or a size out of range): rows * heads * chunks * (dim + 2) * 4, up to 128 chunks of the keys up to
+ * max_len, whatever the lengths and the window are.  64 rows of 64 heads of 128 dims at max_len 131072: 273 MB; 16 drafted rows of each: 4.4 GB. */
 size_t qmm_attn_kv_ws_bytes(int rows, int heads, int dim, int max_len);
 /* causal attention of packed sequences, bf16: q and out [rows][heads][dim], k and v [krows][kv_heads][dim] with row strides in values
  * (multiples of 8, 16-byte aligned).  Sequence b has the q rows cuq[b] .. cuq[b + 1] - 1 and the keys cuk[b] .. cuk[b + 1] - 1
- * (cuk NULL: cuq); of m rows and n keys, row i is at position n - m + i.  The formula of qmm_attn_kv_mxfp4; dim 64, 128 or 256; heads
- * a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were.
+ * (cuk NULL: cuq); of m rows and n keys, row i is at position n - m + i.  The formula of qmm_attn_kv_mxfp4 and its limit on values, weights
+ * rounded to bf16 as there; dim 64, 128 or 256; heads a multiple of kv_heads.  Offsets are kept within rows and krows.  q rows from cuq[nseq] on are left as they were.
  * ws: qmm_attn_prompt_ws_bytes(...) bytes, 16-byte aligned, for calls with few rows and many keys, whose keys are then cut into parts
  * that are joined (the bits are others; a small window is never cut); NULL: no parts.  Calls that overlap need one each. */
 int qmm_attn_prompt_bf16(const uint16_t* q, size_t ldq, const uint16_t* k, size_t ldk, const uint16_t* v, size_t ldv, uint16_t* out, size_t ldo,
