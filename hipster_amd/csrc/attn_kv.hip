@@ -19,8 +19,8 @@
 // 32 heads on 8 of 128 dims, 32 sequences of up to 8192 keys, 180 MB: 50 us with the join's 4.8 on caches in turn, 45 on one again and again, which
 // the last-level cache holds (as in all the times below; loads alone then 34 and the join).  700 keys of one sequence 9.2 us.
 // The join of a workgroup's waves after each chunk, with the sums it writes, takes 5.5 of these us (44.4 traced, without it 38.9), and 8.3 of 44.0 where 16
-// such sequences check 8 drafted rows each, 64 heads on 8 of 64 dims.  That one is bound by vector instructions: 387 of a wave for 32 keys
-// and 64 rows (codes 40, the rest the softmax of four groups of rows) and 88 of the waves' join, 59 % of a SIMD's cycles with two waves on it.
+// such sequences check 8 drafted rows each, 64 heads on 8 of 64 dims.  The larger part there is vector instructions: 387 of a wave for 32
+// keys and 64 rows (codes 40, the rest the softmax of four groups of rows) and 88 of the waves' join, 59 % of a SIMD's cycles with two waves on it.
 //
 // A chunk's length goes by max_len and the dims alone, its steps lie at fixed multiples of 32 keys, and keys that a row does not see add exact
 // zeros.  So a row's bits do not depend on the other rows and sequences: a draft's rows checked together are what one by one gives.
